@@ -15,6 +15,7 @@ m' = b1 m + (1 - b1) g and v' = b2 v + (1 - b2) g^2 (products and sums rounded o
   rounding          the float's 20 surplus bits plus a random number r < 2^20 carry into the code (stochastic rounding);
                     x = 32-bit mix of (seed, step, tensor, block, element), r_m = 16 (x >> 16) + 8, r_v = 16 (x & 65535) + 8
 """
+import itertools
 import math
 
 import torch
@@ -74,8 +75,8 @@ def _tensors(case):
     if case["layout"] == "gaussians":
         return [(n * k, lr, 0.0, c, s, g) for k, lr, c, s, g in GAUSSIAN_GROUPS]
     if case["layout"] == "net":  # per layer four square matrices, two four times as wide, two vectors (not decayed)
-        layer = [(n * n, 3e-4, 0.1, 0.0, 0.02, 1e-3)] * 4 + [(4 * n * n, 3e-4, 0.1, 0.0, 0.02, 1e-3)] * 2 + [(n, 3e-4, 0.0, 1.0, 0.02, 1e-2)] * 2
-        return layer * case["layers"]
+        square, wide, vector = ((k, 3e-4, wd, c, 0.02, g) for k, wd, c, g in ((n * n, 0.1, 0.0, 1e-3), (4 * n * n, 0.1, 0.0, 1e-3), (n, 0.0, 1.0, 1e-2)))
+        return ([square] * 4 + [wide] * 2) * case["layers"] + [vector] * 2 * case["layers"]
     if case["layout"] == "ragged":  # 1, 3, odd and even sizes to about 300 000
         return [(1 + (7919 * i * i + 13 * i) % 300007 if i > 2 else (1, 3, 257)[i], 1e-3, 0.01, 0.0, 0.5, 1e-2) for i in range(n)]
     return [(n, 1e-3, 0.01, 0.0, 0.02, 1e-4)]
@@ -150,7 +151,8 @@ def prepare(case, seed):
     if own:
         from vcr_gaus_amd.optim import AdamW
         params = [torch.nn.Parameter(t) for t in view(s["p"])]
-        s["opt"] = AdamW([dict(params=[p], lr=t[1], weight_decay=t[2]) for p, t in zip(params, spec)], betas=BETAS, eps=_eps(case),
+        s["opt"] = AdamW([dict(params=[p for p, _ in of], lr=rates[0], weight_decay=rates[1])
+                          for rates, of in itertools.groupby(zip(params, spec), key=lambda x: x[1][1:3])], betas=BETAS, eps=_eps(case),
                          state_bits=case["bits"], master_weights=case["master"], seed=SEED)
         bits8 = case["bits"] == 8
         cut = lambda f: [f[a // BLOCK:a // BLOCK + b] for a, b in zip(starts, blocks)]  # noqa: E731
