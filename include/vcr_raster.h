@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define VCR_ABI_VERSION 19
+#define VCR_ABI_VERSION 20
 
 /* Buffers whose size depends on the number of tile instances R are obtained through this callback
  * (the Python shim backs it with torch's caching allocator, so no hipMalloc on the hot path).
@@ -251,6 +251,65 @@ int vcr_knn3_mean_dist2(int N, const float* points, float* out, void* stream);
 int vcr_adam_step(int ntensors, float* const* params, const float* const* grads, float* const* exp_avg,
                   float* const* exp_avg_sq, const int64_t* numel, const float* lr, float beta1, float beta2,
                   float eps, int step, float grad_scale, void* stream);
+/* ---- optimizer over many tensors at once: AdamW with the moments in 32 or in 8 bits, gradient norm and clipping ------------
+ * A PLAN holds what stays from step to step: one record per tensor and the map from workgroups to tensors.  It is built on the
+ * host (vcr_optim_plan) and copied to the device by the caller; the gradients' addresses come with every call. */
+#define VCR_F32 0
+#define VCR_BF16 1
+#define VCR_F16 2
+typedef struct VcrOptimTensor {
+    void* p;                  /* parameter, numel elements of the call's param_type; any alignment its type allows */
+    float* master;            /* fp32 copy that the update works on (16-bit parameters with masters), else NULL */
+    void* m;                  /* first moment: fp32, or uint8 codes */
+    void* v;                  /* second moment: fp32, or uint8 codes */
+    uint8_t* m_scale;         /* 8 bits: one exponent per 256 elements, ceil(numel / 256) bytes; 32 bits: NULL */
+    uint8_t* v_scale;
+    int32_t* step;            /* device counter: steps taken */
+    int64_t numel;
+    int32_t group;            /* index into VcrAdamWStep.groups */
+    int32_t index;            /* the tensor's number in the random sequence of the 8-bit moments */
+} VcrOptimTensor;
+typedef struct VcrOptimGroup {
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* lr_dev;      /* device scalar used instead of lr (a captured step whose rate changes), or NULL */
+} VcrOptimGroup;
+typedef struct VcrAdamWStep {
+    int32_t ntensors, ngroups;
+    int32_t chunk;            /* elements per workgroup: a multiple of 1024, the plan's */
+    int32_t param_type;       /* VCR_F32 / VCR_BF16 / VCR_F16, of parameters and gradients alike */
+    int32_t state_bits;       /* 32 or 8 */
+    int32_t masters;          /* != 0: 16-bit parameters with fp32 masters */
+    uint32_t seed;            /* of the stochastic rounding of 8-bit moments */
+    int32_t npartials;        /* > 0: clip by max_norm / skip the step when the norm is not finite */
+    const void* plan;         /* device */
+    const void* const* grads; /* HOST array of device pointers; NULL = this tensor is not stepped */
+    const int64_t* numel;     /* HOST, as in the plan */
+    const VcrOptimGroup* groups; /* HOST */
+    double grad_scale;        /* multiplies every gradient (1 / world after a sum all-reduce, 1 / loss scale) */
+    double max_norm;
+    const double* partials;   /* device, from vcr_grad_norm_accumulate over ALL gradients of the step */
+    float* norm_out;          /* device scalar: norm of grad * grad_scale, or NULL */
+    void* work;               /* device, vcr_adamw_work_bytes(ntensors), 16-byte aligned */
+} VcrAdamWStep;
+size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel, int chunk);
+int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, int chunk, void* host_plan, size_t bytes);
+size_t vcr_adamw_work_bytes(int ntensors);
+/* One AdamW step (decoupled weight decay, torch.optim.AdamW's arithmetic) on every tensor with a gradient; see csrc/optim.hip. */
+int vcr_adamw_step(const VcrAdamWStep* args, void* stream);
+/* Values of the 8-bit moments (a NULL pointer leaves that output out), and 8-bit moments from fp32 values (to the nearest). */
+int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, int chunk, void* const* exp_avg,
+                        void* const* exp_avg_sq, int type, void* stream);
+int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, int chunk, const float* const* exp_avg,
+                        const float* const* exp_avg_sq, void* stream);
+/* 2-norm over all tensors: accumulate once per type into `partials` (room for vcr_grad_norm_partials of every call together;
+ * *npartials counts them), then finish: *norm = sqrt(sum) * |grad_scale|. */
+int vcr_grad_norm_partials(int ntensors, const int64_t* numel);
+int vcr_grad_norm_accumulate(int ntensors, const void* const* tensors, const int64_t* numel, int type, double* partials,
+                             int capacity, int* npartials, void* stream);
+int vcr_grad_norm_finish(const double* partials, int npartials, double grad_scale, float* norm, void* stream);
+/* tensors *= min(1, max_norm / (*norm + 1e-6)), in place. */
+int vcr_clip_gradients(int ntensors, void* const* tensors, const int64_t* numel, int type, const float* norm, double max_norm,
+                       void* stream);
 /* The static tail of a training iteration in ONE pass over the Gaussians (no densify / prune / reset this iteration; data
  * parallel: on the all-reduced ACTIVATED-space gradients, grad_scale = 1 / world, normals_world = 1): adjoint of the fused activation (the four upstream gradients are those of vcr_rasterize_backward w.r.t. the
  * ACTIVATED scales / rotations / opacities / camera-space normals of this iteration's render; `aux`, `Rw2c` as saved by

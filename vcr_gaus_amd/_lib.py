@@ -16,7 +16,7 @@ c_int_p = C.POINTER(C.c_int32)
 ALLOC_FN = C.CFUNCTYPE(C.c_void_p, C.c_void_p, C.c_int32, C.c_size_t)
 HOOK_FN = C.CFUNCTYPE(None, C.c_void_p)
 BUF_GEOM, BUF_BINNING, BUF_IMAGE, BUF_SCRATCH = 0, 1, 2, 3
-ABI_VERSION = 19         # VCR_ABI_VERSION of include/vcr_raster.h this binding was written against
+ABI_VERSION = 20         # VCR_ABI_VERSION of include/vcr_raster.h this binding was written against
 
 
 class VcrShUpdate(C.Structure):
@@ -26,6 +26,22 @@ class VcrShUpdate(C.Structure):
         ("m_dc", C.c_void_p), ("v_dc", C.c_void_p), ("m_rest", C.c_void_p), ("v_rest", C.c_void_p),
         ("lr_dc", C.c_float), ("lr_rest", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
     ]
+
+
+class VcrOptimTensor(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("p", "master", "m", "v", "m_scale", "v_scale", "step")] + \
+               [("numel", C.c_int64), ("group", C.c_int32), ("index", C.c_int32)]
+
+
+class VcrOptimGroup(C.Structure):
+    _fields_ = [(k, C.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("lr_dev", C.c_void_p)]
+
+
+class VcrAdamWStep(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("ntensors", "ngroups", "chunk", "param_type", "state_bits", "masters")] + \
+               [("seed", C.c_uint32), ("npartials", C.c_int32), ("plan", C.c_void_p), ("grads", C.POINTER(C.c_void_p)),
+                ("numel", C.POINTER(C.c_int64)), ("groups", C.POINTER(VcrOptimGroup)), ("grad_scale", C.c_double),
+                ("max_norm", C.c_double), ("partials", C.c_void_p), ("norm_out", C.c_void_p), ("work", C.c_void_p)]
 
 
 class VcrGeometryStep(C.Structure):
@@ -118,6 +134,20 @@ SYMBOLS = {
     "vcr_geometry_step": (C.c_int, [C.POINTER(VcrGeometryStep), C.c_void_p]),
     "vcr_rasterize_backward_tail": (C.c_int, [C.POINTER(VcrRasterArgs), C.POINTER(VcrBackwardIO), C.POINTER(VcrGeometryStep), ALLOC_FN,
                                               C.c_void_p, C.c_void_p]),
+    "vcr_optim_plan_bytes": (C.c_size_t, [C.c_int, C.POINTER(C.c_int64), C.c_int]),
+    "vcr_optim_plan": (C.c_int, [C.c_int, C.POINTER(VcrOptimTensor), C.c_int, C.c_void_p, C.c_size_t]),
+    "vcr_adamw_work_bytes": (C.c_size_t, [C.c_int]),
+    "vcr_adamw_step": (C.c_int, [C.POINTER(VcrAdamWStep), C.c_void_p]),
+    "vcr_moments8_decode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_void_p),
+                                      C.POINTER(C.c_void_p), C.c_int, C.c_void_p]),
+    "vcr_moments8_encode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_void_p),
+                                      C.POINTER(C.c_void_p), C.c_void_p]),
+    "vcr_grad_norm_partials": (C.c_int, [C.c_int, C.POINTER(C.c_int64)]),
+    "vcr_grad_norm_accumulate": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.c_int, C.c_void_p, C.c_int,
+                                           c_int_p, C.c_void_p]),
+    "vcr_grad_norm_finish": (C.c_int, [C.c_void_p, C.c_int, C.c_double, C.c_void_p, C.c_void_p]),
+    "vcr_clip_gradients": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.c_int, C.c_void_p, C.c_double,
+                                     C.c_void_p]),
     "vcr_densify_stats": (C.c_int, [C.c_int] + [C.c_void_p] * 6),
     "vcr_depth_to_normal_forward": (C.c_int, [C.c_int, C.c_int] + [C.c_float] * 4 + [C.c_void_p] * 3),
     "vcr_depth_to_normal_backward": (C.c_int, [C.c_int, C.c_int] + [C.c_float] * 4 + [C.c_void_p] * 5),

@@ -1,0 +1,583 @@
+"""Optimizer operators over many tensors at once: `AdamW` (moments in 32 or in 8 bits), `grad_norm`, `clip_grad_norm_`.
+
+They stand beside `gaussian_model.FusedAdam` (Adam on the Gaussian model's groups, fp32, at most 8 tensors a launch) for what that one
+does not do: decoupled weight decay, any number of tensors of any size and alignment, fp32 / bf16 / fp16 parameters with or without
+fp32 masters, clipping by the norm of all gradients without a host round trip, step counters that live on the device (a captured
+step replays), and moments in a quarter of the memory.  The reference trains with torch.optim.Adam only
+(`scene/gaussian_model.py:258`); the update is torch.optim.AdamW's.  All arithmetic runs in csrc/optim.hip; there is no fallback.
+"""
+import ctypes as C
+from operator import attrgetter
+
+import torch
+
+from . import _lib
+
+BLOCK = 256                                    # elements that share the scale of an 8-bit moment
+CHUNK = 4096                                   # elements per workgroup
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_PTR, _CONTIGUOUS, _GRAD, _DTYPE = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, attrgetter("grad"), attrgetter("dtype")
+
+
+def _pointers(ptrs):
+    return (C.c_void_p * len(ptrs))(*ptrs)
+
+
+def _numels(ns):
+    return (C.c_int64 * len(ns))(*ns)
+
+
+class _on:
+    """Makes `dev` the current device for a library call on its stream (launches go to the current device)."""
+    __slots__ = ("dev", "was")
+
+    def __init__(self, dev):
+        self.dev = dev.index if dev.index is not None else torch.cuda.current_device()
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.was != self.dev:
+            torch.cuda.set_device(self.was)
+        return False
+
+
+def _check_list(tensors, what):
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    for k, t in enumerate(tensors):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}[{k}] is a {type(t).__name__}, not a tensor")
+        if t.dtype not in _TYPES:
+            raise ValueError(f"{what}[{k}] has type {t.dtype}: float32, bfloat16 or float16 are supported")
+        if not t.is_cuda or t.layout != torch.strided:
+            raise ValueError(f"{what}[{k}] is not a dense tensor on a HIP device")
+        if t.device != tensors[0].device:
+            raise ValueError(f"{what}[{k}] is on {t.device}, {what}[0] on {tensors[0].device}")
+    return tensors
+
+
+class _Partials:
+    """The partial sums of one norm: allocated on the current stream for this call alone."""
+
+    def __init__(self, lists, device):
+        lib = _lib.load()
+        self.lists = [(t, _pointers(p), _numels(n), len(p)) for t, p, n in lists if p]
+        self.capacity = sum(lib.vcr_grad_norm_partials(k, n) for _, _, n, k in self.lists)
+        self.buffer = torch.empty(max(1, self.capacity), dtype=torch.float64, device=device)
+        self.count = C.c_int(0)
+
+    def launch(self, stream):
+        lib = _lib.load()
+        for t, p, n, k in self.lists:
+            _lib.check(lib.vcr_grad_norm_accumulate(k, p, n, t, self.buffer.data_ptr(), self.capacity, C.byref(self.count), stream))
+        return self
+
+
+def _by_type(tensors):
+    out = {}
+    for t in tensors:
+        p, n = out.setdefault(_TYPES[t.dtype], ([], []))
+        p.append(t.data_ptr())
+        n.append(t.numel())
+    return [(t, p, n) for t, (p, n) in out.items()]
+
+
+@torch.no_grad()
+def grad_norm(tensors, out=None):
+    """2-norm over all elements of all `tensors` (a list, or one tensor; float32 / bfloat16 / float16, mixed as they come) as a 0-dim
+    float32 tensor on their device.  Sums in 64 bits in a fixed order: the same result on every run; NaN or infinity anywhere gives
+    NaN or infinity.  No tensors: an error, as there is no device to put the result on -- unless `out` is given."""
+    tensors = _check_list(tensors, "tensors")
+    if out is None:
+        if not tensors:
+            raise ValueError("grad_norm: no tensors and no `out`")
+        out = torch.empty((), device=tensors[0].device)
+    elif out.dtype != torch.float32 or out.numel() != 1 or not out.is_cuda or (tensors and out.device != tensors[0].device):
+        raise ValueError("grad_norm: `out` must be one float32 element on the tensors' device")
+    keep = [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    with _on(out.device):
+        st = _lib.stream_of(out)
+        parts = _Partials(_by_type(keep), out.device).launch(st)
+        _lib.check(_lib.load().vcr_grad_norm_finish(parts.buffer.data_ptr(), parts.count.value, 1.0, out.data_ptr(), st))
+    return out
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)), norm their 2-norm over all; -> norm (a 0-dim
+    float32 tensor; nothing waits for it).  For optimizers that take gradients as they are; `AdamW.step(max_norm=...)` applies the
+    factor inside the update instead, without writing the gradients again."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    max_norm = _positive(max_norm, "max_norm")
+    grads = _check_list([p.grad for p in parameters if p.grad is not None], "gradients")
+    if not grads:
+        raise ValueError("clip_grad_norm_: no parameter has a gradient")
+    work = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    norm = grad_norm(work)
+    with _on(norm.device):
+        st = _lib.stream_of(norm)
+        for t, p, n in _by_type(work):
+            _lib.check(_lib.load().vcr_clip_gradients(len(p), _pointers(p), _numels(n), t, norm.data_ptr(), max_norm, st))
+    for g, w in zip(grads, work):
+        if g is not w:
+            g.copy_(w)
+    return norm
+
+
+def _positive(x, what):
+    x = float(x)
+    if not x > 0.0:
+        raise ValueError(f"{what} = {x}: must be > 0")
+    return x
+
+
+class _Watched(dict):
+    """A dictionary of the optimizer's state: an entry that is replaced, added or removed makes the optimizer look at its tensors anew
+    (their addresses are on the device).  Values may be changed in place freely."""
+    __slots__ = ("_owner",)
+
+    def __init__(self, owner, items=()):
+        dict.__init__(self, items)
+        self._owner = owner
+
+    def _touch(name):
+        def method(self, *a, **k):
+            self._owner._plan = None
+            return getattr(dict, name)(self, *a, **k)
+        method.__name__ = name
+        return method
+
+    for _n in ("__setitem__", "__delitem__", "pop", "popitem", "clear", "update", "setdefault", "__ior__"):
+        locals()[_n] = _touch(_n)
+    del _n, _touch
+
+    def __reduce__(self):
+        return dict, (dict(self),)
+
+
+class _Bucket:
+    """The tensors of one type: their plan on the device and what a call needs of them on the host."""
+    __slots__ = ("type", "at", "numels", "plan", "work_bytes", "n")
+
+
+class _Plan:
+    __slots__ = ("params", "ptrs", "dtypes", "keys", "groups_of", "sizes", "buckets", "device", "stream", "captured")
+
+
+class AdamW:
+    """AdamW over any number of tensors (a list, or groups: dicts with `params` and optionally `name`, `lr`, `betas`, `eps`,
+    `weight_decay`), updated in one launch per 400 tensors of a type:
+
+        m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2;  p <- p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    with g = grad * `grad_scale`.  `state_bits=8` keeps both moments in 8 bits, blocks of 256 elements sharing a power-of-two scale
+    (2.01 instead of 8 bytes per parameter), rounded stochastically from `seed`, the step and the element's place: the same run
+    gives the same bits.  `master_weights=True` keeps fp32 copies of 16-bit parameters and updates those; without, the update is
+    rounded into the 16-bit parameter.  `lr` may be a float32 device scalar (a captured step reads it at replay).
+
+    `state[key]`: `step` (int32 on the device), `exp_avg`, `exp_avg_sq` (float32, or uint8 codes with `exp_avg_scale` /
+    `exp_avg_sq_scale`), `master`; key = the group's name if the group has one tensor, else "<name or number>.<i>".
+    Parameters must be contiguous; gradients of another layout are copied.  Tensors without a gradient are skipped, and so are
+    their counters, as in torch.  Memory: plan and state belong to the optimizer; a captured step keeps its plan alive."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False, seed=0):
+        params = list(params)
+        if not params:
+            raise ValueError("AdamW: no parameters")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits = {state_bits}: 8 or 32")
+        self.defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay)
+        groups = params if isinstance(params[0], dict) else [dict(params=params)]
+        self.param_groups = []
+        for g in groups:
+            if not isinstance(g, dict) or "params" not in g:
+                raise TypeError("AdamW: groups are dictionaries with `params`")
+            ps = g["params"]
+            g["params"] = [ps] if isinstance(ps, torch.Tensor) else list(ps)
+            for k, v in self.defaults.items():
+                g.setdefault(k, v)
+            self.param_groups.append(g)
+        self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed) & 0xFFFFFFFF
+        self.grad_scale = 1.0
+        self._plan, self._captured = None, []
+        self._state_dict = _Watched(self)
+        for k, g in enumerate(self.param_groups):
+            self._hyper(k, g)
+        seen = set()
+        for p in self._tensors():
+            if not isinstance(p, torch.Tensor):
+                raise TypeError(f"AdamW: a {type(p).__name__} among the parameters")
+            if id(p) in seen:
+                raise ValueError("AdamW: a parameter appears twice")
+            seen.add(id(p))
+
+    # ---- what is trained ---------------------------------------------------------------------------------------------
+    @property
+    def state(self):
+        return self._state_dict
+
+    @state.setter
+    def state(self, new):
+        self._plan = None
+        self._state_dict = _Watched(self, {k: _Watched(self, v) for k, v in new.items()})
+
+    def _tensors(self):
+        return [p for g in self.param_groups for p in g["params"]]
+
+    def _keys(self):
+        out = []
+        for i, g in enumerate(self.param_groups):
+            name, n = str(g.get("name", i)), len(g["params"])
+            out += [name] if n == 1 else [f"{name}.{j}" for j in range(n)]
+        if len(set(out)) != len(out):
+            raise ValueError(f"AdamW: group names are not unique: {sorted(k for k in set(out) if out.count(k) > 1)}")
+        return out
+
+    @staticmethod
+    def _hyper(k, g):
+        lr, (b1, b2), eps, wd = g["lr"], g["betas"], g["eps"], g["weight_decay"]
+        dev = None
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+                raise ValueError(f"AdamW: group {k}: a tensor `lr` must be one float32 element on the device")
+            dev, lr = lr.data_ptr(), 0.0
+        if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and wd >= 0.0):
+            raise ValueError(f"AdamW: group {k}: lr {lr}, betas {(b1, b2)}, eps {eps}, weight_decay {wd} out of range")
+        return _lib.VcrOptimGroup(float(lr), float(b1), float(b2), float(eps), float(wd), dev)
+
+    def _fresh(self, p):
+        dev, n = p.device, p.numel()
+        st = dict(step=torch.zeros((), dtype=torch.int32, device=dev))
+        if self.state_bits == 32:
+            st.update(exp_avg=torch.zeros(p.shape, device=dev), exp_avg_sq=torch.zeros(p.shape, device=dev))
+        else:
+            nb = -(-n // BLOCK)
+            st.update({k: torch.zeros(p.shape, dtype=torch.uint8, device=dev) for k in ("exp_avg", "exp_avg_sq")})
+            st.update({k: torch.ones(nb, dtype=torch.uint8, device=dev) for k in ("exp_avg_scale", "exp_avg_sq_scale")})
+        if self._has_master(p):
+            st["master"] = p.detach().float().contiguous()
+        return _Watched(self, st)
+
+    def _has_master(self, p):
+        return self.master_weights and p.dtype != torch.float32
+
+    def _check_state(self, key, p, st):
+        n, nb = p.numel(), -(-p.numel() // BLOCK)
+        want = {"step": (torch.int32, 1)}
+        kind = torch.float32 if self.state_bits == 32 else torch.uint8
+        want.update(exp_avg=(kind, n), exp_avg_sq=(kind, n))
+        if self.state_bits == 8:
+            want.update(exp_avg_scale=(kind, nb), exp_avg_sq_scale=(kind, nb))
+        if self._has_master(p):
+            want["master"] = (torch.float32, n)
+        for k, (dt, m) in want.items():
+            t = st.get(k)
+            if not isinstance(t, torch.Tensor) or t.dtype != dt or t.numel() != m or t.device != p.device or not t.is_contiguous():
+                raise ValueError(f"AdamW: state[{key!r}][{k!r}] must be {m} contiguous elements of {dt} on {p.device}")
+
+    def _build(self):
+        """Plan of all parameters that have a gradient or a state."""
+        lib = _lib.load()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the first step after its tensors changed cannot be captured; take one step before the capture")
+        keys, groups_of = self._keys(), [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
+        plan = _Plan()
+        plan.params, plan.keys, plan.groups_of, plan.captured = self._tensors(), keys, groups_of, False
+        plan.sizes = [len(g["params"]) for g in self.param_groups]
+        _check_list(plan.params, "params")
+        plan.device = plan.params[0].device
+        plan.ptrs, plan.dtypes = list(map(_PTR, plan.params)), list(map(_DTYPE, plan.params))
+        by = {}
+        for i, (p, key) in enumerate(zip(plan.params, keys)):
+            if not p.is_contiguous():
+                raise ValueError(f"AdamW: parameter {key!r} is not contiguous")
+            if key not in self.state:
+                if p.grad is None:
+                    continue
+                dict.__setitem__(self.state, key, self._fresh(p))
+            self._check_state(key, p, self.state[key])
+            by.setdefault(_TYPES[p.dtype], []).append(i)
+        plan.buckets = []
+        for kind, at in by.items():
+            b = _Bucket()
+            b.type, b.at, b.n = kind, at, len(at)
+            ns = [plan.params[i].numel() for i in at]
+            b.numels = _numels(ns)
+            rec = (_lib.VcrOptimTensor * b.n)()
+            for r, i in zip(rec, at):
+                p, st = plan.params[i], self.state[keys[i]]
+                ptr = lambda k: st[k].data_ptr() if k in st else None  # noqa: E731
+                r.p, r.master, r.numel, r.group, r.index = p.data_ptr(), ptr("master") if self._has_master(p) else None, p.numel(), groups_of[i], i
+                r.m, r.v, r.step = ptr("exp_avg"), ptr("exp_avg_sq"), ptr("step")
+                if self.state_bits == 8 and p.numel():
+                    r.m_scale, r.v_scale = ptr("exp_avg_scale"), ptr("exp_avg_sq_scale")
+            size = lib.vcr_optim_plan_bytes(b.n, b.numels, CHUNK)
+            host = torch.empty(size, dtype=torch.uint8)
+            _lib.check(lib.vcr_optim_plan(b.n, rec, CHUNK, host.data_ptr(), size))
+            b.plan = host.to(plan.device)
+            b.work_bytes = lib.vcr_adamw_work_bytes(b.n)
+            plan.buckets.append(b)
+        stream = torch.cuda.current_stream(plan.device)
+        stream.synchronize()                     # (the upload is finished whatever stream the steps use)
+        plan.stream = stream.cuda_stream
+        self._plan = plan
+        return plan
+
+    def _current(self, need=()):
+        """The plan, rebuilt where a parameter or a state entry is another tensor than it holds; `need`: indices that must be in it."""
+        plan = self._plan
+        params = self._tensors()
+        if plan is None or [len(g["params"]) for g in self.param_groups] != plan.sizes or any(a is not b for a, b in zip(params, plan.params)) \
+                or list(map(_PTR, params)) != plan.ptrs or list(map(_DTYPE, params)) != plan.dtypes:
+            plan = self._build()
+        elif need and sum(b.n for b in plan.buckets) < len(params):
+            known = {i for b in plan.buckets for i in b.at}
+            if any(i not in known for i in need):
+                plan = self._build()
+        stream = torch.cuda.current_stream(plan.device)
+        if stream.cuda_stream != plan.stream:
+            for b in plan.buckets:
+                b.plan.record_stream(stream)
+        if not plan.captured and torch.cuda.is_current_stream_capturing():
+            plan.captured = True
+            self._captured.append(plan)          # the graph holds its addresses
+        return plan, stream.cuda_stream
+
+    # ---- the step -----------------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, only=None, max_norm=None):
+        """One update of every parameter that has a gradient (`only`: of the groups with these names; their gradients are released
+        afterwards, as in `FusedAdam.step`).  `max_norm`: the gradients count with the factor min(1, max_norm / (norm + 1e-6)), norm
+        the 2-norm of all gradients of this step times `grad_scale`; -> the norm (0-dim float32; nothing waits for it), and if that is
+        not finite in float32 the whole step is skipped on the device: parameters, moments and counters stay.  Without: -> None."""
+        lib = _lib.load()
+        if max_norm is not None:
+            max_norm = _positive(max_norm, "max_norm")
+        params = self._tensors()
+        grads = list(map(_GRAD, params))
+        if only is not None:
+            flags = [g.get("name") in only for g in self.param_groups for _ in g["params"]]
+            grads = [g if f else None for g, f in zip(grads, flags)]
+        live = [i for i, g in enumerate(grads) if g is not None]
+        if not live:
+            return None
+        plan, stream = self._current(need=live)
+        for i in live:
+            g = grads[i]
+            if g.dtype is not plan.dtypes[i]:
+                raise ValueError(f"AdamW: the gradient of {plan.keys[i]!r} has type {g.dtype}, the parameter {plan.dtypes[i]}")
+            if not g.is_contiguous():
+                grads[i] = g.contiguous()
+        ptrs = [0 if g is None else g.data_ptr() for g in grads]
+        groups = (_lib.VcrOptimGroup * len(self.param_groups))(*[self._hyper(k, g) for k, g in enumerate(self.param_groups)])
+        norm = parts = None
+        with _on(plan.device):
+            if max_norm is not None:
+                norm = torch.empty((), device=plan.device)
+                lists = []
+                for b in plan.buckets:
+                    at = [k for k, i in enumerate(b.at) if ptrs[i]]
+                    lists.append((b.type, [ptrs[b.at[k]] for k in at], [b.numels[k] for k in at]))
+                parts = _Partials(lists, plan.device).launch(stream)
+            for b in plan.buckets:
+                mine = [ptrs[i] for i in b.at]
+                if not any(mine):
+                    continue
+                work = torch.empty(b.work_bytes, dtype=torch.uint8, device=plan.device)
+                a = _lib.VcrAdamWStep(ntensors=b.n, ngroups=len(groups), chunk=CHUNK, param_type=b.type, state_bits=self.state_bits,
+                                      masters=int(self.master_weights and b.type != 0), seed=self.seed,
+                                      npartials=parts.count.value if parts else 0, plan=b.plan.data_ptr(), grads=_pointers(mine),
+                                      numel=b.numels, groups=groups, grad_scale=float(self.grad_scale),
+                                      max_norm=max_norm or 0.0, partials=parts.buffer.data_ptr() if parts else None,
+                                      norm_out=norm.data_ptr() if parts else None, work=work.data_ptr())
+                _lib.check(lib.vcr_adamw_step(C.byref(a), stream))
+        if only is not None:
+            for i in live:
+                params[i].grad = None
+        return norm
+
+    def zero_grad(self, set_to_none=True):
+        for p in self._tensors():
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.zero_()
+
+    # ---- moments as values ---------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def moments(self, exp_avgs=None, exp_avg_sqs=None, dtype=torch.float32):
+        """The moments as values, whatever they are held in: two lists, one tensor for each parameter in the groups' order.  Given
+        lists are written to (contiguous, all of one type) instead of new tensors of `dtype`; a parameter that has not been stepped
+        yet has zeros.  8-bit moments are exact in bfloat16."""
+        params = self._tensors()
+        outs = []
+        for given in (exp_avgs, exp_avg_sqs):
+            if given is None:
+                given = [torch.empty(p.shape, dtype=dtype, device=p.device) for p in params]
+            elif len(given) != len(params):
+                raise ValueError(f"moments: {len(given)} tensors for {len(params)} parameters")
+            outs.append(given)
+        kinds = {t.dtype for o in outs for t in o}
+        if len(kinds) != 1 or not kinds <= set(_TYPES):
+            raise ValueError(f"moments: the outputs must be of one type among float32, bfloat16, float16: {kinds}")
+        for o in outs:
+            for t, p in zip(o, params):
+                if t.numel() != p.numel() or t.device != p.device or not t.is_contiguous():
+                    raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
+        plan, stream = self._current()
+        held = {i for b in plan.buckets for i in b.at}
+        for i in range(len(params)):
+            if i not in held:
+                outs[0][i].zero_()
+                outs[1][i].zero_()
+            elif self.state_bits == 32:
+                for o, k in zip(outs, ("exp_avg", "exp_avg_sq")):
+                    o[i].copy_(self.state[plan.keys[i]][k].view(o[i].shape))
+        if self.state_bits == 8:
+            kind = _TYPES[kinds.pop()]
+            with _on(plan.device):
+                for b in plan.buckets:
+                    m, v = (_pointers([o[i].data_ptr() for i in b.at]) for o in outs)
+                    _lib.check(_lib.load().vcr_moments8_decode(b.n, b.plan.data_ptr(), b.numels, CHUNK, m, v, kind, stream))
+        return outs
+
+    @torch.no_grad()
+    def set_moments(self, key, exp_avg, exp_avg_sq, step=None):
+        """Gives the parameter of `key` these moments (float32 values of its shape; 8 bits: rounded to the nearest code)."""
+        keys = self._keys()
+        if key not in keys:
+            raise KeyError(f"AdamW: no parameter {key!r}")
+        p = self._tensors()[keys.index(key)]
+        for t in (exp_avg, exp_avg_sq):
+            if t.numel() != p.numel():
+                raise ValueError(f"set_moments: {t.numel()} values for the {p.numel()} elements of {key!r}")
+        old = self.state.get(key)
+        st = self._fresh(p)
+        if old is not None:
+            st["step"] = old["step"]
+            if "master" in old and old["master"].numel() == p.numel():
+                st["master"] = old["master"]
+        if step is not None:
+            st["step"].fill_(int(step))
+        m, v = (t.detach().to(device=p.device, dtype=torch.float32).reshape(p.shape).contiguous() for t in (exp_avg, exp_avg_sq))
+        if self.state_bits == 32:
+            st["exp_avg"], st["exp_avg_sq"] = m, v
+        elif p.numel():
+            encode8(m, v, st)
+        self.state[key] = st
+
+    # ---- checkpoints -----------------------------------------------------------------------------------------------------
+    def state_dict(self):
+        """torch.optim.AdamW's layout (state by running index, `step` a float32 scalar).  8-bit moments are stored as they are held
+        (uint8 codes and scales); `moments()` gives the values another optimizer could load."""
+        template = torch.optim.AdamW([torch.zeros(1)]).param_groups[0]
+        state, groups, idx = {}, [], 0
+        for i, (key, p) in enumerate(zip(self._keys(), self._tensors())):
+            st = self.state.get(key)
+            if st is not None:
+                state[i] = {k: torch.tensor(float(int(t))) if k == "step" else t for k, t in st.items()}
+        for g in self.param_groups:
+            wg = {k: v for k, v in template.items() if k != "params"}
+            wg.update({k: v for k, v in g.items() if k != "params"})
+            wg["params"] = list(range(idx, idx + len(g["params"])))
+            idx += len(g["params"])
+            groups.append(wg)
+        return dict(state=state, param_groups=groups)
+
+    @torch.no_grad()
+    def load_state_dict(self, sd):
+        """Takes what `state_dict()` gave -- or torch.optim.AdamW's: float moments are rounded into the 8-bit form where this optimizer
+        has that, and 8-bit ones expanded where it has not.  Tensors that already have this optimizer's type, layout and device are
+        kept, not copied, as torch does.  Groups are matched in order."""
+        if len(sd["param_groups"]) != len(self.param_groups):
+            raise ValueError(f"AdamW: {len(sd['param_groups'])} groups saved, {len(self.param_groups)} here")
+        order = []
+        for k, (wg, g) in enumerate(zip(sd["param_groups"], self.param_groups)):
+            if len(wg["params"]) != len(g["params"]):
+                raise ValueError(f"AdamW: group {k}: {len(wg['params'])} tensors saved, {len(g['params'])} here")
+            order += list(wg["params"])
+        new = {}
+        for i, key, p in zip(order, self._keys(), self._tensors()):
+            st = sd["state"].get(i)
+            if st is not None:
+                new[key] = self._converted(key, p, st)
+        for wg, g in zip(sd["param_groups"], self.param_groups):
+            for k in ("lr", "eps", "weight_decay"):
+                if k in wg:
+                    g[k] = wg[k]
+            if "betas" in wg:
+                g["betas"] = tuple(wg["betas"])
+        self.state = new
+
+    def _converted(self, key, p, st):
+        dev, n, nb = p.device, p.numel(), -(-p.numel() // BLOCK)
+        for k in ("exp_avg", "exp_avg_sq"):
+            if st[k].numel() != n:
+                raise ValueError(f"optimizer state of {key!r} has shape {tuple(st[k].shape)}, parameter {tuple(p.shape)}")
+        out = dict(step=torch.tensor(int(round(float(st["step"]))), dtype=torch.int32).to(dev))
+        as_held = lambda t, dt: t.detach().to(device=dev, dtype=dt).contiguous()  # noqa: E731
+        codes = st["exp_avg"].dtype == torch.uint8
+        if codes:
+            raw = {k: as_held(st[k], torch.uint8) for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
+            if any(raw[k].numel() != nb for k in ("exp_avg_scale", "exp_avg_sq_scale")):
+                raise ValueError(f"optimizer state of {key!r}: {nb} block scales expected")
+            out.update(raw)
+            if self.state_bits == 32:
+                out.update(zip(("exp_avg", "exp_avg_sq"), decode8(raw, p)))
+                del out["exp_avg_scale"], out["exp_avg_sq_scale"]
+        else:
+            m, v = as_held(st["exp_avg"], torch.float32), as_held(st["exp_avg_sq"], torch.float32)
+            if self.state_bits == 32:
+                out.update(exp_avg=m, exp_avg_sq=v)
+            else:
+                out.update({k: torch.zeros(p.shape, dtype=torch.uint8, device=dev) for k in ("exp_avg", "exp_avg_sq")})
+                out.update({k: torch.ones(nb, dtype=torch.uint8, device=dev) for k in ("exp_avg_scale", "exp_avg_sq_scale")})
+                encode8(m, v, out)
+        if self._has_master(p):
+            out["master"] = as_held(st["master"], torch.float32) if "master" in st else p.detach().float().contiguous()
+        return out
+
+
+def _single(st, n):
+    """A plan of one tensor's 8-bit moments, for the code <-> value kernels."""
+    lib = _lib.load()
+    dev = st["exp_avg"].device
+    rec = (_lib.VcrOptimTensor * 1)()
+    rec[0].p = rec[0].m = st["exp_avg"].data_ptr()
+    rec[0].v, rec[0].m_scale, rec[0].v_scale = (st[k].data_ptr() for k in ("exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"))
+    rec[0].step, rec[0].numel = st["exp_avg"].data_ptr(), n
+    ns = _numels([n])
+    size = lib.vcr_optim_plan_bytes(1, ns, CHUNK)
+    host = torch.empty(size, dtype=torch.uint8)
+    _lib.check(lib.vcr_optim_plan(1, rec, CHUNK, host.data_ptr(), size))
+    return host.to(dev), ns
+
+
+def encode8(exp_avg, exp_avg_sq, st):
+    """float32 moments into the uint8 tensors `exp_avg`, `exp_avg_sq`, `exp_avg_scale`, `exp_avg_sq_scale` of `st`, to the nearest."""
+    if exp_avg.numel() == 0:
+        return
+    dev = st["exp_avg"].device
+    if dev.type != "cuda":
+        raise ValueError("8-bit moments need a HIP device")
+    with _on(dev):
+        plan, ns = _single(st, exp_avg.numel())
+        _lib.check(_lib.load().vcr_moments8_encode(1, plan.data_ptr(), ns, CHUNK, _pointers([exp_avg.data_ptr()]),
+                                                   _pointers([exp_avg_sq.data_ptr()]), _lib.stream_of(st["exp_avg"])))
+
+
+def decode8(st, p):
+    """-> the float32 values of the 8-bit moments in `st`, of `p`'s shape."""
+    dev = st["exp_avg"].device
+    outs = [torch.empty(p.shape, device=dev) for _ in range(2)]
+    if p.numel():
+        if dev.type != "cuda":
+            raise ValueError("8-bit moments need a HIP device")
+        with _on(dev):
+            plan, ns = _single(st, p.numel())
+            _lib.check(_lib.load().vcr_moments8_decode(1, plan.data_ptr(), ns, CHUNK, *[_pointers([o.data_ptr()]) for o in outs], 0,
+                                                       _lib.stream_of(st["exp_avg"])))
+    return outs
