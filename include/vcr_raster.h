@@ -265,6 +265,7 @@ typedef struct VcrOptimTensor {
     uint8_t* m_scale;         /* 8 bits: one exponent per 256 elements, ceil(numel / 256) bytes; 32 bits: NULL */
     uint8_t* v_scale;
     int32_t* step;            /* device counter: steps taken */
+    uint32_t* arrived;        /* device word, zero between calls */
     int64_t numel;
     int32_t group;            /* index into VcrAdamWStep.groups */
     int32_t index;            /* the tensor's number in the random sequence of the 8-bit moments */
@@ -280,20 +281,17 @@ typedef struct VcrAdamWStep {
     int32_t state_bits;       /* 32 or 8 */
     int32_t masters;          /* != 0: 16-bit parameters with fp32 masters */
     uint32_t seed;            /* of the stochastic rounding of 8-bit moments */
-    int32_t npartials;        /* > 0: clip by max_norm / skip the step when the norm is not finite */
+    int32_t pad;
     const void* plan;         /* device */
     const void* const* grads; /* HOST array of device pointers; NULL = this tensor is not stepped */
     const int64_t* numel;     /* HOST, as in the plan */
+    const int32_t* group_of;  /* HOST, as in the plan; ascending */
     const VcrOptimGroup* groups; /* HOST */
-    double grad_scale;        /* multiplies every gradient (1 / world after a sum all-reduce, 1 / loss scale) */
-    double max_norm;
-    const double* partials;   /* device, from vcr_grad_norm_accumulate over ALL gradients of the step */
-    float* norm_out;          /* device scalar: norm of grad * grad_scale, or NULL */
-    void* work;               /* device, vcr_adamw_work_bytes(ntensors), 16-byte aligned */
+    double grad_scale;        /* multiplies every gradient (1 / world after a sum all-reduce, 1 / loss scale); not with `clip` */
+    const void* clip;         /* device: 8 bytes that vcr_grad_norm wrote (factor, skip), or NULL */
 } VcrAdamWStep;
 size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel, int chunk);
 int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, int chunk, void* host_plan, size_t bytes);
-size_t vcr_adamw_work_bytes(int ntensors);
 /* One AdamW step (decoupled weight decay, torch.optim.AdamW's arithmetic) on every tensor with a gradient; see csrc/optim.hip. */
 int vcr_adamw_step(const VcrAdamWStep* args, void* stream);
 /* Values of the 8-bit moments (a NULL pointer leaves that output out), and 8-bit moments from fp32 values (to the nearest). */
@@ -301,15 +299,15 @@ int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, in
                         void* const* exp_avg_sq, int type, void* stream);
 int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, int chunk, const float* const* exp_avg,
                         const float* const* exp_avg_sq, void* stream);
-/* 2-norm over all tensors: accumulate once per type into `partials` (room for vcr_grad_norm_partials of every call together;
- * *npartials counts them), then finish: *norm = sqrt(sum) * |grad_scale|. */
+/* 2-norm over all tensors, mixed types (HOST arrays): *norm = sqrt(sum of squares) * |grad_scale|, and with `clip` (8 bytes on the
+ * device) the factor grad_scale * min(1, max_norm / (norm + 1e-6)) of a clipped step, which is skipped if the norm is not finite.
+ * `partials`: scratch for `capacity` >= vcr_grad_norm_partials(ntensors, numel) doubles. */
 int vcr_grad_norm_partials(int ntensors, const int64_t* numel);
-int vcr_grad_norm_accumulate(int ntensors, const void* const* tensors, const int64_t* numel, int type, double* partials,
-                             int capacity, int* npartials, void* stream);
-int vcr_grad_norm_finish(const double* partials, int npartials, double grad_scale, float* norm, void* stream);
+int vcr_grad_norm(int ntensors, const void* const* tensors, const int64_t* numel, const int32_t* types, double* partials,
+                  int capacity, double grad_scale, double max_norm, float* norm, void* clip, void* stream);
 /* tensors *= min(1, max_norm / (*norm + 1e-6)), in place. */
-int vcr_clip_gradients(int ntensors, void* const* tensors, const int64_t* numel, int type, const float* norm, double max_norm,
-                       void* stream);
+int vcr_clip_gradients(int ntensors, void* const* tensors, const int64_t* numel, const int32_t* types, const float* norm,
+                       double max_norm, void* stream);
 /* The static tail of a training iteration in ONE pass over the Gaussians (no densify / prune / reset this iteration; data
  * parallel: on the all-reduced ACTIVATED-space gradients, grad_scale = 1 / world, normals_world = 1): adjoint of the fused activation (the four upstream gradients are those of vcr_rasterize_backward w.r.t. the
  * ACTIVATED scales / rotations / opacities / camera-space normals of this iteration's render; `aux`, `Rw2c` as saved by

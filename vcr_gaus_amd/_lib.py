@@ -29,7 +29,7 @@ class VcrShUpdate(C.Structure):
 
 
 class VcrOptimTensor(C.Structure):
-    _fields_ = [(k, C.c_void_p) for k in ("p", "master", "m", "v", "m_scale", "v_scale", "step")] + \
+    _fields_ = [(k, C.c_void_p) for k in ("p", "master", "m", "v", "m_scale", "v_scale", "step", "arrived")] + \
                [("numel", C.c_int64), ("group", C.c_int32), ("index", C.c_int32)]
 
 
@@ -39,9 +39,9 @@ class VcrOptimGroup(C.Structure):
 
 class VcrAdamWStep(C.Structure):
     _fields_ = [(k, C.c_int32) for k in ("ntensors", "ngroups", "chunk", "param_type", "state_bits", "masters")] + \
-               [("seed", C.c_uint32), ("npartials", C.c_int32), ("plan", C.c_void_p), ("grads", C.POINTER(C.c_void_p)),
-                ("numel", C.POINTER(C.c_int64)), ("groups", C.POINTER(VcrOptimGroup)), ("grad_scale", C.c_double),
-                ("max_norm", C.c_double), ("partials", C.c_void_p), ("norm_out", C.c_void_p), ("work", C.c_void_p)]
+               [("seed", C.c_uint32), ("pad", C.c_int32), ("plan", C.c_void_p), ("grads", C.POINTER(C.c_void_p)),
+                ("numel", C.POINTER(C.c_int64)), ("group_of", c_int_p), ("groups", C.POINTER(VcrOptimGroup)),
+                ("grad_scale", C.c_double), ("clip", C.c_void_p)]
 
 
 class VcrGeometryStep(C.Structure):
@@ -136,18 +136,15 @@ SYMBOLS = {
                                               C.c_void_p, C.c_void_p]),
     "vcr_optim_plan_bytes": (C.c_size_t, [C.c_int, C.POINTER(C.c_int64), C.c_int]),
     "vcr_optim_plan": (C.c_int, [C.c_int, C.POINTER(VcrOptimTensor), C.c_int, C.c_void_p, C.c_size_t]),
-    "vcr_adamw_work_bytes": (C.c_size_t, [C.c_int]),
     "vcr_adamw_step": (C.c_int, [C.POINTER(VcrAdamWStep), C.c_void_p]),
     "vcr_moments8_decode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_void_p),
                                       C.POINTER(C.c_void_p), C.c_int, C.c_void_p]),
     "vcr_moments8_encode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_void_p),
                                       C.POINTER(C.c_void_p), C.c_void_p]),
     "vcr_grad_norm_partials": (C.c_int, [C.c_int, C.POINTER(C.c_int64)]),
-    "vcr_grad_norm_accumulate": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.c_int, C.c_void_p, C.c_int,
-                                           c_int_p, C.c_void_p]),
-    "vcr_grad_norm_finish": (C.c_int, [C.c_void_p, C.c_int, C.c_double, C.c_void_p, C.c_void_p]),
-    "vcr_clip_gradients": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.c_int, C.c_void_p, C.c_double,
-                                     C.c_void_p]),
+    "vcr_grad_norm": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), c_int_p, C.c_void_p, C.c_int, C.c_double,
+                                C.c_double, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "vcr_clip_gradients": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), c_int_p, C.c_void_p, C.c_double, C.c_void_p]),
     "vcr_densify_stats": (C.c_int, [C.c_int] + [C.c_void_p] * 6),
     "vcr_depth_to_normal_forward": (C.c_int, [C.c_int, C.c_int] + [C.c_float] * 4 + [C.c_void_p] * 3),
     "vcr_depth_to_normal_backward": (C.c_int, [C.c_int, C.c_int] + [C.c_float] * 4 + [C.c_void_p] * 5),

@@ -16,7 +16,8 @@ from . import _lib
 BLOCK = 256                                    # elements that share the scale of an 8-bit moment
 CHUNK = 4096                                   # elements per workgroup
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_PTR, _CONTIGUOUS, _GRAD, _DTYPE = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, attrgetter("grad"), attrgetter("dtype")
+_PTR, _CONTIGUOUS, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
+_GRAD, _DTYPE, _DEVICE, _LAYOUT = attrgetter("grad"), attrgetter("dtype"), attrgetter("device"), attrgetter("layout")
 
 
 def _pointers(ptrs):
@@ -27,26 +28,26 @@ def _numels(ns):
     return (C.c_int64 * len(ns))(*ns)
 
 
-class _on:
-    """Makes `dev` the current device for a library call on its stream (launches go to the current device)."""
-    __slots__ = ("dev", "was")
+def _kinds(dtypes):
+    return (C.c_int32 * len(dtypes))(*[_TYPES[d] for d in dtypes])
 
-    def __init__(self, dev):
-        self.dev = dev.index if dev.index is not None else torch.cuda.current_device()
 
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.was != self.dev:
-            torch.cuda.set_device(self.was)
-        return False
+def _on(dev, call, *args):
+    """`call(*args)` with `dev` the current device: the library launches on the current device, whatever device the stream is of."""
+    if torch.cuda.current_device() == dev.index:
+        return call(*args)
+    with torch.cuda.device(dev):
+        return call(*args)
 
 
 def _check_list(tensors, what):
+    """The list, its types and its device; every tensor dense, of a supported type and on the device of the first."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if all(isinstance(t, torch.Tensor) for t in tensors):
+        dtypes, devices = list(map(_DTYPE, tensors)), set(map(_DEVICE, tensors))
+        if _TYPES.keys() >= set(dtypes) and len(devices) <= 1 and set(map(_LAYOUT, tensors)) <= {torch.strided} \
+                and all(d.type == "cuda" for d in devices):
+            return tensors, dtypes, devices.pop() if devices else None
     for k, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}[{k}] is a {type(t).__name__}, not a tensor")
@@ -56,52 +57,35 @@ def _check_list(tensors, what):
             raise ValueError(f"{what}[{k}] is not a dense tensor on a HIP device")
         if t.device != tensors[0].device:
             raise ValueError(f"{what}[{k}] is on {t.device}, {what}[0] on {tensors[0].device}")
-    return tensors
 
 
-class _Partials:
-    """The partial sums of one norm: allocated on the current stream for this call alone."""
-
-    def __init__(self, lists, device):
-        lib = _lib.load()
-        self.lists = [(t, _pointers(p), _numels(n), len(p)) for t, p, n in lists if p]
-        self.capacity = sum(lib.vcr_grad_norm_partials(k, n) for _, _, n, k in self.lists)
-        self.buffer = torch.empty(max(1, self.capacity), dtype=torch.float64, device=device)
-        self.count = C.c_int(0)
-
-    def launch(self, stream):
-        lib = _lib.load()
-        for t, p, n, k in self.lists:
-            _lib.check(lib.vcr_grad_norm_accumulate(k, p, n, t, self.buffer.data_ptr(), self.capacity, C.byref(self.count), stream))
-        return self
+def _norm(ptrs, numels, kinds, out, grad_scale=1.0, max_norm=0.0, clip=False):
+    """Launches the norm of the listed tensors into `out`; -> with `clip` the buffer whose first 8 bytes are the clipped step's factor.
+    The scratch belongs to this call (allocated on the current stream): two captured calls share nothing."""
+    lib = _lib.load()
+    n = len(numels)
+    room = lib.vcr_grad_norm_partials(n, numels)
+    buffer = torch.empty(room + 1, dtype=torch.float64, device=out.device)
+    at = buffer.data_ptr()
+    _lib.check(lib.vcr_grad_norm(n, ptrs, numels, kinds, at + 8, room, grad_scale, max_norm, out.data_ptr(), at if clip else None,
+                                 _lib.stream_of(out)))
+    return buffer
 
 
-def _by_type(tensors):
-    out = {}
-    for t in tensors:
-        p, n = out.setdefault(_TYPES[t.dtype], ([], []))
-        p.append(t.data_ptr())
-        n.append(t.numel())
-    return [(t, p, n) for t, (p, n) in out.items()]
-
-
-@torch.no_grad()
 def grad_norm(tensors, out=None):
     """2-norm over all elements of all `tensors` (a list, or one tensor; float32 / bfloat16 / float16, mixed as they come) as a 0-dim
     float32 tensor on their device.  Sums in 64 bits in a fixed order: the same result on every run; NaN or infinity anywhere gives
     NaN or infinity.  No tensors: an error, as there is no device to put the result on -- unless `out` is given."""
-    tensors = _check_list(tensors, "tensors")
+    tensors, dtypes, dev = _check_list(tensors, "tensors")
     if out is None:
-        if not tensors:
+        if dev is None:
             raise ValueError("grad_norm: no tensors and no `out`")
-        out = torch.empty((), device=tensors[0].device)
-    elif out.dtype != torch.float32 or out.numel() != 1 or not out.is_cuda or (tensors and out.device != tensors[0].device):
+        out = torch.empty((), device=dev)
+    elif out.dtype != torch.float32 or out.numel() != 1 or not out.is_cuda or dev not in (None, out.device):
         raise ValueError("grad_norm: `out` must be one float32 element on the tensors' device")
-    keep = [t if t.is_contiguous() else t.contiguous() for t in tensors]
-    with _on(out.device):
-        st = _lib.stream_of(out)
-        parts = _Partials(_by_type(keep), out.device).launch(st)
-        _lib.check(_lib.load().vcr_grad_norm_finish(parts.buffer.data_ptr(), parts.count.value, 1.0, out.data_ptr(), st))
+    if not all(map(_CONTIGUOUS, tensors)):
+        tensors = [t.detach().contiguous() for t in tensors]
+    _on(out.device, _norm, _pointers(list(map(_PTR, tensors))), _numels(list(map(_NUMEL, tensors))), _kinds(dtypes), out)
     return out
 
 
@@ -112,15 +96,20 @@ def clip_grad_norm_(parameters, max_norm):
     factor inside the update instead, without writing the gradients again."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = _positive(max_norm, "max_norm")
-    grads = _check_list([p.grad for p in parameters if p.grad is not None], "gradients")
+    grads, dtypes, dev = _check_list([p.grad for p in parameters if p.grad is not None], "gradients")
     if not grads:
         raise ValueError("clip_grad_norm_: no parameter has a gradient")
-    work = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    norm = grad_norm(work)
-    with _on(norm.device):
-        st = _lib.stream_of(norm)
-        for t, p, n in _by_type(work):
-            _lib.check(_lib.load().vcr_clip_gradients(len(p), _pointers(p), _numels(n), t, norm.data_ptr(), max_norm, st))
+    if len(set(map(id, grads))) != len(grads):
+        raise ValueError("clip_grad_norm_: a gradient appears twice")
+    work = [g.contiguous() for g in grads]
+    norm = torch.empty((), device=dev)
+    lists = _pointers(list(map(_PTR, work))), _numels(list(map(_NUMEL, work))), _kinds(dtypes)
+
+    def both():
+        _norm(*lists, norm)
+        _lib.check(_lib.load().vcr_clip_gradients(len(work), *lists, norm.data_ptr(), max_norm, _lib.stream_of(norm)))
+
+    _on(dev, both)
     for g, w in zip(grads, work):
         if g is not w:
             g.copy_(w)
@@ -160,11 +149,11 @@ class _Watched(dict):
 
 class _Bucket:
     """The tensors of one type: their plan on the device and what a call needs of them on the host."""
-    __slots__ = ("type", "at", "numels", "plan", "work_bytes", "n")
+    __slots__ = ("type", "at", "numels", "kinds", "group_of", "plan", "grads", "args", "n", "every")
 
 
 class _Plan:
-    __slots__ = ("params", "ptrs", "dtypes", "keys", "groups_of", "sizes", "buckets", "device", "stream", "captured")
+    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "buckets", "arrived", "device", "stream", "captured", "covered")
 
 
 class AdamW:
@@ -202,7 +191,7 @@ class AdamW:
             self.param_groups.append(g)
         self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed) & 0xFFFFFFFF
         self.grad_scale = 1.0
-        self._plan, self._captured = None, []
+        self._plan, self._captured, self._rates = None, [], None
         self._state_dict = _Watched(self)
         for k, g in enumerate(self.param_groups):
             self._hyper(k, g)
@@ -285,11 +274,10 @@ class AdamW:
             raise RuntimeError("AdamW: the first step after its tensors changed cannot be captured; take one step before the capture")
         keys, groups_of = self._keys(), [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
         plan = _Plan()
-        plan.params, plan.keys, plan.groups_of, plan.captured = self._tensors(), keys, groups_of, False
+        plan.params, plan.dtypes, plan.device = _check_list(self._tensors(), "params")
+        plan.keys, plan.captured = keys, False
         plan.sizes = [len(g["params"]) for g in self.param_groups]
-        _check_list(plan.params, "params")
-        plan.device = plan.params[0].device
-        plan.ptrs, plan.dtypes = list(map(_PTR, plan.params)), list(map(_DTYPE, plan.params))
+        plan.ids, plan.ptrs = list(map(id, plan.params)), list(map(_PTR, plan.params))
         by = {}
         for i, (p, key) in enumerate(zip(plan.params, keys)):
             if not p.is_contiguous():
@@ -300,25 +288,31 @@ class AdamW:
                 dict.__setitem__(self.state, key, self._fresh(p))
             self._check_state(key, p, self.state[key])
             by.setdefault(_TYPES[p.dtype], []).append(i)
-        plan.buckets = []
+        plan.buckets, plan.covered = [], sum(map(len, by.values()))
+        plan.arrived = torch.zeros(max(1, plan.covered), dtype=torch.int32, device=plan.device)
+        word = plan.arrived.data_ptr()
         for kind, at in by.items():
             b = _Bucket()
-            b.type, b.at, b.n = kind, at, len(at)
+            b.type, b.at, b.n, b.every = kind, at, len(at), len(at) == len(plan.params)
             ns = [plan.params[i].numel() for i in at]
-            b.numels = _numels(ns)
+            b.numels, b.kinds, b.group_of = _numels(ns), (C.c_int32 * b.n)(*[kind] * b.n), (C.c_int32 * b.n)(*[groups_of[i] for i in at])
             rec = (_lib.VcrOptimTensor * b.n)()
             for r, i in zip(rec, at):
                 p, st = plan.params[i], self.state[keys[i]]
                 ptr = lambda k: st[k].data_ptr() if k in st else None  # noqa: E731
                 r.p, r.master, r.numel, r.group, r.index = p.data_ptr(), ptr("master") if self._has_master(p) else None, p.numel(), groups_of[i], i
-                r.m, r.v, r.step = ptr("exp_avg"), ptr("exp_avg_sq"), ptr("step")
+                r.m, r.v, r.step, r.arrived = ptr("exp_avg"), ptr("exp_avg_sq"), ptr("step"), word
+                word += 4
                 if self.state_bits == 8 and p.numel():
                     r.m_scale, r.v_scale = ptr("exp_avg_scale"), ptr("exp_avg_sq_scale")
             size = lib.vcr_optim_plan_bytes(b.n, b.numels, CHUNK)
             host = torch.empty(size, dtype=torch.uint8)
             _lib.check(lib.vcr_optim_plan(b.n, rec, CHUNK, host.data_ptr(), size))
             b.plan = host.to(plan.device)
-            b.work_bytes = lib.vcr_adamw_work_bytes(b.n)
+            b.grads = (C.c_void_p * b.n)()
+            b.args = _lib.VcrAdamWStep(ntensors=b.n, chunk=CHUNK, param_type=kind, state_bits=self.state_bits,
+                                       masters=int(self.master_weights and kind != 0), seed=self.seed, plan=b.plan.data_ptr(),
+                                       grads=b.grads, numel=b.numels, group_of=b.group_of)
             plan.buckets.append(b)
         stream = torch.cuda.current_stream(plan.device)
         stream.synchronize()                     # (the upload is finished whatever stream the steps use)
@@ -326,14 +320,13 @@ class AdamW:
         self._plan = plan
         return plan
 
-    def _current(self, need=()):
+    def _current(self, params, need=()):
         """The plan, rebuilt where a parameter or a state entry is another tensor than it holds; `need`: indices that must be in it."""
         plan = self._plan
-        params = self._tensors()
-        if plan is None or [len(g["params"]) for g in self.param_groups] != plan.sizes or any(a is not b for a, b in zip(params, plan.params)) \
-                or list(map(_PTR, params)) != plan.ptrs or list(map(_DTYPE, params)) != plan.dtypes:
+        if plan is None or list(map(id, params)) != plan.ids or list(map(_PTR, params)) != plan.ptrs \
+                or [len(g["params"]) for g in self.param_groups] != plan.sizes or list(map(_DTYPE, params)) != plan.dtypes:
             plan = self._build()
-        elif need and sum(b.n for b in plan.buckets) < len(params):
+        elif plan.covered < len(params):
             known = {i for b in plan.buckets for i in b.at}
             if any(i not in known for i in need):
                 plan = self._build()
@@ -341,19 +334,26 @@ class AdamW:
         if stream.cuda_stream != plan.stream:
             for b in plan.buckets:
                 b.plan.record_stream(stream)
+            plan.arrived.record_stream(stream)
         if not plan.captured and torch.cuda.is_current_stream_capturing():
             plan.captured = True
             self._captured.append(plan)          # the graph holds its addresses
         return plan, stream.cuda_stream
 
+    def _group_table(self):
+        """The groups' rates as the library takes them, formed anew only where one has changed."""
+        key = [(g["lr"].data_ptr() if isinstance(g["lr"], torch.Tensor) else float(g["lr"]), g["betas"], g["eps"], g["weight_decay"])
+               for g in self.param_groups]
+        if self._rates is None or self._rates[0] != key:
+            self._rates = key, (_lib.VcrOptimGroup * len(key))(*[self._hyper(k, g) for k, g in enumerate(self.param_groups)])
+        return self._rates[1]
+
     # ---- the step -----------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, only=None, max_norm=None):
         """One update of every parameter that has a gradient (`only`: of the groups with these names; their gradients are released
         afterwards, as in `FusedAdam.step`).  `max_norm`: the gradients count with the factor min(1, max_norm / (norm + 1e-6)), norm
         the 2-norm of all gradients of this step times `grad_scale`; -> the norm (0-dim float32; nothing waits for it), and if that is
         not finite in float32 the whole step is skipped on the device: parameters, moments and counters stay.  Without: -> None."""
-        lib = _lib.load()
         if max_norm is not None:
             max_norm = _positive(max_norm, "max_norm")
         params = self._tensors()
@@ -364,39 +364,40 @@ class AdamW:
         live = [i for i, g in enumerate(grads) if g is not None]
         if not live:
             return None
-        plan, stream = self._current(need=live)
-        for i in live:
-            g = grads[i]
-            if g.dtype is not plan.dtypes[i]:
-                raise ValueError(f"AdamW: the gradient of {plan.keys[i]!r} has type {g.dtype}, the parameter {plan.dtypes[i]}")
-            if not g.is_contiguous():
-                grads[i] = g.contiguous()
-        ptrs = [0 if g is None else g.data_ptr() for g in grads]
-        groups = (_lib.VcrOptimGroup * len(self.param_groups))(*[self._hyper(k, g) for k, g in enumerate(self.param_groups)])
-        norm = parts = None
-        with _on(plan.device):
-            if max_norm is not None:
-                norm = torch.empty((), device=plan.device)
-                lists = []
-                for b in plan.buckets:
-                    at = [k for k, i in enumerate(b.at) if ptrs[i]]
-                    lists.append((b.type, [ptrs[b.at[k]] for k in at], [b.numels[k] for k in at]))
-                parts = _Partials(lists, plan.device).launch(stream)
-            for b in plan.buckets:
-                mine = [ptrs[i] for i in b.at]
-                if not any(mine):
-                    continue
-                work = torch.empty(b.work_bytes, dtype=torch.uint8, device=plan.device)
-                a = _lib.VcrAdamWStep(ntensors=b.n, ngroups=len(groups), chunk=CHUNK, param_type=b.type, state_bits=self.state_bits,
-                                      masters=int(self.master_weights and b.type != 0), seed=self.seed,
-                                      npartials=parts.count.value if parts else 0, plan=b.plan.data_ptr(), grads=_pointers(mine),
-                                      numel=b.numels, groups=groups, grad_scale=float(self.grad_scale),
-                                      max_norm=max_norm or 0.0, partials=parts.buffer.data_ptr() if parts else None,
-                                      norm_out=norm.data_ptr() if parts else None, work=work.data_ptr())
-                _lib.check(lib.vcr_adamw_step(C.byref(a), stream))
+        plan, stream = self._current(params, live)
+        if len(live) == len(grads):
+            same = list(map(_DTYPE, grads)) == plan.dtypes
+            if not all(map(_CONTIGUOUS, grads)):
+                grads = [g.detach().contiguous() for g in grads]
+            ptrs = list(map(_PTR, grads))
+        else:
+            same = all(grads[i].dtype is plan.dtypes[i] for i in live)
+            grads = [None if g is None else g.detach().contiguous() for g in grads]
+            ptrs = [None if g is None else g.data_ptr() for g in grads]
+        if not same:
+            i = next(i for i in live if grads[i].dtype is not plan.dtypes[i])
+            raise ValueError(f"AdamW: the gradient of {plan.keys[i]!r} has type {grads[i].dtype}, the parameter {plan.dtypes[i]}")
+        norm = _on(plan.device, self._launch, plan, ptrs, live, max_norm, stream)
         if only is not None:
             for i in live:
                 params[i].grad = None
+        return norm
+
+    def _launch(self, plan, ptrs, live, max_norm, stream):
+        groups, lib, norm, clip = self._group_table(), _lib.load(), None, None
+        if max_norm is not None:
+            norm = torch.empty((), device=plan.device)
+            if len(live) == len(ptrs) and len(plan.buckets) == 1:
+                b = plan.buckets[0]
+                lists = _pointers(ptrs), b.numels, b.kinds
+            else:
+                lists = _pointers([ptrs[i] for i in live]), _numels([plan.params[i].numel() for i in live]), _kinds([plan.dtypes[i] for i in live])
+            clip = _norm(*lists, norm, float(self.grad_scale), max_norm, True)
+        for b in plan.buckets:
+            b.grads[:] = ptrs if b.every else [ptrs[i] for i in b.at]
+            a = b.args
+            a.groups, a.ngroups, a.grad_scale, a.clip = groups, len(groups), self.grad_scale, None if clip is None else clip.data_ptr()
+            _lib.check(lib.vcr_adamw_step(C.byref(a), stream))
         return norm
 
     def zero_grad(self, set_to_none=True):
@@ -427,7 +428,7 @@ class AdamW:
             for t, p in zip(o, params):
                 if t.numel() != p.numel() or t.device != p.device or not t.is_contiguous():
                     raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
-        plan, stream = self._current()
+        plan, stream = self._current(params)
         held = {i for b in plan.buckets for i in b.at}
         for i in range(len(params)):
             if i not in held:
@@ -438,10 +439,9 @@ class AdamW:
                     o[i].copy_(self.state[plan.keys[i]][k].view(o[i].shape))
         if self.state_bits == 8:
             kind = _TYPES[kinds.pop()]
-            with _on(plan.device):
-                for b in plan.buckets:
-                    m, v = (_pointers([o[i].data_ptr() for i in b.at]) for o in outs)
-                    _lib.check(_lib.load().vcr_moments8_decode(b.n, b.plan.data_ptr(), b.numels, CHUNK, m, v, kind, stream))
+            for b in plan.buckets:
+                m, v = (_pointers([o[i].data_ptr() for i in b.at]) for o in outs)
+                _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), b.numels, CHUNK, m, v, kind, stream))
         return outs
 
     @torch.no_grad()
@@ -548,7 +548,8 @@ def _single(st, n):
     rec = (_lib.VcrOptimTensor * 1)()
     rec[0].p = rec[0].m = st["exp_avg"].data_ptr()
     rec[0].v, rec[0].m_scale, rec[0].v_scale = (st[k].data_ptr() for k in ("exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"))
-    rec[0].step, rec[0].numel = st["exp_avg"].data_ptr(), n
+    rec[0].step = rec[0].arrived = st["exp_avg"].data_ptr()               # (unused by these kernels, but not optional)
+    rec[0].numel = n
     ns = _numels([n])
     size = lib.vcr_optim_plan_bytes(1, ns, CHUNK)
     host = torch.empty(size, dtype=torch.uint8)
@@ -563,10 +564,9 @@ def encode8(exp_avg, exp_avg_sq, st):
     dev = st["exp_avg"].device
     if dev.type != "cuda":
         raise ValueError("8-bit moments need a HIP device")
-    with _on(dev):
-        plan, ns = _single(st, exp_avg.numel())
-        _lib.check(_lib.load().vcr_moments8_encode(1, plan.data_ptr(), ns, CHUNK, _pointers([exp_avg.data_ptr()]),
-                                                   _pointers([exp_avg_sq.data_ptr()]), _lib.stream_of(st["exp_avg"])))
+    plan, ns = _single(st, exp_avg.numel())
+    _lib.check(_on(dev, _lib.load().vcr_moments8_encode, 1, plan.data_ptr(), ns, CHUNK, _pointers([exp_avg.data_ptr()]),
+                   _pointers([exp_avg_sq.data_ptr()]), _lib.stream_of(st["exp_avg"])))
 
 
 def decode8(st, p):
@@ -576,8 +576,7 @@ def decode8(st, p):
     if p.numel():
         if dev.type != "cuda":
             raise ValueError("8-bit moments need a HIP device")
-        with _on(dev):
-            plan, ns = _single(st, p.numel())
-            _lib.check(_lib.load().vcr_moments8_decode(1, plan.data_ptr(), ns, CHUNK, *[_pointers([o.data_ptr()]) for o in outs], 0,
-                                                       _lib.stream_of(st["exp_avg"])))
+        plan, ns = _single(st, p.numel())
+        _lib.check(_on(dev, _lib.load().vcr_moments8_decode, 1, plan.data_ptr(), ns, CHUNK, *[_pointers([o.data_ptr()]) for o in outs], 0,
+                       _lib.stream_of(st["exp_avg"])))
     return outs
