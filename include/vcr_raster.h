@@ -253,7 +253,7 @@ int vcr_adam_step(int ntensors, float* const* params, const float* const* grads,
                   float eps, int step, float grad_scale, void* stream);
 /* ---- optimizer over many tensors at once: AdamW with the moments in 32 or in 8 bits, gradient norm and clipping ------------
  * A PLAN holds what stays from step to step: one record per tensor and the map from workgroups to tensors.  It is built on the
- * host (vcr_optim_plan) and copied to the device by the caller; the gradients' addresses come with every call. */
+ * host (vcr_optim_plan) and copied to the device by the caller, 16-byte aligned; the gradients' addresses come with every call. */
 #define VCR_F32 0
 #define VCR_BF16 1
 #define VCR_F16 2
@@ -265,10 +265,11 @@ typedef struct VcrOptimTensor {
     uint8_t* m_scale;         /* 8 bits: one exponent per 256 elements, ceil(numel / 256) bytes; 32 bits: NULL */
     uint8_t* v_scale;
     int32_t* step;            /* device counter: steps taken */
-    uint32_t* arrived;        /* device word, zero between calls */
     int64_t numel;
     int32_t group;            /* index into VcrAdamWStep.groups */
     int32_t index;            /* the tensor's number in the random sequence of the 8-bit moments */
+    int32_t words;            /* set by vcr_optim_plan */
+    int32_t pad;
 } VcrOptimTensor;
 typedef struct VcrOptimGroup {
     double lr, beta1, beta2, eps, weight_decay;
@@ -276,13 +277,11 @@ typedef struct VcrOptimGroup {
 } VcrOptimGroup;
 typedef struct VcrAdamWStep {
     int32_t ntensors, ngroups;
-    int32_t chunk;            /* elements per workgroup: a multiple of 1024, the plan's */
     int32_t param_type;       /* VCR_F32 / VCR_BF16 / VCR_F16, of parameters and gradients alike */
     int32_t state_bits;       /* 32 or 8 */
     int32_t masters;          /* != 0: 16-bit parameters with fp32 masters */
     uint32_t seed;            /* of the stochastic rounding of 8-bit moments */
-    int32_t pad;
-    const void* plan;         /* device */
+    void* plan;               /* device; the step keeps its tickets there */
     const void* const* grads; /* HOST array of device pointers; NULL = this tensor is not stepped */
     const int64_t* numel;     /* HOST, as in the plan */
     const int32_t* group_of;  /* HOST, as in the plan; ascending */
@@ -290,14 +289,14 @@ typedef struct VcrAdamWStep {
     double grad_scale;        /* multiplies every gradient (1 / world after a sum all-reduce, 1 / loss scale); not with `clip` */
     const void* clip;         /* device: 8 bytes that vcr_grad_norm wrote (factor, skip), or NULL */
 } VcrAdamWStep;
-size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel, int chunk);
-int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, int chunk, void* host_plan, size_t bytes);
+size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel);
+int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, void* host_plan, size_t bytes);
 /* One AdamW step (decoupled weight decay, torch.optim.AdamW's arithmetic) on every tensor with a gradient; see csrc/optim.hip. */
 int vcr_adamw_step(const VcrAdamWStep* args, void* stream);
 /* Values of the 8-bit moments (a NULL pointer leaves that output out), and 8-bit moments from fp32 values (to the nearest). */
-int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, int chunk, void* const* exp_avg,
+int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, void* const* exp_avg,
                         void* const* exp_avg_sq, int type, void* stream);
-int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, int chunk, const float* const* exp_avg,
+int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, const float* const* exp_avg,
                         const float* const* exp_avg_sq, void* stream);
 /* 2-norm over all tensors, mixed types (HOST arrays): *norm = sqrt(sum of squares) * |grad_scale|, and with `clip` (8 bytes on the
  * device) the factor grad_scale * min(1, max_norm / (norm + 1e-6)) of a clipped step, which is skipped if the norm is not finite.

@@ -29,8 +29,8 @@ class VcrShUpdate(C.Structure):
 
 
 class VcrOptimTensor(C.Structure):
-    _fields_ = [(k, C.c_void_p) for k in ("p", "master", "m", "v", "m_scale", "v_scale", "step", "arrived")] + \
-               [("numel", C.c_int64), ("group", C.c_int32), ("index", C.c_int32)]
+    _fields_ = [(k, C.c_void_p) for k in ("p", "master", "m", "v", "m_scale", "v_scale", "step")] + \
+               [("numel", C.c_int64)] + [(k, C.c_int32) for k in ("group", "index", "words", "pad")]
 
 
 class VcrOptimGroup(C.Structure):
@@ -38,8 +38,8 @@ class VcrOptimGroup(C.Structure):
 
 
 class VcrAdamWStep(C.Structure):
-    _fields_ = [(k, C.c_int32) for k in ("ntensors", "ngroups", "chunk", "param_type", "state_bits", "masters")] + \
-               [("seed", C.c_uint32), ("pad", C.c_int32), ("plan", C.c_void_p), ("grads", C.POINTER(C.c_void_p)),
+    _fields_ = [(k, C.c_int32) for k in ("ntensors", "ngroups", "param_type", "state_bits", "masters")] + \
+               [("seed", C.c_uint32), ("plan", C.c_void_p), ("grads", C.POINTER(C.c_void_p)),
                 ("numel", C.POINTER(C.c_int64)), ("group_of", c_int_p), ("groups", C.POINTER(VcrOptimGroup)),
                 ("grad_scale", C.c_double), ("clip", C.c_void_p)]
 
@@ -134,12 +134,12 @@ SYMBOLS = {
     "vcr_geometry_step": (C.c_int, [C.POINTER(VcrGeometryStep), C.c_void_p]),
     "vcr_rasterize_backward_tail": (C.c_int, [C.POINTER(VcrRasterArgs), C.POINTER(VcrBackwardIO), C.POINTER(VcrGeometryStep), ALLOC_FN,
                                               C.c_void_p, C.c_void_p]),
-    "vcr_optim_plan_bytes": (C.c_size_t, [C.c_int, C.POINTER(C.c_int64), C.c_int]),
-    "vcr_optim_plan": (C.c_int, [C.c_int, C.POINTER(VcrOptimTensor), C.c_int, C.c_void_p, C.c_size_t]),
+    "vcr_optim_plan_bytes": (C.c_size_t, [C.c_int, C.POINTER(C.c_int64)]),
+    "vcr_optim_plan": (C.c_int, [C.c_int, C.POINTER(VcrOptimTensor), C.c_void_p, C.c_size_t]),
     "vcr_adamw_step": (C.c_int, [C.POINTER(VcrAdamWStep), C.c_void_p]),
-    "vcr_moments8_decode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_void_p),
+    "vcr_moments8_decode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_void_p),
                                       C.POINTER(C.c_void_p), C.c_int, C.c_void_p]),
-    "vcr_moments8_encode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_void_p),
+    "vcr_moments8_encode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_void_p),
                                       C.POINTER(C.c_void_p), C.c_void_p]),
     "vcr_grad_norm_partials": (C.c_int, [C.c_int, C.POINTER(C.c_int64)]),
     "vcr_grad_norm": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), c_int_p, C.c_void_p, C.c_int, C.c_double,

@@ -19,11 +19,13 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <math.h>
-#include <new>
+#include <string.h>
 
 namespace {
 
 #define VCR_OPT_BLOCK 256          // elements that share a scale
+#define VCR_OPT_THREADS 1024
+#define VCR_OPT_CHUNK 4096         // elements per workgroup of the update kernels
 #define VCR_OPT_TENSORS 352        // tensors and ...
 #define VCR_OPT_GROUPS 14          // ... hyper-parameter groups per launch: both travel in the kernel arguments (4 KB)
 #define VCR_OPT_NORM_TENSORS 192   // tensors per launch of the norm kernel
@@ -40,71 +42,88 @@ static_assert(sizeof(StepPack) <= 4000 && sizeof(NormPack) <= 4000 && sizeof(Pai
 struct Coef { float decay, step_size, inv_sqrt_bc2, eps, b1, omb1, b2, omb2; };
 struct Clip { float gscale; int skip; };       // of a clipped step, written by the finish kernel
 
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+// Pointers read from memory are generic to the compiler (flat_* accesses, which wait on two counters); these are global.
+#define GLOBAL __attribute__((address_space(1)))
+template <typename T> __device__ __forceinline__ GLOBAL T* global(T* p) { return (GLOBAL T*)(uintptr_t)p; }
 
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ float load1(const __hip_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float load1(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ void store1(float* p, float x) { *p = x; }
-__device__ __forceinline__ void store1(__hip_bfloat16* p, float x) { *p = __float2bfloat16(x); }
-__device__ __forceinline__ void store1(__half* p, float x) { *p = __float2half(x); }
-
-// V consecutive elements of an aligned array, V = 4 or 8
-template <int V> struct Vec { float x[V]; };
-template <int V> __device__ __forceinline__ Vec<V> loadv(const float* p) {
-    Vec<V> r;
-#pragma unroll
-    for (int k = 0; k < V; k += 4) {
-        const f4 q = *reinterpret_cast<const f4*>(p + k);
-        r.x[k] = q.x; r.x[k + 1] = q.y; r.x[k + 2] = q.z; r.x[k + 3] = q.w;
-    }
-    return r;
+__device__ __forceinline__ float load1(const GLOBAL float* p) { return *p; }
+__device__ __forceinline__ float load1(const GLOBAL __hip_bfloat16* p) {
+    return __uint_as_float((uint32_t)*(const GLOBAL unsigned short*)p << 16);
 }
-__device__ __forceinline__ void widen(uint32_t w, float* x, const __hip_bfloat16*) {
+__device__ __forceinline__ float load1(const GLOBAL __half* p) { return __half2float(__ushort_as_half(*(const GLOBAL unsigned short*)p)); }
+__device__ __forceinline__ void store1(GLOBAL float* p, float x) { *p = x; }
+__device__ __forceinline__ void store1(GLOBAL __hip_bfloat16* p, float x) {
+    *(GLOBAL unsigned short*)p = __bfloat16_as_ushort(__float2bfloat16(x));
+}
+__device__ __forceinline__ void store1(GLOBAL __half* p, float x) { *(GLOBAL unsigned short*)p = __half_as_ushort(__float2half(x)); }
+
+// Four consecutive elements at any address that the element's type allows: the types below are aligned to one element, and the
+// hardware takes such addresses in its 8- and 16-byte accesses as they are.  NT: past the caches' retention, for what a step
+// touches once (all of it: parameters, gradients, moments).
+typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u2a __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u1a __attribute__((aligned(1)));
+template <bool NT, typename Q> __device__ __forceinline__ Q ldq(const GLOBAL void* p) {
+    if constexpr (NT) return __builtin_nontemporal_load((const GLOBAL Q*)p);
+    else return *(const GLOBAL Q*)p;
+}
+template <bool NT, typename Q> __device__ __forceinline__ void stq(GLOBAL void* p, Q q) {
+    if constexpr (NT) __builtin_nontemporal_store(q, (GLOBAL Q*)p);
+    else *(GLOBAL Q*)p = q;
+}
+template <int V> struct Vec { float x[V]; };
+__device__ __forceinline__ void widen(uint32_t w, float* x, const GLOBAL __hip_bfloat16*) {
     x[0] = __uint_as_float(w << 16); x[1] = __uint_as_float(w & 0xFFFF0000u);
 }
-__device__ __forceinline__ void widen(uint32_t w, float* x, const __half*) {
+__device__ __forceinline__ void widen(uint32_t w, float* x, const GLOBAL __half*) {
     x[0] = __half2float(__ushort_as_half((unsigned short)(w & 0xFFFFu))); x[1] = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
 }
-__device__ __forceinline__ uint32_t narrow(const float* x, const __hip_bfloat16*) {
+__device__ __forceinline__ uint32_t narrow(const float* x, const GLOBAL __hip_bfloat16*) {
     return (uint32_t)__bfloat16_as_ushort(__float2bfloat16(x[0])) | (uint32_t)__bfloat16_as_ushort(__float2bfloat16(x[1])) << 16;
 }
-__device__ __forceinline__ uint32_t narrow(const float* x, const __half*) {
+__device__ __forceinline__ uint32_t narrow(const float* x, const GLOBAL __half*) {
     return (uint32_t)__half_as_ushort(__float2half(x[0])) | (uint32_t)__half_as_ushort(__float2half(x[1])) << 16;
 }
-template <int V, typename T> __device__ __forceinline__ Vec<V> loadv(const T* p) {
+// (V = 4, or as many elements as 16 bytes hold)
+template <int V, bool NT, typename T> __device__ __forceinline__ Vec<V> loadv(const GLOBAL T* p) {
     Vec<V> r;
-    if constexpr (V == 8) {
-        const u4 q = *reinterpret_cast<const u4*>(p);
+    if constexpr (sizeof(T) == 4) {
+        const f4a q = ldq<NT, f4a>(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.x[k] = q[k];
+    } else if constexpr (V == 8) {
+        const u4a q = ldq<NT, u4a>(p);
 #pragma unroll
         for (int k = 0; k < 4; ++k) widen(q[k], r.x + 2 * k, p);
     } else {
-        const u2 q = *reinterpret_cast<const u2*>(p);
+        const u2a q = ldq<NT, u2a>(p);
 #pragma unroll
         for (int k = 0; k < 2; ++k) widen(q[k], r.x + 2 * k, p);
     }
     return r;
 }
-template <int V> __device__ __forceinline__ void storev(float* p, const Vec<V>& r) {
-#pragma unroll
-    for (int k = 0; k < V; k += 4) *reinterpret_cast<f4*>(p + k) = f4{r.x[k], r.x[k + 1], r.x[k + 2], r.x[k + 3]};
-}
-template <int V, typename T> __device__ __forceinline__ void storev(T* p, const Vec<V>& r) {
-    if constexpr (V == 8) {
-        u4 q;
+template <int V, bool NT, typename T> __device__ __forceinline__ void storev(GLOBAL T* p, const Vec<V>& r) {
+    if constexpr (sizeof(T) == 4) {
+        stq<NT>(p, f4a{r.x[0], r.x[1], r.x[2], r.x[3]});
+    } else if constexpr (V == 8) {
+        u4a q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) q[k] = narrow(r.x + 2 * k, p);
-        *reinterpret_cast<u4*>(p) = q;
+        stq<NT>(p, q);
     } else {
-        u2 q;
+        u2a q;
 #pragma unroll
         for (int k = 0; k < 2; ++k) q[k] = narrow(r.x + 2 * k, p);
-        *reinterpret_cast<u2*>(p) = q;
+        stq<NT>(p, q);
     }
 }
-__device__ __forceinline__ bool aligned(const void* p, uint32_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+// whether 4-element accesses of p and g are naturally aligned: if not, they share cache lines with the neighbours', and the
+// non-temporal kind would move each line twice (fp16, one element off: 52 against 46 us for 9 M elements)
+template <typename T> __device__ __forceinline__ bool aligned(const GLOBAL T* p, const GLOBAL T* g) {
+    return (((uint32_t)(uintptr_t)p | (uint32_t)(uintptr_t)g) & (4 * sizeof(T) - 1)) == 0;
+}
 
 __device__ __forceinline__ void moments_one(float& m, float& v, float g, const Coef& c) {
 #pragma clang fp contract(off)
@@ -117,12 +136,10 @@ __device__ __forceinline__ float root(float v) {
     const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p+32f : v);
     return small ? r * 0x1p-16f : r;
 }
-// square root and reciprocal are the instructions' own 1 ulp: 2e-7 of the update, which itself is rounded into p.  (A denominator
-// below 2^-126 -- eps under 1e-38 and no gradient ever -- or above 2^126 takes the division.)
+// Square root and reciprocal are the instructions' own, 1 ulp: 2e-7 of the update, which is itself rounded into p.  (The host refuses
+// an eps that is denormal in fp32, so the denominator is 0, normal or infinite.)
 __device__ __forceinline__ float param_one(float p, float m, float v, const Coef& c) {
-    const float d = root(v) * c.inv_sqrt_bc2 + c.eps;
-    const float q = d >= 0x1p-126f && d <= 0x1p+126f ? m * __builtin_amdgcn_rcpf(d) : m / d;
-    return p * c.decay - c.step_size * q;
+    return p * c.decay - c.step_size * (m * __builtin_amdgcn_rcpf(root(v) * c.inv_sqrt_bc2 + c.eps));
 }
 
 // 32-bit mix (constants found by a search for even avalanche over counters and random words)
@@ -167,10 +184,6 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
     const uint32_t a = __float_as_uint(x) & 0x7FFFFFFFu;
     return a >= INF_BITS ? 0u : a;
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-    for (int d = 32; d >= 1; d >>= 1) { const uint32_t y = __shfl_xor(x, d); x = x > y ? x : y; }
-    return x;
-}
 __device__ __forceinline__ int scale_of(uint32_t bits) { const int s = (int)(bits >> 23); return s > 1 ? s : 1; }
 
 // ---- norm -------------------------------------------------------------------------------------------------------
@@ -193,12 +206,6 @@ __device__ __forceinline__ Piece piece_of(const NormPack& pk, int n, uint32_t ch
     const long long off = (long long)(c - pk.start[lo]) * chunk, left = pk.n[lo] - off;
     return {lo, off, left < (long long)chunk ? (uint32_t)left : chunk};
 }
-// elements in front of the first 16-byte boundary
-template <typename T> __device__ __forceinline__ uint32_t head_of(const T* p, uint32_t cnt) {
-    const uint32_t h = (uint32_t)((16u - ((uintptr_t)p & 15u)) & 15u) / sizeof(T);
-    return h < cnt ? h : cnt;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(256) norm_kernel(NormPack pk, int n, uint32_t chunk, double* __restrict__ partials) {
     __shared__ double lds[4];
@@ -206,14 +213,12 @@ __global__ void __launch_bounds__(256) norm_kernel(NormPack pk, int n, uint32_t 
     double sum[V] = {};
     for (uint32_t c = blockIdx.x; c < pk.start[n]; c += gridDim.x) {
         const Piece q = piece_of(pk, n, chunk, c);
-        const T* g = (const T*)pk.g[q.tensor] + q.off;
-        const uint32_t head = head_of(g, q.cnt), vecs = (q.cnt - head) / V, tail = head + vecs * V;
-        if (threadIdx.x < head) { const double x = (double)load1(g + threadIdx.x); sum[0] += x * x; }
+        const GLOBAL T* g = global((const T*)pk.g[q.tensor]) + q.off;
+        const uint32_t vecs = q.cnt / V, tail = vecs * V;
         if (threadIdx.x < q.cnt - tail) { const double x = (double)load1(g + tail + threadIdx.x); sum[0] += x * x; }
-        const T* body = g + head;
 #pragma unroll 4
         for (uint32_t i = threadIdx.x; i < vecs; i += 256) {
-            const Vec<V> x = loadv<V>(body + (size_t)i * V);
+            const Vec<V> x = loadv<V, false>(g + (size_t)i * V);
 #pragma unroll
             for (int k = 0; k < V; ++k) { const double y = (double)x.x[k]; sum[k] += y * y; }
         }
@@ -253,33 +258,31 @@ __global__ void __launch_bounds__(256) scale_kernel(NormPack pk, int n, uint32_t
     if (f == 1.f) return;
     for (uint32_t c = blockIdx.x; c < pk.start[n]; c += gridDim.x) {
         const Piece q = piece_of(pk, n, chunk, c);
-        T* g = (T*)pk.g[q.tensor] + q.off;
-        const uint32_t head = head_of(g, q.cnt), vecs = (q.cnt - head) / V, tail = head + vecs * V;
-        if (threadIdx.x < head) store1(g + threadIdx.x, load1(g + threadIdx.x) * f);
+        GLOBAL T* g = global((T*)pk.g[q.tensor]) + q.off;
+        const uint32_t vecs = q.cnt / V, tail = vecs * V;
         if (threadIdx.x < q.cnt - tail) store1(g + tail + threadIdx.x, load1(g + tail + threadIdx.x) * f);
-        T* body = g + head;
         for (uint32_t i = threadIdx.x; i < vecs; i += 256) {
-            Vec<V> x = loadv<V>(body + (size_t)i * V);
+            Vec<V> x = loadv<V, false>(g + (size_t)i * V);
 #pragma unroll
             for (int k = 0; k < V; ++k) x.x[k] *= f;
-            storev<V>(body + (size_t)i * V, x);
+            storev<V, false>(g + (size_t)i * V, x);
         }
     }
 }
 
 // ---- what every workgroup of an update does first -------------------------------------------------------------------------
 // Step counters live on the device (a captured step replays, a skipped one does not count) and one launch does it all, so each
-// workgroup forms its tensor's factors itself, in fp64, from the counter: lanes 0 and 1 of a wave share one expm1.  The counter
-// may move only when every workgroup of the tensor has read it: each draws a ticket after its read, the last one writes.
-struct Work { const void* g; uint32_t cnt; long long off; int step; float gs; };
-
+// workgroup forms its tensor's factors itself from the counter: its first wave does, lanes 0 and 1 sharing one expm1,
+// while the data loads of all waves are in flight.  The counter may move only when every workgroup of the tensor has read
+// it: each draws a ticket after its read, the last one writes.
 __device__ __forceinline__ float from_lane(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
 
 __device__ __forceinline__ Coef coef_of(const Group& G, int t) {
+    // 1 - b^t from the rounded exponent: 1e-7 of the update, like its root and reciprocal
     const int odd = threadIdx.x & 1;
-    const double bc = -expm1((double)t * (odd ? G.log_b2 : G.log_b1));           // 1 - b^t
+    const float bc = -expm1f((float)((double)t * (odd ? G.log_b2 : G.log_b1)));
     const double lr = G.lr_dev ? (double)*G.lr_dev : G.lr;
-    const float f = odd ? (float)(1.0 / sqrt(bc)) : (float)(lr / bc);
+    const float f = odd ? 1.f / sqrtf(bc) : (float)lr / bc;
     Coef c;
     c.step_size = from_lane(f, 0);
     c.inv_sqrt_bc2 = from_lane(f, 1);
@@ -288,174 +291,275 @@ __device__ __forceinline__ Coef coef_of(const Group& G, int t) {
     return c;
 }
 
-// reads the counter, then counts this workgroup in; -> the step this update is
-__device__ __forceinline__ int enter(const VcrOptimTensor& R, uint32_t nchunks) {
-    __shared__ int step;
-    if (threadIdx.x == 0) {
-        int* counter = R.step;
-        uint32_t* arrived = R.arrived;
-        const int t = __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        step = t + 1;
-        if (nchunks == 1) {
-            *counter = t + 1;
+// Counts this workgroup out (its read of the counter is long done: the factors came from it).  Tickets on one address come at 12.5 ns each (a
+// tensor of 400 M elements in 195 000 workgroups would take 2.4 ms for them alone, measured), so a tensor with many chunks
+// has 64 first-level words, and only the last arrival of each goes to the second level.
+#define TICKET_GROUPS 64
+#define TICKET_FLAT 64             // up to this many chunks: one level
+#define TICKET_STRIDE 16           // words between two tickets: a cache line of their own
+__device__ __forceinline__ bool last_of(GLOBAL uint32_t* word, uint32_t of) {
+    if (__hip_atomic_fetch_add(word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != of - 1) return false;
+    __hip_atomic_store(word, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+__device__ __forceinline__ void leave(const VcrOptimTensor& R, uint32_t* words, uint32_t c, int step) {
+    if (threadIdx.x != 0) return;
+    const uint32_t nchunks = (uint32_t)((R.numel + VCR_OPT_CHUNK - 1) / VCR_OPT_CHUNK);
+    bool last = true;
+    if (nchunks > 1) {
+        GLOBAL uint32_t* w = global(words) + (size_t)R.words * TICKET_STRIDE;
+        if (nchunks <= TICKET_FLAT) {
+            last = last_of(w, nchunks);
         } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::"v"(t) : "memory");              // (the read is done before the ticket is drawn)
-            if (__hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nchunks - 1) {
-                __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(counter, t + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+            const uint32_t g = c % TICKET_GROUPS;
+            last = last_of(w + (1 + g) * TICKET_STRIDE, (nchunks - g + TICKET_GROUPS - 1) / TICKET_GROUPS) && last_of(w, TICKET_GROUPS);
         }
     }
+    if (last) *global(R.step) = step;
+}
+// the step that this update is, and its factors, the same in every lane; `leave` follows when the results are out
+struct Entry { int step; Coef coef; };
+__device__ __forceinline__ Entry enter(const VcrOptimTensor& R, const Group& G) {
+    __shared__ Entry entry;
+    if (threadIdx.x < 64) {
+        const int t = *global(R.step) + 1;
+        const Coef coef = coef_of(G, t);
+        if (threadIdx.x == 0) { entry.step = t; entry.coef = coef; }
+    }
     __syncthreads();
-    return step;
+    return entry;
 }
 
-// ---- update, moments in 32 bits --------------------------------------------------------------------------------------
+// ---- update, moments in 32 bits: four consecutive elements per lane, 4096 per workgroup ------------------------------------
 template <typename T, bool MASTER>
-__global__ void __launch_bounds__(256) adamw_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
-                                                    uint32_t chunk, const Clip* __restrict__ clip, float gscale, StepPack pk,
-                                                    int t0, int g0) {
-    constexpr int V = 16 / sizeof(T);
+__global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
+                                                                uint32_t* __restrict__ words, const Clip* __restrict__ clip, float gscale,
+                                                                StepPack pk, int t0, int g0) {
     const uint2 cw = chunks[blockIdx.x];
-    const T* g = (const T*)pk.g[cw.x - t0];
+    const GLOBAL T* g = global((const T*)pk.g[cw.x - t0]);
     if (!g || (clip && clip->skip)) return;
     const VcrOptimTensor& R = tensors[cw.x];
     const float gs = clip ? clip->gscale : gscale;
-    const long long off = (long long)cw.y * chunk, left = R.numel - off;
-    const uint32_t cnt = left < (long long)chunk ? (uint32_t)left : chunk;
-    const Coef c = coef_of(pk.group[R.group - g0], enter(R, (uint32_t)((R.numel + chunk - 1) / chunk)));
-    T* p = (T*)R.p + off;
-    float* mst = MASTER ? R.master + off : nullptr;
-    float *m = (float*)R.m + off, *v = (float*)R.v + off;
+    const long long off = (long long)cw.y * VCR_OPT_CHUNK + threadIdx.x * 4, left = R.numel - off;
+    GLOBAL T* p = global((T*)R.p) + off;
+    GLOBAL float* mst = MASTER ? global(R.master) + off : nullptr;
+    GLOBAL float *m = global((float*)R.m) + off, *v = global((float*)R.v) + off;
     g += off;
-    uint32_t done = 0;
-    if (aligned(g, 16) && aligned(p, 16) && aligned(m, 16) && aligned(v, 16) && (!MASTER || aligned(mst, 16))) {
-        done = cnt / V * V;
-        for (uint32_t i = threadIdx.x * V; i < done; i += 256 * V) {
-            const Vec<V> gg = loadv<V>(g + i);
-            Vec<V> mm = loadv<V>(m + i), vv = loadv<V>(v + i), x;
-            if constexpr (MASTER) x = loadv<V>(mst + i); else x = loadv<V>(p + i);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                moments_one(mm.x[k], vv.x[k], gg.x[k] * gs, c);
-                x.x[k] = param_one(x.x[k], mm.x[k], vv.x[k], c);
-            }
-            storev<V>(m + i, mm);
-            storev<V>(v + i, vv);
-            if constexpr (MASTER) storev<V>(mst + i, x);
-            storev<V>(p + i, x);
+    const bool fit = aligned(p, g);
+    Vec<4> gg = {}, mm = {}, vv = {}, x = {};
+    if (left >= 4) {
+        gg = fit ? loadv<4, true>(g) : loadv<4, false>(g);
+        mm = loadv<4, true>(m);
+        vv = loadv<4, true>(v);
+        if constexpr (MASTER) x = loadv<4, true>(mst);
+        else x = fit ? loadv<4, true>(p) : loadv<4, false>(p);
+    } else {
+        for (int k = 0; k < left; ++k) {
+            gg.x[k] = load1(g + k); mm.x[k] = m[k]; vv.x[k] = v[k];
+            x.x[k] = MASTER ? mst[k] : load1(p + k);
         }
     }
-    for (uint32_t i = done + threadIdx.x; i < cnt; i += 256) {
-        float mm = m[i], vv = v[i];
-        moments_one(mm, vv, load1(g + i) * gs, c);
-        const float x = param_one(MASTER ? mst[i] : load1(p + i), mm, vv, c);
-        m[i] = mm; v[i] = vv;
-        if (MASTER) mst[i] = x;
-        store1(p + i, x);
+    const Entry e = enter(R, pk.group[R.group - g0]);
+    const Coef c = e.coef;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        moments_one(mm.x[k], vv.x[k], gg.x[k] * gs, c);
+        x.x[k] = param_one(x.x[k], mm.x[k], vv.x[k], c);
     }
+    if (left >= 4) {
+        storev<4, true>(m, mm);
+        storev<4, true>(v, vv);
+        if constexpr (MASTER) storev<4, true>(mst, x);
+        if (fit) storev<4, true>(p, x); else storev<4, false>(p, x);
+    } else {
+        for (int k = 0; k < left; ++k) {
+            m[k] = mm.x[k]; v[k] = vv.x[k];
+            if (MASTER) mst[k] = x.x[k];
+            store1(p + k, x.x[k]);
+        }
+    }
+    leave(R, words, cw.y, e.step);
 }
 
 // ---- update, moments in 8 bits: one wave per block of 256, four consecutive elements per lane ---------------------------
-template <typename T>
-__device__ __forceinline__ Vec<4> load_some(const T* p, uint32_t i, uint32_t cnt, bool whole) {
-    if (whole) return loadv<4>(p + i);
-    Vec<4> r;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) r.x[k] = i + k < cnt ? load1(p + i + k) : 0.f;
-    return r;
+// Maximum over a wave: within rows of 16 by lane permutations, across the four rows on the scalar side.
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 15, 15, true); }
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+    x = max(x, dpp<0xB1>(x));          // lanes 1 0 3 2
+    x = max(x, dpp<0x4E>(x));          // lanes 2 3 0 1
+    x = max(x, dpp<0x141>(x));         // halves of 8 mirrored
+    return max(x, dpp<0x140>(x));      // rows of 16 mirrored
 }
-template <typename T>
-__device__ __forceinline__ void store_some(T* p, uint32_t i, uint32_t cnt, bool whole, const Vec<4>& r) {
-    if (whole) { storev<4>(p + i, r); return; }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) if (i + k < cnt) store1(p + i + k, r.x[k]);
+__device__ __forceinline__ uint32_t rows_max(uint32_t x) {
+    const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+    const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+    return max(max(a, b), max(c, d));
 }
-__device__ __forceinline__ uint32_t codes_some(const uint8_t* p, uint32_t i, uint32_t cnt, bool whole) {
-    if (whole) return *reinterpret_cast<const uint32_t*>(p + i);
-    uint32_t r = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) if (i + k < cnt) r |= (uint32_t)p[i + k] << (8 * k);
-    return r;
+
+struct Lane8 { Vec<4> g, x; uint32_t cm, cv; };      // what a lane loads: gradient, parameter, codes
+
+// byte 3 of four words, in order
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0703u), __builtin_amdgcn_perm(b, a, 0x0C0C0703u), 0x05040100u);
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, uint32_t i, uint32_t cnt, bool whole, uint32_t r) {
-    if (whole) { *reinterpret_cast<uint32_t*>(p + i) = r; return; }
+
+// A whole block of finite numbers.  Returns false, with nothing changed, where it does not apply: a code or a moment that is not
+// finite, or a second moment below 2^-126 (the square root instruction would flush it).
+__device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, uint32_t j0, float gs, const Coef& c) {
+    // a byte 0x7F / 0xFF among the first moment's codes, a byte 0xFF among the second's
+    uint32_t odd = ((r.cm & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    odd |= ((r.cv & 0x7F7F7F7Fu) + 0x01010101u) & r.cv & 0x80808080u;
+    float m[4], v[4];
+    bool tiny = false;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) if (i + k < cnt) p[i + k] = (uint8_t)(r >> (8 * k));
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t bits = ((r.cm >> (8 * k) & 0x7Fu) << 20) | (r.cm << (24 - 8 * k) & 0x80000000u);
+        m[k] = ldexpf(__uint_as_float(bits), sm - M_TOP);
+        v[k] = ldexpf(__uint_as_float((r.cv >> (8 * k) & 0xFFu) << 20), sv - V_TOP);
+        moments_one(m[k], v[k], r.g.x[k] * gs, c);
+        tiny |= __builtin_amdgcn_classf(v[k], 0x90);               // denormal
+    }
+    const float ma = fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])));
+    const uint32_t va = max(max(__float_as_uint(v[0]), __float_as_uint(v[1])), max(__float_as_uint(v[2]), __float_as_uint(v[3])));
+    const uint32_t mr = row_max(__float_as_uint(ma)), vr = row_max(va);
+    const uint32_t mb = rows_max(mr), vb = rows_max(vr);
+    if (vb >= INF_BITS || __any(tiny | (odd != 0))) return false;          // (m' is finite where v' is)
+    sm = scale_of(mb);
+    sv = scale_of(vb);
+    uint32_t zm[4], zv[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float d = __builtin_amdgcn_sqrtf(v[k]) * c.inv_sqrt_bc2 + c.eps;
+        r.x.x[k] = r.x.x[k] * c.decay - c.step_size * (m[k] * __builtin_amdgcn_rcpf(d));
+        const uint32_t w = element_word(bkey, (j0 + k) * LANE_STEP);
+        // sign at bit 31, code at bits 20 ... 26;  code at bits 20 ... 27, at least 1 where v' > 0
+        zm[k] = __float_as_uint(ldexpf(m[k], M_TOP - sm)) + random_m(w);
+        zv[k] = max(__float_as_uint(ldexpf(v[k], V_TOP - sv)) + random_v(w), min(__float_as_uint(v[k]), 1u << 20));
+    }
+    r.cm = (top_bytes(zm[0], zm[1], zm[2], zm[3]) & 0x80808080u) | top_bytes(zm[0] << 4, zm[1] << 4, zm[2] << 4, zm[3] << 4);
+    r.cv = top_bytes(zv[0] << 4, zv[1] << 4, zv[2] << 4, zv[3] << 4);
+    return true;
+}
+
+// Any block: `n` of the lane's four elements exist.
+__device__ __forceinline__ void block_any(Lane8& r, int& sm, int& sv, uint32_t bkey, uint32_t j0, int n, float gs, const Coef& c) {
+    float m[4], v[4];
+    uint32_t mb = 0, vb = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m[k] = decode_m(r.cm >> (8 * k) & 255u, sm);
+        v[k] = decode_v(r.cv >> (8 * k) & 255u, sv);
+        moments_one(m[k], v[k], r.g.x[k] * gs, c);
+        r.x.x[k] = param_one(r.x.x[k], m[k], v[k], c);
+        if (k < n) { mb = max(mb, finite_bits(m[k])); vb = max(vb, finite_bits(v[k])); }
+    }
+    sm = scale_of(rows_max(row_max(mb)));
+    sv = scale_of(rows_max(row_max(vb)));
+    r.cm = r.cv = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t w = element_word(bkey, (j0 + k) * LANE_STEP);
+        r.cm |= encode_m(m[k], sm, random_m(w)) << (8 * k);
+        r.cv |= encode_v(v[k], sv, random_v(w)) << (8 * k);
+    }
 }
 
 template <typename T, bool MASTER>
-__global__ void __launch_bounds__(256) adamw8_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
-                                                     uint32_t chunk, const Clip* __restrict__ clip, float gscale, StepPack pk,
-                                                     int t0, int g0, uint32_t seed) {
+__global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
+                                                                 uint32_t* __restrict__ words, const Clip* __restrict__ clip, float gscale,
+                                                                 StepPack pk, int t0, int g0, uint32_t seed) {
     const uint2 cw = chunks[blockIdx.x];
-    const T* g = (const T*)pk.g[cw.x - t0];
+    const GLOBAL T* g = global((const T*)pk.g[cw.x - t0]);
     if (!g || (clip && clip->skip)) return;
     const VcrOptimTensor& R = tensors[cw.x];
     const float gs = clip ? clip->gscale : gscale;
-    const long long off = (long long)cw.y * chunk, left = R.numel - off;
-    const uint32_t cnt = left < (long long)chunk ? (uint32_t)left : chunk;
-    const int step = enter(R, (uint32_t)((R.numel + chunk - 1) / chunk));
-    const Coef c = coef_of(pk.group[R.group - g0], step);
-    T* p = (T*)R.p + off;
-    float* mst = MASTER ? R.master + off : nullptr;
-    uint8_t *mc = (uint8_t*)R.m + off, *vc = (uint8_t*)R.v + off;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j0 = (threadIdx.x & 63) * 4;
+    const uint32_t blk = cw.y * (VCR_OPT_CHUNK / VCR_OPT_BLOCK) + wave;
+    const long long first = (long long)blk * VCR_OPT_BLOCK, have = R.numel - first;    // of this wave's block; may be past the end
+    const long long off = first + j0;
+    GLOBAL T* p = global((T*)R.p) + off;
+    GLOBAL float* mst = MASTER ? global(R.master) + off : nullptr;
+    GLOBAL uint8_t *mc = global((uint8_t*)R.m) + off, *vc = global((uint8_t*)R.v) + off;
+    GLOBAL uint8_t *ms = global(R.m_scale) + blk, *vs = global(R.v_scale) + blk;
     g += off;
-    const bool al = aligned(g, 4 * sizeof(T)) && aligned(p, 4 * sizeof(T)) && aligned(mc, 4) && aligned(vc, 4) && (!MASTER || aligned(mst, 16));
-    const uint32_t j0 = (threadIdx.x & 63) * 4;
-    const uint32_t key = mix32(mix32(mix32(seed) + (uint32_t)step) + (uint32_t)R.index);
-    const uint32_t blk0 = (uint32_t)(off / VCR_OPT_BLOCK);
-    const uint8_t *ms = R.m_scale + blk0, *vs = R.v_scale + blk0;
-    for (uint32_t b = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); b * VCR_OPT_BLOCK < cnt; b += 4) {
-        const uint32_t i = b * VCR_OPT_BLOCK + j0;
-        const bool whole = al && (b + 1) * VCR_OPT_BLOCK <= cnt;
-        const int sm = ms[b], sv = vs[b];
-        const Vec<4> gg = load_some(g, i, cnt, whole);
-        Vec<4> x;
-        if constexpr (MASTER) x = load_some(mst, i, cnt, whole); else x = load_some(p, i, cnt, whole);
-        uint32_t cm = codes_some(mc, i, cnt, whole), cv = codes_some(vc, i, cnt, whole);
-        float mm[4], vv[4];
-        uint32_t mb = 0, vb = 0;
+    const bool whole = have >= VCR_OPT_BLOCK, fit = aligned(p, g);
+    const int n = whole ? 4 : have > j0 ? (int)min((long long)4, have - j0) : 0;
+    Lane8 r = {};
+    int sm = 1, sv = 1;
+    if (whole) {
+        r.g = fit ? loadv<4, true>(g) : loadv<4, false>(g);
+        if constexpr (MASTER) r.x = loadv<4, true>(mst);
+        else r.x = fit ? loadv<4, true>(p) : loadv<4, false>(p);
+        r.cm = ldq<true, u1a>(mc);
+        r.cv = ldq<true, u1a>(vc);
+    } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            mm[k] = decode_m(cm >> (8 * k) & 255u, sm);
-            vv[k] = decode_v(cv >> (8 * k) & 255u, sv);
-            moments_one(mm[k], vv[k], gg.x[k] * gs, c);
-            x.x[k] = param_one(x.x[k], mm[k], vv[k], c);
-            mb = max(mb, finite_bits(mm[k]));
-            vb = max(vb, finite_bits(vv[k]));
-        }
-        if constexpr (MASTER) store_some(mst, i, cnt, whole, x);
-        store_some(p, i, cnt, whole, x);
-        const int nm = scale_of(wave_max(mb)), nv = scale_of(wave_max(vb));
-        const uint32_t bkey = mix32(key + blk0 + b);
-        cm = cv = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t w = element_word(bkey, (j0 + k) * LANE_STEP);
-            cm |= encode_m(mm[k], nm, random_m(w)) << (8 * k);
-            cv |= encode_v(vv[k], nv, random_v(w)) << (8 * k);
-        }
-        store_codes(mc, i, cnt, whole, cm);
-        store_codes(vc, i, cnt, whole, cv);
-        if (j0 == 0) { R.m_scale[blk0 + b] = (uint8_t)nm; R.v_scale[blk0 + b] = (uint8_t)nv; }
+        for (int k = 0; k < 4; ++k)
+            if (k < n) {
+                r.g.x[k] = load1(g + k);
+                r.x.x[k] = MASTER ? mst[k] : load1(p + k);
+                r.cm |= (uint32_t)mc[k] << (8 * k);
+                r.cv |= (uint32_t)vc[k] << (8 * k);
+            }
     }
+    if (have > 0) { sm = *ms; sv = *vs; }
+    const Entry e = enter(R, pk.group[R.group - g0]);
+    if (have <= 0) return;
+    const uint32_t bkey = mix32(mix32(mix32(mix32(seed) + (uint32_t)__builtin_amdgcn_readfirstlane(e.step)) + (uint32_t)R.index) + blk);
+    sm = __builtin_amdgcn_readfirstlane(sm);
+    sv = __builtin_amdgcn_readfirstlane(sv);
+    if (!whole || !block_fast(r, sm, sv, bkey, j0, gs, e.coef)) block_any(r, sm, sv, bkey, j0, n, gs, e.coef);
+    if (whole) {
+        if constexpr (MASTER) storev<4, true>(mst, r.x);
+        if (fit) storev<4, true>(p, r.x); else storev<4, false>(p, r.x);
+        stq<true>(mc, (u1a)r.cm);
+        stq<true>(vc, (u1a)r.cv);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < n) {
+                if (MASTER) mst[k] = r.x.x[k];
+                store1(p + k, r.x.x[k]);
+                mc[k] = (uint8_t)(r.cm >> (8 * k));
+                vc[k] = (uint8_t)(r.cv >> (8 * k));
+            }
+    }
+    if (j0 == 0) { *ms = (uint8_t)sm; *vs = (uint8_t)sv; }
+    leave(R, words, cw.y, e.step);
 }
 
 // ---- codes -> values, values -> codes (to the nearest, ties to even) ------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) decode_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
-                                                     uint32_t chunk, PairPack out, int t0) {
+__global__ void __launch_bounds__(VCR_OPT_THREADS) decode_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
+                                                                 PairPack out, int t0) {
     const uint2 cw = chunks[blockIdx.x];
     const VcrOptimTensor& R = tensors[cw.x];
-    const long long off = (long long)cw.y * chunk;
-    const long long left = R.numel - off;
-    const uint32_t cnt = left < (long long)chunk ? (uint32_t)left : chunk;
-    T *mo = (T*)out.a[cw.x - t0], *vo = (T*)out.b[cw.x - t0];
-    for (uint32_t i = threadIdx.x; i < cnt; i += 256) {
-        const long long e = off + i;
-        if (mo) store1(mo + e, decode_m(((const uint8_t*)R.m)[e], R.m_scale[e / VCR_OPT_BLOCK]));
-        if (vo) store1(vo + e, decode_v(((const uint8_t*)R.v)[e], R.v_scale[e / VCR_OPT_BLOCK]));
+    const long long off = (long long)cw.y * VCR_OPT_CHUNK + threadIdx.x * 4, left = R.numel - off;
+    if (left <= 0) return;
+    GLOBAL T *mo = global((T*)out.a[cw.x - t0]), *vo = global((T*)out.b[cw.x - t0]);
+    const GLOBAL uint8_t *mc = global((const uint8_t*)R.m) + off, *vc = global((const uint8_t*)R.v) + off;
+    const int sm = global(R.m_scale)[off / VCR_OPT_BLOCK], sv = global(R.v_scale)[off / VCR_OPT_BLOCK];
+    uint32_t cm = 0, cv = 0;
+    if (left >= 4) {
+        cm = ldq<true, u1a>(mc);
+        cv = ldq<true, u1a>(vc);
+    } else {
+        for (int k = 0; k < left; ++k) { cm |= (uint32_t)mc[k] << (8 * k); cv |= (uint32_t)vc[k] << (8 * k); }
+    }
+    Vec<4> m, v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m.x[k] = decode_m(cm >> (8 * k) & 255u, sm);
+        v.x[k] = decode_v(cv >> (8 * k) & 255u, sv);
+    }
+    if (left >= 4) {
+        if (mo) storev<4, true>(mo + off, m);
+        if (vo) storev<4, true>(vo + off, v);
+    } else {
+        for (int k = 0; k < left; ++k) {
+            if (mo) store1(mo + off + k, m.x[k]);
+            if (vo) store1(vo + off + k, v.x[k]);
+        }
     }
 }
 
@@ -468,44 +572,49 @@ __device__ __forceinline__ uint32_t nearest_v(float v, int s) {
     return encode_v(v, s, 0x7FFFFu + (y >> 20 & 1u));
 }
 __global__ void __launch_bounds__(256) encode_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
-                                                     uint32_t chunk, PairPack in, int t0) {
+                                                     PairPack in, int t0) {
     const uint2 cw = chunks[blockIdx.x];
     const VcrOptimTensor& R = tensors[cw.x];
-    const long long off = (long long)cw.y * chunk;
-    const long long left = R.numel - off;
-    const uint32_t cnt = left < (long long)chunk ? (uint32_t)left : chunk;
-    const float *mi = (const float*)in.a[cw.x - t0] + off, *vi = (const float*)in.b[cw.x - t0] + off;
-    uint8_t *mc = (uint8_t*)R.m + off, *vc = (uint8_t*)R.v + off;
+    const GLOBAL float *mi = global((const float*)in.a[cw.x - t0]), *vi = global((const float*)in.b[cw.x - t0]);
+    GLOBAL uint8_t *mc = global((uint8_t*)R.m), *vc = global((uint8_t*)R.v);
     const uint32_t lane = threadIdx.x & 63;
-    for (uint32_t b = threadIdx.x >> 6; b * VCR_OPT_BLOCK < cnt; b += 4) {
-        const long long blk = off / VCR_OPT_BLOCK + b;
+    for (uint32_t b = threadIdx.x >> 6; b < VCR_OPT_CHUNK / VCR_OPT_BLOCK; b += 4) {
+        const long long blk = (long long)cw.y * (VCR_OPT_CHUNK / VCR_OPT_BLOCK) + b, first = blk * VCR_OPT_BLOCK + lane;
+        if (blk * VCR_OPT_BLOCK >= R.numel) break;
+        float m[4], v[4];
         uint32_t mb = 0, vb = 0;
-        for (uint32_t i = b * VCR_OPT_BLOCK + lane; i < cnt && i < (b + 1) * VCR_OPT_BLOCK; i += 64) {
-            mb = max(mb, finite_bits(mi[i]));
-            vb = max(vb, finite_bits(vi[i]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long i = first + 64 * k;
+            m[k] = i < R.numel ? mi[i] : 0.f;
+            v[k] = i < R.numel ? vi[i] : 0.f;
+            mb = max(mb, finite_bits(m[k]));
+            vb = max(vb, finite_bits(v[k]));
         }
-        const int nm = scale_of(wave_max(mb)), nv = scale_of(wave_max(vb));
-        for (uint32_t i = b * VCR_OPT_BLOCK + lane; i < cnt && i < (b + 1) * VCR_OPT_BLOCK; i += 64) {
-            mc[i] = (uint8_t)nearest_m(mi[i], nm);
-            vc[i] = (uint8_t)nearest_v(vi[i], nv);
+        const int nm = scale_of(rows_max(row_max(mb))), nv = scale_of(rows_max(row_max(vb)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long i = first + 64 * k;
+            if (i < R.numel) { mc[i] = (uint8_t)nearest_m(m[k], nm); vc[i] = (uint8_t)nearest_v(v[k], nv); }
         }
-        if (lane == 0) { R.m_scale[blk] = (uint8_t)nm; R.v_scale[blk] = (uint8_t)nv; }
+        if (lane == 0) { global(R.m_scale)[blk] = (uint8_t)nm; global(R.v_scale)[blk] = (uint8_t)nv; }
     }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
 inline int64_t chunks_of(int64_t numel, int64_t chunk) { return (numel + chunk - 1) / chunk; }
 inline size_t plan_head(int n) { return vcr_align(sizeof(VcrOptimTensor) * (size_t)n); }
-inline bool chunk_ok(int chunk) { return chunk >= 1024 && chunk % 1024 == 0 && chunk <= (1 << 20); }
+inline size_t plan_words(int n, int64_t chunks) { return vcr_align(plan_head(n) + sizeof(uint2) * (size_t)chunks); }
+inline uint32_t tickets_of(int64_t chunks) { return chunks > TICKET_FLAT ? 1 + TICKET_GROUPS : 1; }
 inline const uint2* plan_chunks(const void* plan, int n) { return (const uint2*)((const char*)plan + plan_head(n)); }
 
 // checks that the calls on a plan share; returns the number of chunks, -1 with an error set
-int64_t plan_check(const char* who, const void* plan, int n, const int64_t* numel, int chunk) {
-    if (!plan || !numel || n < 1 || !chunk_ok(chunk)) { vcr_set_error("%s: plan, numel or chunk is missing or out of range", who); return -1; }
+int64_t plan_check(const char* who, const void* plan, int n, const int64_t* numel) {
+    if (!plan || !numel || n < 1) { vcr_set_error("%s: plan or numel is missing", who); return -1; }
     int64_t total = 0;
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0) { vcr_set_error("%s: tensor %d has numel %lld", who, k, (long long)numel[k]); return -1; }
-        total += chunks_of(numel[k], chunk);
+        total += chunks_of(numel[k], VCR_OPT_CHUNK);
     }
     if (total > 0x7FFFFFFF) { vcr_set_error("%s: %lld chunks", who, (long long)total); return -1; }
     return total;
@@ -550,32 +659,44 @@ int list_check(const char* who, int n, const void* const* tensors, const int64_t
 
 }  // namespace
 
-extern "C" size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel, int chunk) {
-    if (ntensors < 1 || !numel || !chunk_ok(chunk)) return 0;
-    size_t total = 0;
-    for (int k = 0; k < ntensors; ++k) total += numel[k] > 0 ? (size_t)chunks_of(numel[k], chunk) : 0;
-    return plan_head(ntensors) + sizeof(uint2) * total;
+extern "C" size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel) {
+    if (ntensors < 1 || !numel) return 0;
+    int64_t total = 0;
+    size_t tickets = 0;
+    for (int k = 0; k < ntensors; ++k) {
+        const int64_t nc = numel[k] > 0 ? chunks_of(numel[k], VCR_OPT_CHUNK) : 0;
+        total += nc;
+        tickets += tickets_of(nc);
+    }
+    return plan_words(ntensors, total) + tickets * TICKET_STRIDE * sizeof(uint32_t);
 }
 
-extern "C" int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, int chunk, void* host_plan, size_t bytes) {
-    if (ntensors < 1 || !tensors || !host_plan || !chunk_ok(chunk)) { vcr_set_error("vcr_optim_plan: tensors, plan or chunk is missing or out of range"); return 1; }
-    size_t total = 0;
+extern "C" int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, void* host_plan, size_t bytes) {
+    if (ntensors < 1 || !tensors || !host_plan) { vcr_set_error("vcr_optim_plan: tensors or plan is missing"); return 1; }
+    int64_t total = 0;
+    size_t tickets = 0;
     for (int k = 0; k < ntensors; ++k) {
         const VcrOptimTensor& t = tensors[k];
-        if (t.numel < 0 || !t.step || !t.arrived || (t.numel > 0 && (!t.p || !t.m || !t.v)) || (!t.m_scale != !t.v_scale)) {
+        if (t.numel < 0 || !t.step || (t.numel > 0 && (!t.p || !t.m || !t.v)) || (!t.m_scale != !t.v_scale)) {
             vcr_set_error("vcr_optim_plan: tensor %d has numel %lld and a pointer missing", k, (long long)t.numel);
             return 1;
         }
-        total += (size_t)chunks_of(t.numel, chunk);
+        total += chunks_of(t.numel, VCR_OPT_CHUNK);
+        tickets += tickets_of(chunks_of(t.numel, VCR_OPT_CHUNK));
     }
-    if (total > 0x7FFFFFFF || bytes < plan_head(ntensors) + sizeof(uint2) * total) { vcr_set_error("vcr_optim_plan: %zu bytes for %zu chunks", bytes, total); return 1; }
+    const size_t words = plan_words(ntensors, total), need = words + tickets * TICKET_STRIDE * sizeof(uint32_t);
+    if (total > 0x7FFFFFFF || tickets > 0x7FFFFFFF || bytes < need) { vcr_set_error("vcr_optim_plan: %zu bytes for %lld chunks", bytes, (long long)total); return 1; }
     VcrOptimTensor* out = (VcrOptimTensor*)host_plan;
     uint2* c = (uint2*)((char*)host_plan + plan_head(ntensors));
+    int32_t word = 0;
     for (int k = 0; k < ntensors; ++k) {
+        const uint32_t nc = (uint32_t)chunks_of(tensors[k].numel, VCR_OPT_CHUNK);
         out[k] = tensors[k];
-        const uint32_t nc = (uint32_t)chunks_of(tensors[k].numel, chunk);
+        out[k].words = word;
+        word += (int32_t)tickets_of(nc);
         for (uint32_t i = 0; i < nc; ++i) *c++ = make_uint2((uint32_t)k, i);
     }
+    memset((char*)host_plan + words, 0, need - words);
     return 0;
 }
 
@@ -583,7 +704,8 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
     if (!args) { vcr_set_error("vcr_adamw_step: args is NULL"); return 1; }
     const VcrAdamWStep& a = *args;
     if (a.ntensors == 0) return 0;
-    if (plan_check("vcr_adamw_step", a.plan, a.ntensors, a.numel, a.chunk) < 0) return 1;
+    const int64_t nall = plan_check("vcr_adamw_step", a.plan, a.ntensors, a.numel);
+    if (nall < 0) return 1;
     if (!a.grads || !a.groups || !a.group_of || a.ngroups < 1 || a.param_type < 0 || a.param_type > VCR_F16 ||
         (a.state_bits != 32 && a.state_bits != 8) || (a.masters && a.param_type == VCR_F32)) {
         vcr_set_error("vcr_adamw_step: inconsistent arguments");
@@ -604,6 +726,7 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     const VcrOptimTensor* tensors = (const VcrOptimTensor*)a.plan;
     const uint2* chunks = plan_chunks(a.plan, a.ntensors);
+    uint32_t* words = (uint32_t*)((char*)a.plan + plan_words(a.ntensors, nall));
     const Clip* clip = (const Clip*)a.clip;
     for (int t0 = 0, t1 = 0; t0 < a.ntensors; t0 = t1) {
         StepPack pk = {};
@@ -612,7 +735,7 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
         const int g0 = a.group_of[t0];
         for (; t1 < a.ntensors && t1 - t0 < VCR_OPT_TENSORS && a.group_of[t1] - g0 < VCR_OPT_GROUPS; ++t1) {
             pk.g[t1 - t0] = a.grads[t1];
-            nchunks += chunks_of(a.numel[t1], a.chunk);
+            nchunks += chunks_of(a.numel[t1], VCR_OPT_CHUNK);
             any |= a.grads[t1] != nullptr && a.numel[t1] > 0;
         }
         for (int k = g0; k <= a.group_of[t1 - 1]; ++k) {
@@ -621,10 +744,10 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
                                 (float)g.beta1, (float)(1.0 - g.beta1), (float)g.beta2, (float)(1.0 - g.beta2), 0};
         }
         if (any) {
-            const dim3 grid((uint32_t)nchunks), block(256);
+            const dim3 grid((uint32_t)nchunks), block(VCR_OPT_THREADS);
             const float gs = (float)a.grad_scale;
-#define LAUNCH32(T, M) hipLaunchKernelGGL((adamw_kernel<T, M>), grid, block, 0, st, tensors, chunks, (uint32_t)a.chunk, clip, gs, pk, t0, g0)
-#define LAUNCH8(T, M) hipLaunchKernelGGL((adamw8_kernel<T, M>), grid, block, 0, st, tensors, chunks, (uint32_t)a.chunk, clip, gs, pk, t0, g0, a.seed)
+#define LAUNCH32(T, M) hipLaunchKernelGGL((adamw_kernel<T, M>), grid, block, 0, st, tensors, chunks, words, clip, gs, pk, t0, g0)
+#define LAUNCH8(T, M) hipLaunchKernelGGL((adamw8_kernel<T, M>), grid, block, 0, st, tensors, chunks, words, clip, gs, pk, t0, g0, a.seed)
 #define LAUNCH(T, M) do { if (a.state_bits == 32) LAUNCH32(T, M); else LAUNCH8(T, M); } while (0)
             if (a.param_type == VCR_F32) LAUNCH(float, false);
             else if (a.param_type == VCR_BF16) { if (a.masters) LAUNCH(__hip_bfloat16, true); else LAUNCH(__hip_bfloat16, false); }
@@ -639,10 +762,10 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
     return 0;
 }
 
-static int pairs_call(const char* who, int n, const void* plan, const int64_t* numel, int chunk, const void* const* a, const void* const* b,
+static int pairs_call(const char* who, int n, const void* plan, const int64_t* numel, const void* const* a, const void* const* b,
                       int type, bool encode, hipStream_t st) {
     if (n == 0) return 0;
-    if (plan_check(who, plan, n, numel, chunk) < 0) return 1;
+    if (plan_check(who, plan, n, numel) < 0) return 1;
     if (!a || !b || type < 0 || type > VCR_F16) { vcr_set_error("%s: inconsistent arguments", who); return 1; }
     const VcrOptimTensor* tensors = (const VcrOptimTensor*)plan;
     const uint2* chunks = plan_chunks(plan, n);
@@ -653,14 +776,14 @@ static int pairs_call(const char* who, int n, const void* plan, const int64_t* n
             pk.a[k] = a[t0 + k];
             pk.b[k] = b[t0 + k];
             if (encode && numel[t0 + k] > 0 && (!pk.a[k] || !pk.b[k])) { vcr_set_error("%s: values of tensor %d are missing", who, t0 + k); return 1; }
-            nchunks += chunks_of(numel[t0 + k], chunk);
+            nchunks += chunks_of(numel[t0 + k], VCR_OPT_CHUNK);
         }
         if (nchunks > 0) {
-            const dim3 grid((uint32_t)nchunks), block(256);
-            if (encode) hipLaunchKernelGGL(encode_kernel, grid, block, 0, st, tensors, chunks, (uint32_t)chunk, pk, t0);
-            else if (type == VCR_F32) hipLaunchKernelGGL(decode_kernel<float>, grid, block, 0, st, tensors, chunks, (uint32_t)chunk, pk, t0);
-            else if (type == VCR_BF16) hipLaunchKernelGGL(decode_kernel<__hip_bfloat16>, grid, block, 0, st, tensors, chunks, (uint32_t)chunk, pk, t0);
-            else hipLaunchKernelGGL(decode_kernel<__half>, grid, block, 0, st, tensors, chunks, (uint32_t)chunk, pk, t0);
+            const dim3 grid((uint32_t)nchunks), block(encode ? 256 : VCR_OPT_THREADS);
+            if (encode) hipLaunchKernelGGL(encode_kernel, grid, block, 0, st, tensors, chunks, pk, t0);
+            else if (type == VCR_F32) hipLaunchKernelGGL(decode_kernel<float>, grid, block, 0, st, tensors, chunks, pk, t0);
+            else if (type == VCR_BF16) hipLaunchKernelGGL(decode_kernel<__hip_bfloat16>, grid, block, 0, st, tensors, chunks, pk, t0);
+            else hipLaunchKernelGGL(decode_kernel<__half>, grid, block, 0, st, tensors, chunks, pk, t0);
         }
         chunks += nchunks;
     }
@@ -668,13 +791,13 @@ static int pairs_call(const char* who, int n, const void* plan, const int64_t* n
     return 0;
 }
 
-extern "C" int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, int chunk, void* const* exp_avg,
+extern "C" int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, void* const* exp_avg,
                                    void* const* exp_avg_sq, int type, void* stream) {
-    return pairs_call("vcr_moments8_decode", ntensors, plan, numel, chunk, exp_avg, exp_avg_sq, type, false, (hipStream_t)stream);
+    return pairs_call("vcr_moments8_decode", ntensors, plan, numel, exp_avg, exp_avg_sq, type, false, (hipStream_t)stream);
 }
-extern "C" int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, int chunk, const float* const* exp_avg,
+extern "C" int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, const float* const* exp_avg,
                                    const float* const* exp_avg_sq, void* stream) {
-    return pairs_call("vcr_moments8_encode", ntensors, plan, numel, chunk, (const void* const*)exp_avg, (const void* const*)exp_avg_sq, VCR_F32,
+    return pairs_call("vcr_moments8_encode", ntensors, plan, numel, (const void* const*)exp_avg, (const void* const*)exp_avg_sq, VCR_F32,
                       true, (hipStream_t)stream);
 }
 

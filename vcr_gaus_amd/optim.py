@@ -14,7 +14,6 @@ import torch
 from . import _lib
 
 BLOCK = 256                                    # elements that share the scale of an 8-bit moment
-CHUNK = 4096                                   # elements per workgroup
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _PTR, _CONTIGUOUS, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
 _GRAD, _DTYPE, _DEVICE, _LAYOUT = attrgetter("grad"), attrgetter("dtype"), attrgetter("device"), attrgetter("layout")
@@ -153,7 +152,7 @@ class _Bucket:
 
 
 class _Plan:
-    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "buckets", "arrived", "device", "stream", "captured", "covered")
+    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "buckets", "device", "stream", "captured", "covered")
 
 
 class AdamW:
@@ -233,7 +232,7 @@ class AdamW:
             if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
                 raise ValueError(f"AdamW: group {k}: a tensor `lr` must be one float32 element on the device")
             dev, lr = lr.data_ptr(), 0.0
-        if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and wd >= 0.0):
+        if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and (eps == 0.0 or eps >= 2.0 ** -126) and wd >= 0.0):
             raise ValueError(f"AdamW: group {k}: lr {lr}, betas {(b1, b2)}, eps {eps}, weight_decay {wd} out of range")
         return _lib.VcrOptimGroup(float(lr), float(b1), float(b2), float(eps), float(wd), dev)
 
@@ -289,8 +288,6 @@ class AdamW:
             self._check_state(key, p, self.state[key])
             by.setdefault(_TYPES[p.dtype], []).append(i)
         plan.buckets, plan.covered = [], sum(map(len, by.values()))
-        plan.arrived = torch.zeros(max(1, plan.covered), dtype=torch.int32, device=plan.device)
-        word = plan.arrived.data_ptr()
         for kind, at in by.items():
             b = _Bucket()
             b.type, b.at, b.n, b.every = kind, at, len(at), len(at) == len(plan.params)
@@ -301,16 +298,15 @@ class AdamW:
                 p, st = plan.params[i], self.state[keys[i]]
                 ptr = lambda k: st[k].data_ptr() if k in st else None  # noqa: E731
                 r.p, r.master, r.numel, r.group, r.index = p.data_ptr(), ptr("master") if self._has_master(p) else None, p.numel(), groups_of[i], i
-                r.m, r.v, r.step, r.arrived = ptr("exp_avg"), ptr("exp_avg_sq"), ptr("step"), word
-                word += 4
+                r.m, r.v, r.step = ptr("exp_avg"), ptr("exp_avg_sq"), ptr("step")
                 if self.state_bits == 8 and p.numel():
                     r.m_scale, r.v_scale = ptr("exp_avg_scale"), ptr("exp_avg_sq_scale")
-            size = lib.vcr_optim_plan_bytes(b.n, b.numels, CHUNK)
+            size = lib.vcr_optim_plan_bytes(b.n, b.numels)
             host = torch.empty(size, dtype=torch.uint8)
-            _lib.check(lib.vcr_optim_plan(b.n, rec, CHUNK, host.data_ptr(), size))
+            _lib.check(lib.vcr_optim_plan(b.n, rec, host.data_ptr(), size))
             b.plan = host.to(plan.device)
             b.grads = (C.c_void_p * b.n)()
-            b.args = _lib.VcrAdamWStep(ntensors=b.n, chunk=CHUNK, param_type=kind, state_bits=self.state_bits,
+            b.args = _lib.VcrAdamWStep(ntensors=b.n, param_type=kind, state_bits=self.state_bits,
                                        masters=int(self.master_weights and kind != 0), seed=self.seed, plan=b.plan.data_ptr(),
                                        grads=b.grads, numel=b.numels, group_of=b.group_of)
             plan.buckets.append(b)
@@ -334,7 +330,6 @@ class AdamW:
         if stream.cuda_stream != plan.stream:
             for b in plan.buckets:
                 b.plan.record_stream(stream)
-            plan.arrived.record_stream(stream)
         if not plan.captured and torch.cuda.is_current_stream_capturing():
             plan.captured = True
             self._captured.append(plan)          # the graph holds its addresses
@@ -441,7 +436,7 @@ class AdamW:
             kind = _TYPES[kinds.pop()]
             for b in plan.buckets:
                 m, v = (_pointers([o[i].data_ptr() for i in b.at]) for o in outs)
-                _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), b.numels, CHUNK, m, v, kind, stream))
+                _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), b.numels, m, v, kind, stream))
         return outs
 
     @torch.no_grad()
@@ -548,12 +543,12 @@ def _single(st, n):
     rec = (_lib.VcrOptimTensor * 1)()
     rec[0].p = rec[0].m = st["exp_avg"].data_ptr()
     rec[0].v, rec[0].m_scale, rec[0].v_scale = (st[k].data_ptr() for k in ("exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"))
-    rec[0].step = rec[0].arrived = st["exp_avg"].data_ptr()               # (unused by these kernels, but not optional)
+    rec[0].step = st["exp_avg"].data_ptr()               # (not used by these kernels, but not optional)
     rec[0].numel = n
     ns = _numels([n])
-    size = lib.vcr_optim_plan_bytes(1, ns, CHUNK)
+    size = lib.vcr_optim_plan_bytes(1, ns)
     host = torch.empty(size, dtype=torch.uint8)
-    _lib.check(lib.vcr_optim_plan(1, rec, CHUNK, host.data_ptr(), size))
+    _lib.check(lib.vcr_optim_plan(1, rec, host.data_ptr(), size))
     return host.to(dev), ns
 
 
@@ -565,7 +560,7 @@ def encode8(exp_avg, exp_avg_sq, st):
     if dev.type != "cuda":
         raise ValueError("8-bit moments need a HIP device")
     plan, ns = _single(st, exp_avg.numel())
-    _lib.check(_on(dev, _lib.load().vcr_moments8_encode, 1, plan.data_ptr(), ns, CHUNK, _pointers([exp_avg.data_ptr()]),
+    _lib.check(_on(dev, _lib.load().vcr_moments8_encode, 1, plan.data_ptr(), ns, _pointers([exp_avg.data_ptr()]),
                    _pointers([exp_avg_sq.data_ptr()]), _lib.stream_of(st["exp_avg"])))
 
 
@@ -577,6 +572,6 @@ def decode8(st, p):
         if dev.type != "cuda":
             raise ValueError("8-bit moments need a HIP device")
         plan, ns = _single(st, p.numel())
-        _lib.check(_on(dev, _lib.load().vcr_moments8_decode, 1, plan.data_ptr(), ns, CHUNK, *[_pointers([o.data_ptr()]) for o in outs], 0,
+        _lib.check(_on(dev, _lib.load().vcr_moments8_decode, 1, plan.data_ptr(), ns, *[_pointers([o.data_ptr()]) for o in outs], 0,
                        _lib.stream_of(st["exp_avg"])))
     return outs
