@@ -24,8 +24,15 @@
 namespace {
 
 #define VCR_OPT_BLOCK 256          // elements that share a scale
-#define VCR_OPT_THREADS 1024
-#define VCR_OPT_CHUNK 4096         // elements per workgroup of the update kernels
+#define VCR_OPT_CHUNK 4096         // elements per entry of a plan
+// Threads per workgroup, four elements each and no loop: a workgroup reads, computes, writes and is gone, so that the ones in
+// flight work on neighbouring memory (400 M elements: 2 008 us with four rounds of 1024 elements per workgroup, 1 929 us with one).
+#define VCR_OPT_THREADS 256
+// LDS that a workgroup of the fp32 update asks for and does not use: it leaves 4 workgroups on a compute unit instead of 8.  With
+// fewer waves the memory sees longer runs of reads and of writes: 400 M elements 1 929 -> 1 857 us, 1 M Gaussians 279 -> 265 us (6.2
+// TB/s).  16-bit parameters lose by it (9 M fp16 elements, one off alignment: 37 -> 43 us), the 8-bit update, which is bound by its
+// instructions, more still (771 -> 1 099 us).
+#define VCR_OPT_LDS_FP32 40000
 #define VCR_OPT_TENSORS 352        // tensors and ...
 #define VCR_OPT_GROUPS 14          // ... hyper-parameter groups per launch: both travel in the kernel arguments (4 KB)
 #define VCR_OPT_NORM_TENSORS 192   // tensors per launch of the norm kernel
@@ -275,6 +282,14 @@ __global__ void __launch_bounds__(256) scale_kernel(NormPack pk, int n, uint32_t
 // workgroup forms its tensor's factors itself from the counter: its first wave does, lanes 0 and 1 sharing one expm1,
 // while the data loads of all waves are in flight.  The counter may move only when every workgroup of the tensor has read
 // it: each draws a ticket after its read, the last one writes.
+struct Place { uint32_t tensor, part; long long first; };
+// Which elements a workgroup takes, 4 ROUNDS per thread; VCR_OPT_CHUNK / (1024 ROUNDS) workgroups share an entry of the plan.
+template <int ROUNDS> constexpr uint32_t parts() { return VCR_OPT_CHUNK / (4 * VCR_OPT_THREADS * ROUNDS); }
+template <int ROUNDS> __device__ __forceinline__ Place place(const uint2* __restrict__ chunks) {
+    const uint2 c = chunks[blockIdx.x / parts<ROUNDS>()];
+    const uint32_t part = blockIdx.x % parts<ROUNDS>();
+    return {c.x, c.y * parts<ROUNDS>() + part, (long long)c.y * VCR_OPT_CHUNK + part * (4 * VCR_OPT_THREADS * ROUNDS)};
+}
 __device__ __forceinline__ float from_lane(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
 
 __device__ __forceinline__ Coef coef_of(const Group& G, int t) {
@@ -302,17 +317,17 @@ __device__ __forceinline__ bool last_of(GLOBAL uint32_t* word, uint32_t of) {
     __hip_atomic_store(word, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return true;
 }
-__device__ __forceinline__ void leave(const VcrOptimTensor& R, uint32_t* words, uint32_t c, int step) {
+template <int ROUNDS> __device__ __forceinline__ void leave(const VcrOptimTensor& R, uint32_t* words, const Place& at, int step) {
     if (threadIdx.x != 0) return;
-    const uint32_t nchunks = (uint32_t)((R.numel + VCR_OPT_CHUNK - 1) / VCR_OPT_CHUNK);
+    const uint32_t nchunks = (uint32_t)((R.numel + VCR_OPT_CHUNK - 1) / VCR_OPT_CHUNK), n = nchunks * parts<ROUNDS>();
     bool last = true;
-    if (nchunks > 1) {
+    if (n > 1) {
         GLOBAL uint32_t* w = global(words) + (size_t)R.words * TICKET_STRIDE;
         if (nchunks <= TICKET_FLAT) {
-            last = last_of(w, nchunks);
+            last = last_of(w, n);
         } else {
-            const uint32_t g = c % TICKET_GROUPS;
-            last = last_of(w + (1 + g) * TICKET_STRIDE, (nchunks - g + TICKET_GROUPS - 1) / TICKET_GROUPS) && last_of(w, TICKET_GROUPS);
+            const uint32_t g = at.part % TICKET_GROUPS;
+            last = last_of(w + (1 + g) * TICKET_STRIDE, (n - g + TICKET_GROUPS - 1) / TICKET_GROUPS) && last_of(w, TICKET_GROUPS);
         }
     }
     if (last) *global(R.step) = step;
@@ -335,12 +350,12 @@ template <typename T, bool MASTER>
 __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
                                                                 uint32_t* __restrict__ words, const Clip* __restrict__ clip, float gscale,
                                                                 StepPack pk, int t0, int g0) {
-    const uint2 cw = chunks[blockIdx.x];
-    const GLOBAL T* g = global((const T*)pk.g[cw.x - t0]);
+    const Place at = place<1>(chunks);
+    const GLOBAL T* g = global((const T*)pk.g[at.tensor - t0]);
     if (!g || (clip && clip->skip)) return;
-    const VcrOptimTensor& R = tensors[cw.x];
+    const VcrOptimTensor& R = tensors[at.tensor];
     const float gs = clip ? clip->gscale : gscale;
-    const long long off = (long long)cw.y * VCR_OPT_CHUNK + threadIdx.x * 4, left = R.numel - off;
+    const long long off = at.first + threadIdx.x * 4, left = R.numel - off;
     GLOBAL T* p = global((T*)R.p) + off;
     GLOBAL float* mst = MASTER ? global(R.master) + off : nullptr;
     GLOBAL float *m = global((float*)R.m) + off, *v = global((float*)R.v) + off;
@@ -354,10 +369,12 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
         if constexpr (MASTER) x = loadv<4, true>(mst);
         else x = fit ? loadv<4, true>(p) : loadv<4, false>(p);
     } else {
-        for (int k = 0; k < left; ++k) {
-            gg.x[k] = load1(g + k); mm.x[k] = m[k]; vv.x[k] = v[k];
-            x.x[k] = MASTER ? mst[k] : load1(p + k);
-        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < left) {
+                gg.x[k] = load1(g + k); mm.x[k] = m[k]; vv.x[k] = v[k];
+                x.x[k] = MASTER ? mst[k] : load1(p + k);
+            }
     }
     const Entry e = enter(R, pk.group[R.group - g0]);
     const Coef c = e.coef;
@@ -372,13 +389,15 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
         if constexpr (MASTER) storev<4, true>(mst, x);
         if (fit) storev<4, true>(p, x); else storev<4, false>(p, x);
     } else {
-        for (int k = 0; k < left; ++k) {
-            m[k] = mm.x[k]; v[k] = vv.x[k];
-            if (MASTER) mst[k] = x.x[k];
-            store1(p + k, x.x[k]);
-        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < left) {
+                m[k] = mm.x[k]; v[k] = vv.x[k];
+                if (MASTER) mst[k] = x.x[k];
+                store1(p + k, x.x[k]);
+            }
     }
-    leave(R, words, cw.y, e.step);
+    leave<1>(R, words, at, e.step);
 }
 
 // ---- update, moments in 8 bits: one wave per block of 256, four consecutive elements per lane ---------------------------
@@ -397,52 +416,71 @@ __device__ __forceinline__ uint32_t rows_max(uint32_t x) {
 }
 
 struct Lane8 { Vec<4> g, x; uint32_t cm, cv; };      // what a lane loads: gradient, parameter, codes
+typedef float f2 __attribute__((ext_vector_type(2)));
 
 // byte 3 of four words, in order
 __device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0703u), __builtin_amdgcn_perm(b, a, 0x0C0C0703u), 0x05040100u);
 }
+__device__ __forceinline__ float power(int field) { return __uint_as_float((uint32_t)field << 23); }      // 2^(field - 127), 1 <= field <= 254
+// block exponents for which every power of two below is a normal number, and no value that the codes stand for is denormal
+#define M_LOW 40
+#define M_HIGH 139
+#define V_LOW 40
+#define V_HIGH 155
 
-// A whole block of finite numbers.  Returns false, with nothing changed, where it does not apply: a code or a moment that is not
-// finite, or a second moment below 2^-126 (the square root instruction would flush it).
-__device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, uint32_t j0, float gs, const Coef& c) {
+// A whole block of finite numbers of ordinary size: the definition above with its scalings as multiplications by powers of two
+// (exact, so that b2 and the scale of v are one factor), the first moment's codes decoded by the hardware (they are OCP e4m3:
+// bias 7, code exponent 14 = 2^7), and everything shifted up by 4 so that a code is the top byte of its word.  Returns false, with
+// nothing changed, where it does not apply: a code or a moment that is not finite, block exponents out of the ranges above, or a
+// second moment below 2^-126 (the square root instruction would flush it).
+__device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], float gs, const Coef& c) {
+#pragma clang fp contract(off)
+    if (sm < M_LOW || sm > M_HIGH || sv < V_LOW || sv > V_HIGH) return false;
     // a byte 0x7F / 0xFF among the first moment's codes, a byte 0xFF among the second's
     uint32_t odd = ((r.cm & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
     odd |= ((r.cv & 0x7F7F7F7Fu) + 0x01010101u) & r.cv & 0x80808080u;
-    float m[4], v[4];
+    const float m_scale = power(sm - 7), v_scale = power(sv - V_TOP + 127) * c.b2;
+    const f2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(r.cm, m_scale, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(r.cm, m_scale, true);
+    float m[4] = {lo.x, lo.y, hi.x, hi.y}, v[4];
     bool tiny = false;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const uint32_t bits = ((r.cm >> (8 * k) & 0x7Fu) << 20) | (r.cm << (24 - 8 * k) & 0x80000000u);
-        m[k] = ldexpf(__uint_as_float(bits), sm - M_TOP);
-        v[k] = ldexpf(__uint_as_float((r.cv >> (8 * k) & 0xFFu) << 20), sv - V_TOP);
-        moments_one(m[k], v[k], r.g.x[k] * gs, c);
+        const float g = r.g.x[k] * gs;
+        m[k] = m[k] * c.b1 + g * c.omb1;
+        v[k] = __uint_as_float(k < 3 ? (r.cv << (20 - 8 * k)) & 0x0FF00000u : (r.cv >> 4) & 0x0FF00000u) * v_scale + (g * g) * c.omb2;
         tiny |= __builtin_amdgcn_classf(v[k], 0x90);               // denormal
     }
     const float ma = fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])));
     const uint32_t va = max(max(__float_as_uint(v[0]), __float_as_uint(v[1])), max(__float_as_uint(v[2]), __float_as_uint(v[3])));
     const uint32_t mr = row_max(__float_as_uint(ma)), vr = row_max(va);
-    const uint32_t mb = rows_max(mr), vb = rows_max(vr);
-    if (vb >= INF_BITS || __any(tiny | (odd != 0))) return false;          // (m' is finite where v' is)
-    sm = scale_of(mb);
-    sv = scale_of(vb);
+    const uint32_t mb = rows_max(mr), vb = rows_max(vr);                     // (m' is finite where v' is)
+    const int nm = (int)(mb >> 23), nv = (int)(vb >> 23);
+    if (nm < M_LOW || nm > M_HIGH || nv < V_LOW || nv > V_HIGH || __any(tiny | (odd != 0))) return false;
+    sm = nm;
+    sv = nv;
+    const float m_up = power(M_TOP - nm + 127), v_up = power(V_TOP - nv + 127);
     uint32_t zm[4], zv[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float d = __builtin_amdgcn_sqrtf(v[k]) * c.inv_sqrt_bc2 + c.eps;
-        r.x.x[k] = r.x.x[k] * c.decay - c.step_size * (m[k] * __builtin_amdgcn_rcpf(d));
-        const uint32_t w = element_word(bkey, (j0 + k) * LANE_STEP);
-        // sign at bit 31, code at bits 20 ... 26;  code at bits 20 ... 27, at least 1 where v' > 0
-        zm[k] = __float_as_uint(ldexpf(m[k], M_TOP - sm)) + random_m(w);
-        zv[k] = max(__float_as_uint(ldexpf(v[k], V_TOP - sv)) + random_v(w), min(__float_as_uint(v[k]), 1u << 20));
+        {
+#pragma clang fp contract(fast)
+            const float d = __builtin_amdgcn_sqrtf(v[k]) * c.inv_sqrt_bc2 + c.eps;
+            r.x.x[k] = r.x.x[k] * c.decay - c.step_size * (m[k] * __builtin_amdgcn_rcpf(d));
+        }
+        const uint32_t w = element_word(bkey, j_step[k]);
+        zm[k] = (__float_as_uint(fabsf(m[k]) * m_up) << 4) + ((w >> 8 & 0xFFFF00u) | 0x80u);
+        const uint32_t y = max(__float_as_uint(v[k] * v_up), min(__float_as_uint(v[k]), 1u << 20));          // (at least 1 where v' > 0)
+        zv[k] = (y << 4) + ((w << 8 & 0xFFFF00u) | 0x80u);
     }
-    r.cm = (top_bytes(zm[0], zm[1], zm[2], zm[3]) & 0x80808080u) | top_bytes(zm[0] << 4, zm[1] << 4, zm[2] << 4, zm[3] << 4);
-    r.cv = top_bytes(zv[0] << 4, zv[1] << 4, zv[2] << 4, zv[3] << 4);
+    const uint32_t sign = top_bytes(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])) & 0x80808080u;
+    r.cm = sign | top_bytes(zm[0], zm[1], zm[2], zm[3]);
+    r.cv = top_bytes(zv[0], zv[1], zv[2], zv[3]);
     return true;
 }
 
 // Any block: `n` of the lane's four elements exist.
-__device__ __forceinline__ void block_any(Lane8& r, int& sm, int& sv, uint32_t bkey, uint32_t j0, int n, float gs, const Coef& c) {
+__device__ __forceinline__ void block_any(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], int n, float gs, const Coef& c) {
     float m[4], v[4];
     uint32_t mb = 0, vb = 0;
 #pragma unroll
@@ -458,85 +496,118 @@ __device__ __forceinline__ void block_any(Lane8& r, int& sm, int& sv, uint32_t b
     r.cm = r.cv = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const uint32_t w = element_word(bkey, (j0 + k) * LANE_STEP);
+        const uint32_t w = element_word(bkey, j_step[k]);
         r.cm |= encode_m(m[k], sm, random_m(w)) << (8 * k);
         r.cv |= encode_v(v[k], sv, random_v(w)) << (8 * k);
     }
 }
 
+// One block: addresses of its first elements (the same in every lane: the lane's offset j0 is added by the accesses themselves), how
+// many of the lane's four elements exist.
+template <typename T> struct Block8 {
+    const GLOBAL T* g;
+    GLOBAL T* p;
+    GLOBAL float* mst;
+    GLOBAL uint8_t *mc, *vc;
+    bool whole, fit;
+    int n;
+};
+template <typename T, bool MASTER>
+__device__ __forceinline__ Lane8 load_block(const Block8<T>& b, uint32_t j0) {
+    Lane8 r = {};
+    if (b.whole) {
+        r.g = b.fit ? loadv<4, true>(b.g + j0) : loadv<4, false>(b.g + j0);
+        if constexpr (MASTER) r.x = loadv<4, true>(b.mst + j0);
+        else r.x = b.fit ? loadv<4, true>((const GLOBAL T*)b.p + j0) : loadv<4, false>((const GLOBAL T*)b.p + j0);
+        r.cm = ldq<true, u1a>(b.mc + j0);
+        r.cv = ldq<true, u1a>(b.vc + j0);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < b.n) {
+                r.g.x[k] = load1(b.g + j0 + k);
+                r.x.x[k] = MASTER ? b.mst[j0 + k] : load1((const GLOBAL T*)b.p + j0 + k);
+                r.cm |= (uint32_t)b.mc[j0 + k] << (8 * k);
+                r.cv |= (uint32_t)b.vc[j0 + k] << (8 * k);
+            }
+    }
+    return r;
+}
+template <typename T, bool MASTER>
+__device__ __forceinline__ void store_block(const Block8<T>& b, uint32_t j0, const Lane8& r) {
+    if (b.whole) {
+        if constexpr (MASTER) storev<4, true>(b.mst + j0, r.x);
+        if (b.fit) storev<4, true>(b.p + j0, r.x); else storev<4, false>(b.p + j0, r.x);
+        stq<true>(b.mc + j0, (u1a)r.cm);
+        stq<true>(b.vc + j0, (u1a)r.cv);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < b.n) {
+                if (MASTER) b.mst[j0 + k] = r.x.x[k];
+                store1(b.p + j0 + k, r.x.x[k]);
+                b.mc[j0 + k] = (uint8_t)(r.cm >> (8 * k));
+                b.vc[j0 + k] = (uint8_t)(r.cv >> (8 * k));
+            }
+    }
+}
+
+// Blocks of a wave, one after another.  What every wave does once (addresses, factors) is a third of its instructions with one block:
+// 16-bit parameters without masters (10 bytes an element) are bound by instructions and take four (302 M elements 763, 637, 593 us
+// with 1, 2, 4 blocks), with masters two (19 M elements in odd sizes 57.5, 49.4, 51.0 us); fp32 (16 bytes) is bound by memory, which
+// favours short runs of a workgroup, and takes one (295 M elements 761, 862, 899 us; 6.2 TB/s).
+template <typename T, bool MASTER> constexpr int blocks8() { return sizeof(T) == 4 ? 1 : MASTER ? 2 : 4; }
 template <typename T, bool MASTER>
 __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
                                                                  uint32_t* __restrict__ words, const Clip* __restrict__ clip, float gscale,
                                                                  StepPack pk, int t0, int g0, uint32_t seed) {
-    const uint2 cw = chunks[blockIdx.x];
-    const GLOBAL T* g = global((const T*)pk.g[cw.x - t0]);
-    if (!g || (clip && clip->skip)) return;
-    const VcrOptimTensor& R = tensors[cw.x];
+    constexpr int BLOCKS = blocks8<T, MASTER>();
+    const Place at = place<BLOCKS>(chunks);
+    const T* grad = (const T*)pk.g[at.tensor - t0];
+    if (!grad || (clip && clip->skip)) return;
+    const VcrOptimTensor& R = tensors[at.tensor];
     const float gs = clip ? clip->gscale : gscale;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j0 = (threadIdx.x & 63) * 4;
-    const uint32_t blk = cw.y * (VCR_OPT_CHUNK / VCR_OPT_BLOCK) + wave;
-    const long long first = (long long)blk * VCR_OPT_BLOCK, have = R.numel - first;    // of this wave's block; may be past the end
-    const long long off = first + j0;
-    GLOBAL T* p = global((T*)R.p) + off;
-    GLOBAL float* mst = MASTER ? global(R.master) + off : nullptr;
-    GLOBAL uint8_t *mc = global((uint8_t*)R.m) + off, *vc = global((uint8_t*)R.v) + off;
-    GLOBAL uint8_t *ms = global(R.m_scale) + blk, *vs = global(R.v_scale) + blk;
-    g += off;
-    const bool whole = have >= VCR_OPT_BLOCK, fit = aligned(p, g);
-    const int n = whole ? 4 : have > j0 ? (int)min((long long)4, have - j0) : 0;
-    Lane8 r = {};
-    int sm = 1, sv = 1;
-    if (whole) {
-        r.g = fit ? loadv<4, true>(g) : loadv<4, false>(g);
-        if constexpr (MASTER) r.x = loadv<4, true>(mst);
-        else r.x = fit ? loadv<4, true>(p) : loadv<4, false>(p);
-        r.cm = ldq<true, u1a>(mc);
-        r.cv = ldq<true, u1a>(vc);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < n) {
-                r.g.x[k] = load1(g + k);
-                r.x.x[k] = MASTER ? mst[k] : load1(p + k);
-                r.cm |= (uint32_t)mc[k] << (8 * k);
-                r.cv |= (uint32_t)vc[k] << (8 * k);
-            }
-    }
-    if (have > 0) { sm = *ms; sv = *vs; }
     const Entry e = enter(R, pk.group[R.group - g0]);
-    if (have <= 0) return;
-    const uint32_t bkey = mix32(mix32(mix32(mix32(seed) + (uint32_t)__builtin_amdgcn_readfirstlane(e.step)) + (uint32_t)R.index) + blk);
-    sm = __builtin_amdgcn_readfirstlane(sm);
-    sv = __builtin_amdgcn_readfirstlane(sv);
-    if (!whole || !block_fast(r, sm, sv, bkey, j0, gs, e.coef)) block_any(r, sm, sv, bkey, j0, n, gs, e.coef);
-    if (whole) {
-        if constexpr (MASTER) storev<4, true>(mst, r.x);
-        if (fit) storev<4, true>(p, r.x); else storev<4, false>(p, r.x);
-        stq<true>(mc, (u1a)r.cm);
-        stq<true>(vc, (u1a)r.cv);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < n) {
-                if (MASTER) mst[k] = r.x.x[k];
-                store1(p + k, r.x.x[k]);
-                mc[k] = (uint8_t)(r.cm >> (8 * k));
-                vc[k] = (uint8_t)(r.cv >> (8 * k));
-            }
+    const uint32_t j0 = (threadIdx.x & 63) * 4;
+    const uint32_t j_step[4] = {j0 * LANE_STEP, (j0 + 1) * LANE_STEP, (j0 + 2) * LANE_STEP, (j0 + 3) * LANE_STEP};
+    const uint32_t key = mix32(mix32(mix32(seed) + (uint32_t)__builtin_amdgcn_readfirstlane(e.step)) + (uint32_t)R.index);
+    // a wave takes BLOCKS blocks, 4 apart: the workgroup's waves work on neighbouring blocks at a time
+    const uint32_t blk0 = (uint32_t)(at.first / VCR_OPT_BLOCK) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t nblocks = (uint32_t)((R.numel + VCR_OPT_BLOCK - 1) / VCR_OPT_BLOCK);
+#pragma unroll 1
+    for (uint32_t i = 0; i < BLOCKS; ++i) {
+        const uint32_t blk = blk0 + 4 * i;
+        if (blk >= nblocks) break;
+        const long long first = (long long)blk * VCR_OPT_BLOCK, have = R.numel - first;
+        Block8<T> b;
+        b.g = global(grad) + first;
+        b.p = global((T*)R.p) + first;
+        b.mst = MASTER ? global(R.master) + first : nullptr;
+        b.mc = global((uint8_t*)R.m) + first;
+        b.vc = global((uint8_t*)R.v) + first;
+        b.whole = have >= VCR_OPT_BLOCK;
+        b.fit = aligned(b.p, b.g);
+        b.n = b.whole ? 4 : have > j0 ? (int)min((long long)4, have - j0) : 0;
+        Lane8 r = load_block<T, MASTER>(b, j0);
+        GLOBAL uint8_t *ms = global(R.m_scale) + blk, *vs = global(R.v_scale) + blk;
+        int sm = __builtin_amdgcn_readfirstlane(*ms), sv = __builtin_amdgcn_readfirstlane(*vs);
+        const uint32_t bkey = mix32(key + blk);
+        if (!b.whole || !block_fast(r, sm, sv, bkey, j_step, gs, e.coef)) block_any(r, sm, sv, bkey, j_step, b.n, gs, e.coef);
+        store_block<T, MASTER>(b, j0, r);
+        if (j0 == 0) { *ms = (uint8_t)sm; *vs = (uint8_t)sv; }
     }
-    if (j0 == 0) { *ms = (uint8_t)sm; *vs = (uint8_t)sv; }
-    leave(R, words, cw.y, e.step);
+    leave<BLOCKS>(R, words, at, e.step);
 }
 
 // ---- codes -> values, values -> codes (to the nearest, ties to even) ------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(VCR_OPT_THREADS) decode_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
                                                                  PairPack out, int t0) {
-    const uint2 cw = chunks[blockIdx.x];
-    const VcrOptimTensor& R = tensors[cw.x];
-    const long long off = (long long)cw.y * VCR_OPT_CHUNK + threadIdx.x * 4, left = R.numel - off;
+    const Place at = place<1>(chunks);
+    const VcrOptimTensor& R = tensors[at.tensor];
+    const long long off = at.first + threadIdx.x * 4, left = R.numel - off;
     if (left <= 0) return;
-    GLOBAL T *mo = global((T*)out.a[cw.x - t0]), *vo = global((T*)out.b[cw.x - t0]);
+    GLOBAL T *mo = global((T*)out.a[at.tensor - t0]), *vo = global((T*)out.b[at.tensor - t0]);
     const GLOBAL uint8_t *mc = global((const uint8_t*)R.m) + off, *vc = global((const uint8_t*)R.v) + off;
     const int sm = global(R.m_scale)[off / VCR_OPT_BLOCK], sv = global(R.v_scale)[off / VCR_OPT_BLOCK];
     uint32_t cm = 0, cv = 0;
@@ -544,7 +615,9 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) decode_kernel(const VcrOptimT
         cm = ldq<true, u1a>(mc);
         cv = ldq<true, u1a>(vc);
     } else {
-        for (int k = 0; k < left; ++k) { cm |= (uint32_t)mc[k] << (8 * k); cv |= (uint32_t)vc[k] << (8 * k); }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < left) { cm |= (uint32_t)mc[k] << (8 * k); cv |= (uint32_t)vc[k] << (8 * k); }
     }
     Vec<4> m, v;
 #pragma unroll
@@ -556,10 +629,12 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) decode_kernel(const VcrOptimT
         if (mo) storev<4, true>(mo + off, m);
         if (vo) storev<4, true>(vo + off, v);
     } else {
-        for (int k = 0; k < left; ++k) {
-            if (mo) store1(mo + off + k, m.x[k]);
-            if (vo) store1(vo + off + k, v.x[k]);
-        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < left) {
+                if (mo) store1(mo + off + k, m.x[k]);
+                if (vo) store1(vo + off + k, v.x[k]);
+            }
     }
 }
 
@@ -616,7 +691,7 @@ int64_t plan_check(const char* who, const void* plan, int n, const int64_t* nume
         if (numel[k] < 0) { vcr_set_error("%s: tensor %d has numel %lld", who, k, (long long)numel[k]); return -1; }
         total += chunks_of(numel[k], VCR_OPT_CHUNK);
     }
-    if (total > 0x7FFFFFFF) { vcr_set_error("%s: %lld chunks", who, (long long)total); return -1; }
+    if (total > 0x0FFFFFFF) { vcr_set_error("%s: %lld chunks", who, (long long)total); return -1; }
     return total;
 }
 
@@ -685,7 +760,7 @@ extern "C" int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, void*
         tickets += tickets_of(chunks_of(t.numel, VCR_OPT_CHUNK));
     }
     const size_t words = plan_words(ntensors, total), need = words + tickets * TICKET_STRIDE * sizeof(uint32_t);
-    if (total > 0x7FFFFFFF || tickets > 0x7FFFFFFF || bytes < need) { vcr_set_error("vcr_optim_plan: %zu bytes for %lld chunks", bytes, (long long)total); return 1; }
+    if (total > 0x0FFFFFFF || tickets > 0x7FFFFFFF || bytes < need) { vcr_set_error("vcr_optim_plan: %zu bytes for %lld chunks", bytes, (long long)total); return 1; }
     VcrOptimTensor* out = (VcrOptimTensor*)host_plan;
     uint2* c = (uint2*)((char*)host_plan + plan_head(ntensors));
     int32_t word = 0;
@@ -744,10 +819,11 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
                                 (float)g.beta1, (float)(1.0 - g.beta1), (float)g.beta2, (float)(1.0 - g.beta2), 0};
         }
         if (any) {
-            const dim3 grid((uint32_t)nchunks), block(VCR_OPT_THREADS);
+            const dim3 block(VCR_OPT_THREADS);
+            const size_t lds = a.param_type == VCR_F32 ? VCR_OPT_LDS_FP32 : 0;
             const float gs = (float)a.grad_scale;
-#define LAUNCH32(T, M) hipLaunchKernelGGL((adamw_kernel<T, M>), grid, block, 0, st, tensors, chunks, words, clip, gs, pk, t0, g0)
-#define LAUNCH8(T, M) hipLaunchKernelGGL((adamw8_kernel<T, M>), grid, block, 0, st, tensors, chunks, words, clip, gs, pk, t0, g0, a.seed)
+#define LAUNCH32(T, M) hipLaunchKernelGGL((adamw_kernel<T, M>), dim3((uint32_t)nchunks * parts<1>()), block, lds, st, tensors, chunks, words, clip, gs, pk, t0, g0)
+#define LAUNCH8(T, M) hipLaunchKernelGGL((adamw8_kernel<T, M>), dim3((uint32_t)nchunks * parts<blocks8<T, M>()>()), block, 0, st, tensors, chunks, words, clip, gs, pk, t0, g0, a.seed)
 #define LAUNCH(T, M) do { if (a.state_bits == 32) LAUNCH32(T, M); else LAUNCH8(T, M); } while (0)
             if (a.param_type == VCR_F32) LAUNCH(float, false);
             else if (a.param_type == VCR_BF16) { if (a.masters) LAUNCH(__hip_bfloat16, true); else LAUNCH(__hip_bfloat16, false); }
@@ -779,7 +855,7 @@ static int pairs_call(const char* who, int n, const void* plan, const int64_t* n
             nchunks += chunks_of(numel[t0 + k], VCR_OPT_CHUNK);
         }
         if (nchunks > 0) {
-            const dim3 grid((uint32_t)nchunks), block(encode ? 256 : VCR_OPT_THREADS);
+            const dim3 grid((uint32_t)(encode ? nchunks : nchunks * parts<1>())), block(VCR_OPT_THREADS);
             if (encode) hipLaunchKernelGGL(encode_kernel, grid, block, 0, st, tensors, chunks, pk, t0);
             else if (type == VCR_F32) hipLaunchKernelGGL(decode_kernel<float>, grid, block, 0, st, tensors, chunks, pk, t0);
             else if (type == VCR_BF16) hipLaunchKernelGGL(decode_kernel<__hip_bfloat16>, grid, block, 0, st, tensors, chunks, pk, t0);

@@ -16,6 +16,7 @@ from . import _lib
 BLOCK = 256                                    # elements that share the scale of an 8-bit moment
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _PTR, _CONTIGUOUS, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
+_TENSORS = {torch.Tensor, torch.nn.Parameter}
 _GRAD, _DTYPE, _DEVICE, _LAYOUT = attrgetter("grad"), attrgetter("dtype"), attrgetter("device"), attrgetter("layout")
 
 
@@ -42,7 +43,7 @@ def _on(dev, call, *args):
 def _check_list(tensors, what):
     """The list, its types and its device; every tensor dense, of a supported type and on the device of the first."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if all(isinstance(t, torch.Tensor) for t in tensors):
+    if set(map(type, tensors)) <= _TENSORS or all(isinstance(t, torch.Tensor) for t in tensors):
         dtypes, devices = list(map(_DTYPE, tensors)), set(map(_DEVICE, tensors))
         if _TYPES.keys() >= set(dtypes) and len(devices) <= 1 and set(map(_LAYOUT, tensors)) <= {torch.strided} \
                 and all(d.type == "cuda" for d in devices):
@@ -152,7 +153,7 @@ class _Bucket:
 
 
 class _Plan:
-    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "buckets", "device", "stream", "captured", "covered")
+    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "numels", "buckets", "device", "stream", "captured", "covered")
 
 
 class AdamW:
@@ -275,7 +276,7 @@ class AdamW:
         plan = _Plan()
         plan.params, plan.dtypes, plan.device = _check_list(self._tensors(), "params")
         plan.keys, plan.captured = keys, False
-        plan.sizes = [len(g["params"]) for g in self.param_groups]
+        plan.sizes, plan.numels = [len(g["params"]) for g in self.param_groups], list(map(_NUMEL, plan.params))
         plan.ids, plan.ptrs = list(map(id, plan.params)), list(map(_PTR, plan.params))
         by = {}
         for i, (p, key) in enumerate(zip(plan.params, keys)):
@@ -291,7 +292,7 @@ class AdamW:
         for kind, at in by.items():
             b = _Bucket()
             b.type, b.at, b.n, b.every = kind, at, len(at), len(at) == len(plan.params)
-            ns = [plan.params[i].numel() for i in at]
+            ns = [plan.numels[i] for i in at]
             b.numels, b.kinds, b.group_of = _numels(ns), (C.c_int32 * b.n)(*[kind] * b.n), (C.c_int32 * b.n)(*[groups_of[i] for i in at])
             rec = (_lib.VcrOptimTensor * b.n)()
             for r, i in zip(rec, at):
@@ -386,7 +387,7 @@ class AdamW:
                 b = plan.buckets[0]
                 lists = _pointers(ptrs), b.numels, b.kinds
             else:
-                lists = _pointers([ptrs[i] for i in live]), _numels([plan.params[i].numel() for i in live]), _kinds([plan.dtypes[i] for i in live])
+                lists = _pointers([ptrs[i] for i in live]), _numels([plan.numels[i] for i in live]), _kinds([plan.dtypes[i] for i in live])
             clip = _norm(*lists, norm, float(self.grad_scale), max_norm, True)
         for b in plan.buckets:
             b.grads[:] = ptrs if b.every else [ptrs[i] for i in b.at]
@@ -416,26 +417,28 @@ class AdamW:
             elif len(given) != len(params):
                 raise ValueError(f"moments: {len(given)} tensors for {len(params)} parameters")
             outs.append(given)
-        kinds = {t.dtype for o in outs for t in o}
-        if len(kinds) != 1 or not kinds <= set(_TYPES):
+        kinds = set(map(_DTYPE, outs[0])) | set(map(_DTYPE, outs[1]))
+        if len(kinds) != 1 or not kinds <= _TYPES.keys():
             raise ValueError(f"moments: the outputs must be of one type among float32, bfloat16, float16: {kinds}")
-        for o in outs:
-            for t, p in zip(o, params):
-                if t.numel() != p.numel() or t.device != p.device or not t.is_contiguous():
-                    raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
         plan, stream = self._current(params)
-        held = {i for b in plan.buckets for i in b.at}
-        for i in range(len(params)):
-            if i not in held:
-                outs[0][i].zero_()
-                outs[1][i].zero_()
-            elif self.state_bits == 32:
-                for o, k in zip(outs, ("exp_avg", "exp_avg_sq")):
-                    o[i].copy_(self.state[plan.keys[i]][k].view(o[i].shape))
-        if self.state_bits == 8:
+        for o in outs:
+            if list(map(_NUMEL, o)) != plan.numels or set(map(_DEVICE, o)) != {plan.device} or not all(map(_CONTIGUOUS, o)):
+                raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
+        if plan.covered < len(params):
+            held = {i for b in plan.buckets for i in b.at}
+            for i in range(len(params)):
+                if i not in held:
+                    outs[0][i].zero_()
+                    outs[1][i].zero_()
+        if self.state_bits == 32:
+            for b in plan.buckets:
+                for i in b.at:
+                    for o, k in zip(outs, ("exp_avg", "exp_avg_sq")):
+                        o[i].copy_(self.state[plan.keys[i]][k].view(o[i].shape))
+        else:
             kind = _TYPES[kinds.pop()]
             for b in plan.buckets:
-                m, v = (_pointers([o[i].data_ptr() for i in b.at]) for o in outs)
+                m, v = (_pointers(list(map(_PTR, o if b.every else [o[i] for i in b.at]))) for o in outs)
                 _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), b.numels, m, v, kind, stream))
         return outs
 
