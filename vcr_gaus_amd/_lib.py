@@ -39,8 +39,8 @@ class VcrOptimGroup(C.Structure):
 
 class VcrAdamWStep(C.Structure):
     _fields_ = [(k, C.c_int32) for k in ("ntensors", "ngroups", "param_type", "state_bits", "masters")] + \
-               [("seed", C.c_uint32), ("plan", C.c_void_p), ("grads", C.POINTER(C.c_void_p)),
-                ("numel", C.POINTER(C.c_int64)), ("group_of", c_int_p), ("groups", C.POINTER(VcrOptimGroup)),
+               [("seed", C.c_uint32), ("plan", C.c_void_p), ("grads", C.c_void_p),
+                ("numel", C.c_void_p), ("group_of", C.c_void_p), ("groups", C.POINTER(VcrOptimGroup)),
                 ("grad_scale", C.c_double), ("clip", C.c_void_p)]
 
 
@@ -134,17 +134,15 @@ SYMBOLS = {
     "vcr_geometry_step": (C.c_int, [C.POINTER(VcrGeometryStep), C.c_void_p]),
     "vcr_rasterize_backward_tail": (C.c_int, [C.POINTER(VcrRasterArgs), C.POINTER(VcrBackwardIO), C.POINTER(VcrGeometryStep), ALLOC_FN,
                                               C.c_void_p, C.c_void_p]),
-    "vcr_optim_plan_bytes": (C.c_size_t, [C.c_int, C.POINTER(C.c_int64)]),
+    # (lists of tensors go in as the addresses of word arrays)
+    "vcr_optim_plan_bytes": (C.c_size_t, [C.c_int, C.c_void_p]),
     "vcr_optim_plan": (C.c_int, [C.c_int, C.POINTER(VcrOptimTensor), C.c_void_p, C.c_size_t]),
     "vcr_adamw_step": (C.c_int, [C.POINTER(VcrAdamWStep), C.c_void_p]),
-    "vcr_moments8_decode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_void_p),
-                                      C.POINTER(C.c_void_p), C.c_int, C.c_void_p]),
-    "vcr_moments8_encode": (C.c_int, [C.c_int, C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_void_p),
-                                      C.POINTER(C.c_void_p), C.c_void_p]),
-    "vcr_grad_norm_partials": (C.c_int, [C.c_int, C.POINTER(C.c_int64)]),
-    "vcr_grad_norm": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), c_int_p, C.c_void_p, C.c_int, C.c_double,
-                                C.c_double, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "vcr_clip_gradients": (C.c_int, [C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), c_int_p, C.c_void_p, C.c_double, C.c_void_p]),
+    "vcr_moments8_decode": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_void_p]),
+    "vcr_moments8_encode": (C.c_int, [C.c_int] + [C.c_void_p] * 5),
+    "vcr_grad_norm_partials": (C.c_int, [C.c_int, C.c_void_p]),
+    "vcr_grad_norm": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_double, C.c_double] + [C.c_void_p] * 3),
+    "vcr_clip_gradients": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_double, C.c_void_p]),
     "vcr_densify_stats": (C.c_int, [C.c_int] + [C.c_void_p] * 6),
     "vcr_depth_to_normal_forward": (C.c_int, [C.c_int, C.c_int] + [C.c_float] * 4 + [C.c_void_p] * 3),
     "vcr_depth_to_normal_backward": (C.c_int, [C.c_int, C.c_int] + [C.c_float] * 4 + [C.c_void_p] * 5),

@@ -788,7 +788,7 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
     }
     for (int k = 0; k < a.ngroups; ++k) {
         const VcrOptimGroup& g = a.groups[k];
-        if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0)) {
+        if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && (g.eps == 0.0 || g.eps >= 0x1p-126))) {
             vcr_set_error("vcr_adamw_step: group %d has beta1 %g, beta2 %g, eps %g", k, g.beta1, g.beta2, g.eps);
             return 1;
         }

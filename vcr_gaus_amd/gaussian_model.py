@@ -4,7 +4,8 @@ per-step arithmetic routed to HIP kernels:
 
   * activations + shortest-axis normal + camera orientation: one fused kernel each way
     (`fused_activate`, replaces `scene/gaussian_model.py:125-192` + `gaussian_renderer/__init__.py:95-101`)
-  * Adam over all parameter groups: one launch (`FusedAdam`, replaces `torch.optim.Adam` at `:258`)
+  * Adam over all parameter groups: one launch (`FusedAdam`, replaces `torch.optim.Adam` at `:258`); on request AdamW instead
+    (`GaussianAdamW`: decoupled weight decay, clipping, moments in 8 bits)
   * densification statistics: one kernel (`add_densification_stats`, `:669-671` + `trainer.py:345`)
 
   * densify / prune row surgery: parameters, both Adam moments and the statistics of ALL groups re-packed by one
@@ -20,6 +21,7 @@ import torch
 
 from . import _lib
 from .general_utils import build_rotation, get_expon_lr_func, inverse_sigmoid
+from .optim import AdamW
 
 GROUPS = ["xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation", "obj_dc"]
 
@@ -437,6 +439,43 @@ class FusedAdam:
                                              exp_avg_sq=mv(st["exp_avg_sq"]))
 
 
+class GaussianAdamW(AdamW):
+    """`optim.AdamW` on the Gaussian model's groups, with `FusedAdam`'s checkpoint format: state by running index, groups matched by
+    name, the classifier's two tensors as one group -- so checkpoints of either optimizer (and the reference's) load into the
+    other's model; 8-bit moments are written as codes and read by this class only."""
+
+    def state_dict(self):
+        sd, groups = super().state_dict(), []
+        for wg in sd["param_groups"]:
+            wg["name"] = FusedAdam._wire_name(wg["name"])
+            if groups and groups[-1]["name"] == wg["name"]:
+                groups[-1]["params"] += wg["params"]
+            else:
+                groups.append(wg)
+        return dict(state=sd["state"], param_groups=groups)
+
+    def load_state_dict(self, sd):
+        """Takes the learning rates and moments of the groups that the file has; the other hyper-parameters are the configuration's."""
+        saved = {wg.get("name"): wg for wg in sd["param_groups"]}
+        taken, state, groups = {}, {}, []
+        for i, g in enumerate(self.param_groups):
+            wire = FusedAdam._wire_name(g["name"])
+            wg, j = saved.get(wire), taken.get(wire, 0)
+            taken[wire] = j + 1
+            if wg is None:
+                groups.append(dict(params=[i]))
+                continue
+            if j >= len(wg["params"]):
+                raise ValueError(f"optimizer group {wire!r}: {len(wg['params'])} tensors saved, more here")
+            groups.append(dict(params=[i], lr=float(wg["lr"])))
+            if wg["params"][j] in sd["state"]:
+                state[i] = sd["state"][wg["params"][j]]
+        for wire, n in taken.items():
+            if wire in saved and len(saved[wire]["params"]) != n:
+                raise ValueError(f"optimizer group {wire!r}: {len(saved[wire]['params'])} tensors saved, {n} here")
+        super().load_state_dict(dict(state=state, param_groups=groups))
+
+
 class GaussianModel:
     def __init__(self, cfg):
         self.active_sh_degree = 0
@@ -589,7 +628,14 @@ class GaussianModel:
             for pn, prm in self.classifier.named_parameters():
                 groups.append({"params": [prm], "lr": getattr(training_args, "cls_lr", 5e-4), "name": "classifier." + pn,
                                "aux": True})
-        self.optimizer = FusedAdam(groups, eps=1e-15)
+        kind = getattr(training_args, "optimizer", "adam")
+        if kind == "adam":
+            self.optimizer = FusedAdam(groups, eps=1e-15)
+        elif kind == "adamw":
+            self.optimizer = GaussianAdamW(groups, eps=1e-15, weight_decay=float(getattr(training_args, "weight_decay", 0.0)),
+                                           state_bits=int(getattr(training_args, "state_bits", 32)))
+        else:
+            raise ValueError(f"optim.optimizer = {kind!r}: \"adam\" or \"adamw\"")
         self.xyz_scheduler_args = get_expon_lr_func(
             lr_init=training_args.position_lr_init * self.spatial_lr_scale,
             lr_final=training_args.position_lr_final * self.spatial_lr_scale,
@@ -617,6 +663,22 @@ class GaussianModel:
                                          self.denom.data_ptr(), self.max_radii2D.data_ptr(), _lib.stream_of(g)))
 
     # ---- optimiser-state surgery (scene/gaussian_model.py:425-531) -----------------------------------
+    def _moments_of(self, name):
+        """-> the two moments of a group as float32 tensors, or None if it has none yet."""
+        st = self.optimizer.state.get(name)
+        if st is None:
+            return None
+        if isinstance(self.optimizer, AdamW):
+            return self.optimizer.moments_of(name)
+        return st["exp_avg"], st["exp_avg_sq"]
+
+    def _store_moments(self, name, m, v):
+        """The group's parameter has been replaced: these are its moments now (8 bits: to the nearest code)."""
+        if isinstance(self.optimizer, AdamW):
+            self.optimizer.set_moments(name, m, v)
+        else:
+            self.optimizer.state[name]["exp_avg"], self.optimizer.state[name]["exp_avg_sq"] = m, v
+
     def _set_params(self, new):
         for name, attr in self._param_table().items():
             setattr(self, attr, new[name])
@@ -628,11 +690,10 @@ class GaussianModel:
                 continue
             p = g["params"][0]
             newp = torch.nn.Parameter(fn_param(g["name"], p.detach()).contiguous().requires_grad_(True))
-            st = self.optimizer.state.get(g["name"])
-            if st is not None:
-                st["exp_avg"] = fn_state(g["name"], st["exp_avg"]).contiguous()
-                st["exp_avg_sq"] = fn_state(g["name"], st["exp_avg_sq"]).contiguous()
+            mv = self._moments_of(g["name"])
             g["params"][0] = newp
+            if mv is not None:
+                self._store_moments(g["name"], *(fn_state(g["name"], t).contiguous() for t in mv))
             out[g["name"]] = newp
         self._set_params(out)
 
@@ -654,10 +715,10 @@ class GaussianModel:
             if g.get("aux"):
                 continue
             items.append((("p", g), g["params"][0].detach(), False))
-            stt = self.optimizer.state.get(g["name"])
-            if stt is not None:
-                items.append((("m", stt), stt["exp_avg"], True))
-                items.append((("v", stt), stt["exp_avg_sq"], True))
+            mv = self._moments_of(g["name"])
+            if mv is not None:
+                items.append((("m", g["name"]), mv[0], True))
+                items.append((("v", g["name"]), mv[1], True))
         keep_stats = mode == 0 or not reset_stats
         if keep_stats:
             items += [(("s", "xyz_gradient_accum"), self.xyz_gradient_accum, True), (("s", "denom"), self.denom, True),
@@ -674,15 +735,15 @@ class GaussianModel:
             outs.append((t, out))
         arr.n = len(items)
         _lib.check(lib.vcr_rows_move(N, m8.data_ptr(), plan.data_ptr(), C.byref(arr), mode, copies, st))
-        new_params = {}
+        new_params, moved = {}, {}
         for (kind, ref), (_, out) in zip([it[0] for it in items], outs):
             if kind == "p":
                 ref["params"][0] = torch.nn.Parameter(out.requires_grad_(True))
                 new_params[ref["name"]] = ref["params"][0]
             elif kind == "m":
-                ref["exp_avg"] = out
+                moved[ref] = out
             elif kind == "v":
-                ref["exp_avg_sq"] = out
+                self._store_moments(ref, moved[ref], out)
             else:
                 setattr(self, ref, out)
         self._set_params(new_params)
@@ -792,11 +853,9 @@ class GaussianModel:
         new = inverse_sigmoid(torch.min(self.get_opacity, torch.ones_like(self.get_opacity) * 0.01))
         for g in self.optimizer.param_groups:
             if g["name"] == "opacity":
-                st = self.optimizer.state.get("opacity")
-                if st is not None:
-                    st["exp_avg"] = torch.zeros_like(new)
-                    st["exp_avg_sq"] = torch.zeros_like(new)
                 g["params"][0] = torch.nn.Parameter(new.contiguous().requires_grad_(True))
+                if self.optimizer.state.get("opacity") is not None:
+                    self._store_moments("opacity", torch.zeros_like(new), torch.zeros_like(new))
                 self._opacity = g["params"][0]
 
     @torch.no_grad()

@@ -7,6 +7,7 @@ step replays), and moments in a quarter of the memory.  The reference trains wit
 (`scene/gaussian_model.py:258`); the update is torch.optim.AdamW's.  All arithmetic runs in csrc/optim.hip; there is no fallback.
 """
 import ctypes as C
+from array import array
 from operator import attrgetter
 
 import torch
@@ -15,21 +16,15 @@ from . import _lib
 
 BLOCK = 256                                    # elements that share the scale of an 8-bit moment
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_PTR, _CONTIGUOUS, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
 _TENSORS = {torch.Tensor, torch.nn.Parameter}
-_GRAD, _DTYPE, _DEVICE, _LAYOUT = attrgetter("grad"), attrgetter("dtype"), attrgetter("device"), attrgetter("layout")
+_PTR, _CONTIGUOUS, _NUMEL, _DEVICE = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.get_device
+_GRAD, _DTYPE = attrgetter("grad"), attrgetter("dtype")
+# Lists of many tensors are looked at attribute by attribute, not tensor by tensor, and go to the library as arrays of words: at 200
+# tensors the host's share of a call is what a user sees (a loop with the same checks took 94 us, the kernels 10).
 
 
-def _pointers(ptrs):
-    return (C.c_void_p * len(ptrs))(*ptrs)
-
-
-def _numels(ns):
-    return (C.c_int64 * len(ns))(*ns)
-
-
-def _kinds(dtypes):
-    return (C.c_int32 * len(dtypes))(*[_TYPES[d] for d in dtypes])
+def _address(words):
+    return words.buffer_info()[0]
 
 
 def _on(dev, call, *args):
@@ -45,9 +40,8 @@ def _check_list(tensors, what):
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if set(map(type, tensors)) <= _TENSORS or all(isinstance(t, torch.Tensor) for t in tensors):
         dtypes, devices = list(map(_DTYPE, tensors)), set(map(_DEVICE, tensors))
-        if _TYPES.keys() >= set(dtypes) and len(devices) <= 1 and set(map(_LAYOUT, tensors)) <= {torch.strided} \
-                and all(d.type == "cuda" for d in devices):
-            return tensors, dtypes, devices.pop() if devices else None
+        if _TYPES.keys() >= set(dtypes) and len(devices) <= 1 and -1 not in devices:
+            return tensors, dtypes, tensors[0].device if tensors else None
     for k, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}[{k}] is a {type(t).__name__}, not a tensor")
@@ -59,16 +53,34 @@ def _check_list(tensors, what):
             raise ValueError(f"{what}[{k}] is on {t.device}, {what}[0] on {tensors[0].device}")
 
 
-def _norm(ptrs, numels, kinds, out, grad_scale=1.0, max_norm=0.0, clip=False):
+def _dense(tensors, what):
+    """The tensors, contiguous."""
+    try:
+        return tensors if all(map(_CONTIGUOUS, tensors)) else [t.detach().contiguous() for t in tensors]
+    except (RuntimeError, NotImplementedError) as e:          # (layouts that have no strides)
+        raise ValueError(f"{what}: dense tensors are needed: {e}") from None
+
+
+class _List:
+    """Dense tensors as the library takes them: addresses, sizes, types."""
+    __slots__ = ("n", "ptrs", "numels", "kinds")
+
+    def __init__(self, tensors, dtypes):
+        self.n, self.ptrs, self.numels = len(tensors), array("Q", map(_PTR, tensors)), array("q", map(_NUMEL, tensors))
+        self.kinds = array("i", [_TYPES[dtypes[0]]]) * self.n if len(set(dtypes)) == 1 else array("i", [_TYPES[d] for d in dtypes])
+
+    def args(self):
+        return self.n, _address(self.ptrs), _address(self.numels), _address(self.kinds)
+
+
+def _norm(args, out, grad_scale=1.0, max_norm=0.0, clip=False):
     """Launches the norm of the listed tensors into `out`; -> with `clip` the buffer whose first 8 bytes are the clipped step's factor.
     The scratch belongs to this call (allocated on the current stream): two captured calls share nothing."""
     lib = _lib.load()
-    n = len(numels)
-    room = lib.vcr_grad_norm_partials(n, numels)
+    room = lib.vcr_grad_norm_partials(args[0], args[2])
     buffer = torch.empty(room + 1, dtype=torch.float64, device=out.device)
     at = buffer.data_ptr()
-    _lib.check(lib.vcr_grad_norm(n, ptrs, numels, kinds, at + 8, room, grad_scale, max_norm, out.data_ptr(), at if clip else None,
-                                 _lib.stream_of(out)))
+    _lib.check(lib.vcr_grad_norm(*args, at + 8, room, grad_scale, max_norm, out.data_ptr(), at if clip else None, _lib.stream_of(out)))
     return buffer
 
 
@@ -83,9 +95,8 @@ def grad_norm(tensors, out=None):
         out = torch.empty((), device=dev)
     elif out.dtype != torch.float32 or out.numel() != 1 or not out.is_cuda or dev not in (None, out.device):
         raise ValueError("grad_norm: `out` must be one float32 element on the tensors' device")
-    if not all(map(_CONTIGUOUS, tensors)):
-        tensors = [t.detach().contiguous() for t in tensors]
-    _on(out.device, _norm, _pointers(list(map(_PTR, tensors))), _numels(list(map(_NUMEL, tensors))), _kinds(dtypes), out)
+    words = _List(_dense(tensors, "grad_norm"), dtypes)
+    _on(out.device, _norm, words.args(), out)
     return out
 
 
@@ -101,13 +112,12 @@ def clip_grad_norm_(parameters, max_norm):
         raise ValueError("clip_grad_norm_: no parameter has a gradient")
     if len(set(map(id, grads))) != len(grads):
         raise ValueError("clip_grad_norm_: a gradient appears twice")
-    work = [g.contiguous() for g in grads]
-    norm = torch.empty((), device=dev)
-    lists = _pointers(list(map(_PTR, work))), _numels(list(map(_NUMEL, work))), _kinds(dtypes)
+    work = _dense(grads, "clip_grad_norm_")
+    norm, words = torch.empty((), device=dev), _List(work, dtypes)
 
     def both():
-        _norm(*lists, norm)
-        _lib.check(_lib.load().vcr_clip_gradients(len(work), *lists, norm.data_ptr(), max_norm, _lib.stream_of(norm)))
+        _norm(words.args(), norm)
+        _lib.check(_lib.load().vcr_clip_gradients(*words.args(), norm.data_ptr(), max_norm, _lib.stream_of(norm)))
 
     _on(dev, both)
     for g, w in zip(grads, work):
@@ -149,7 +159,7 @@ class _Watched(dict):
 
 class _Bucket:
     """The tensors of one type: their plan on the device and what a call needs of them on the host."""
-    __slots__ = ("type", "at", "numels", "kinds", "group_of", "plan", "grads", "args", "n", "every")
+    __slots__ = ("type", "at", "numels", "kinds", "group_of", "plan", "args", "n", "every")
 
 
 class _Plan:
@@ -267,8 +277,8 @@ class AdamW:
             if not isinstance(t, torch.Tensor) or t.dtype != dt or t.numel() != m or t.device != p.device or not t.is_contiguous():
                 raise ValueError(f"AdamW: state[{key!r}][{k!r}] must be {m} contiguous elements of {dt} on {p.device}")
 
-    def _build(self):
-        """Plan of all parameters that have a gradient or a state."""
+    def _build(self, need):
+        """Plan of all parameters that have a state, and of those in `need`, which get one."""
         lib = _lib.load()
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the first step after its tensors changed cannot be captured; take one step before the capture")
@@ -283,7 +293,7 @@ class AdamW:
             if not p.is_contiguous():
                 raise ValueError(f"AdamW: parameter {key!r} is not contiguous")
             if key not in self.state:
-                if p.grad is None:
+                if i not in need:
                     continue
                 dict.__setitem__(self.state, key, self._fresh(p))
             self._check_state(key, p, self.state[key])
@@ -292,8 +302,8 @@ class AdamW:
         for kind, at in by.items():
             b = _Bucket()
             b.type, b.at, b.n, b.every = kind, at, len(at), len(at) == len(plan.params)
-            ns = [plan.numels[i] for i in at]
-            b.numels, b.kinds, b.group_of = _numels(ns), (C.c_int32 * b.n)(*[kind] * b.n), (C.c_int32 * b.n)(*[groups_of[i] for i in at])
+            b.numels, b.kinds = array("q", [plan.numels[i] for i in at]), array("i", [kind]) * b.n
+            b.group_of = array("i", [groups_of[i] for i in at])
             rec = (_lib.VcrOptimTensor * b.n)()
             for r, i in zip(rec, at):
                 p, st = plan.params[i], self.state[keys[i]]
@@ -302,14 +312,13 @@ class AdamW:
                 r.m, r.v, r.step = ptr("exp_avg"), ptr("exp_avg_sq"), ptr("step")
                 if self.state_bits == 8 and p.numel():
                     r.m_scale, r.v_scale = ptr("exp_avg_scale"), ptr("exp_avg_sq_scale")
-            size = lib.vcr_optim_plan_bytes(b.n, b.numels)
+            size = lib.vcr_optim_plan_bytes(b.n, _address(b.numels))
             host = torch.empty(size, dtype=torch.uint8)
             _lib.check(lib.vcr_optim_plan(b.n, rec, host.data_ptr(), size))
             b.plan = host.to(plan.device)
-            b.grads = (C.c_void_p * b.n)()
             b.args = _lib.VcrAdamWStep(ntensors=b.n, param_type=kind, state_bits=self.state_bits,
                                        masters=int(self.master_weights and kind != 0), seed=self.seed, plan=b.plan.data_ptr(),
-                                       grads=b.grads, numel=b.numels, group_of=b.group_of)
+                                       numel=_address(b.numels), group_of=_address(b.group_of))
             plan.buckets.append(b)
         stream = torch.cuda.current_stream(plan.device)
         stream.synchronize()                     # (the upload is finished whatever stream the steps use)
@@ -321,12 +330,12 @@ class AdamW:
         """The plan, rebuilt where a parameter or a state entry is another tensor than it holds; `need`: indices that must be in it."""
         plan = self._plan
         if plan is None or list(map(id, params)) != plan.ids or list(map(_PTR, params)) != plan.ptrs \
-                or [len(g["params"]) for g in self.param_groups] != plan.sizes or list(map(_DTYPE, params)) != plan.dtypes:
-            plan = self._build()
+                or [len(g["params"]) for g in self.param_groups] != plan.sizes:
+            plan = self._build(set(need))
         elif plan.covered < len(params):
             known = {i for b in plan.buckets for i in b.at}
             if any(i not in known for i in need):
-                plan = self._build()
+                plan = self._build(set(need))
         stream = torch.cuda.current_stream(plan.device)
         if stream.cuda_stream != plan.stream:
             for b in plan.buckets:
@@ -362,17 +371,18 @@ class AdamW:
             return None
         plan, stream = self._current(params, live)
         if len(live) == len(grads):
-            same = list(map(_DTYPE, grads)) == plan.dtypes
-            if not all(map(_CONTIGUOUS, grads)):
-                grads = [g.detach().contiguous() for g in grads]
-            ptrs = list(map(_PTR, grads))
+            grads = _dense(grads, "AdamW: gradients")
+            fits, ptrs = list(map(_NUMEL, grads)) == plan.numels and list(map(_DTYPE, grads)) == plan.dtypes, array("Q", map(_PTR, grads))
         else:
-            same = all(grads[i].dtype is plan.dtypes[i] for i in live)
-            grads = [None if g is None else g.detach().contiguous() for g in grads]
-            ptrs = [None if g is None else g.data_ptr() for g in grads]
-        if not same:
-            i = next(i for i in live if grads[i].dtype is not plan.dtypes[i])
-            raise ValueError(f"AdamW: the gradient of {plan.keys[i]!r} has type {grads[i].dtype}, the parameter {plan.dtypes[i]}")
+            some = _dense([grads[i] for i in live], "AdamW: gradients")
+            fits = all(g.dtype is plan.dtypes[i] and g.numel() == plan.numels[i] for i, g in zip(live, some))
+            ptrs = array("Q", bytes(8 * len(grads)))
+            for i, g in zip(live, some):
+                ptrs[i], grads[i] = g.data_ptr(), g              # (grads: alive until the launch)
+        if not fits:
+            i = next(i for i in live if grads[i].dtype is not plan.dtypes[i] or grads[i].numel() != plan.numels[i])
+            raise ValueError(f"AdamW: the gradient of {plan.keys[i]!r} has type {grads[i].dtype} and {grads[i].numel()} elements, "
+                             f"the parameter {plan.dtypes[i]} and {plan.numels[i]}")
         norm = _on(plan.device, self._launch, plan, ptrs, live, max_norm, stream)
         if only is not None:
             for i in live:
@@ -385,14 +395,16 @@ class AdamW:
             norm = torch.empty((), device=plan.device)
             if len(live) == len(ptrs) and len(plan.buckets) == 1:
                 b = plan.buckets[0]
-                lists = _pointers(ptrs), b.numels, b.kinds
+                words = ptrs, b.numels, b.kinds
             else:
-                lists = _pointers([ptrs[i] for i in live]), _numels([plan.numels[i] for i in live]), _kinds([plan.dtypes[i] for i in live])
-            clip = _norm(*lists, norm, float(self.grad_scale), max_norm, True)
+                words = (array("Q", [ptrs[i] for i in live]), array("q", [plan.numels[i] for i in live]),
+                         array("i", [_TYPES[plan.dtypes[i]] for i in live]))
+            clip = _norm((len(words[0]), *map(_address, words)), norm, float(self.grad_scale), max_norm, True)
         for b in plan.buckets:
-            b.grads[:] = ptrs if b.every else [ptrs[i] for i in b.at]
+            mine = ptrs if b.every else array("Q", [ptrs[i] for i in b.at])
             a = b.args
-            a.groups, a.ngroups, a.grad_scale, a.clip = groups, len(groups), self.grad_scale, None if clip is None else clip.data_ptr()
+            a.grads, a.groups, a.ngroups, a.grad_scale = _address(mine), groups, len(groups), self.grad_scale
+            a.clip = None if clip is None else clip.data_ptr()
             _lib.check(lib.vcr_adamw_step(C.byref(a), stream))
         return norm
 
@@ -422,7 +434,7 @@ class AdamW:
             raise ValueError(f"moments: the outputs must be of one type among float32, bfloat16, float16: {kinds}")
         plan, stream = self._current(params)
         for o in outs:
-            if list(map(_NUMEL, o)) != plan.numels or set(map(_DEVICE, o)) != {plan.device} or not all(map(_CONTIGUOUS, o)):
+            if list(map(_NUMEL, o)) != plan.numels or set(map(_DEVICE, o)) != {plan.device.index} or not all(map(_CONTIGUOUS, o)):
                 raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
         if plan.covered < len(params):
             held = {i for b in plan.buckets for i in b.at}
@@ -438,9 +450,18 @@ class AdamW:
         else:
             kind = _TYPES[kinds.pop()]
             for b in plan.buckets:
-                m, v = (_pointers(list(map(_PTR, o if b.every else [o[i] for i in b.at]))) for o in outs)
-                _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), b.numels, m, v, kind, stream))
+                m, v = (array("Q", map(_PTR, o if b.every else [o[i] for i in b.at])) for o in outs)
+                _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), _address(b.numels), _address(m),
+                               _address(v), kind, stream))
         return outs
+
+    @torch.no_grad()
+    def moments_of(self, key):
+        """The two moments of one parameter, by the state's key: the float32 tensors themselves, or what the 8-bit codes stand for."""
+        st = self.state[key]
+        if self.state_bits == 32:
+            return st["exp_avg"], st["exp_avg_sq"]
+        return tuple(decode8(st))
 
     @torch.no_grad()
     def set_moments(self, key, exp_avg, exp_avg_sq, step=None):
@@ -524,7 +545,7 @@ class AdamW:
                 raise ValueError(f"optimizer state of {key!r}: {nb} block scales expected")
             out.update(raw)
             if self.state_bits == 32:
-                out.update(zip(("exp_avg", "exp_avg_sq"), decode8(raw, p)))
+                out.update(zip(("exp_avg", "exp_avg_sq"), decode8(raw)))
                 del out["exp_avg_scale"], out["exp_avg_sq_scale"]
         else:
             m, v = as_held(st["exp_avg"], torch.float32), as_held(st["exp_avg_sq"], torch.float32)
@@ -548,8 +569,8 @@ def _single(st, n):
     rec[0].v, rec[0].m_scale, rec[0].v_scale = (st[k].data_ptr() for k in ("exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"))
     rec[0].step = st["exp_avg"].data_ptr()               # (not used by these kernels, but not optional)
     rec[0].numel = n
-    ns = _numels([n])
-    size = lib.vcr_optim_plan_bytes(1, ns)
+    ns = array("q", [n])
+    size = lib.vcr_optim_plan_bytes(1, _address(ns))
     host = torch.empty(size, dtype=torch.uint8)
     _lib.check(lib.vcr_optim_plan(1, rec, host.data_ptr(), size))
     return host.to(dev), ns
@@ -563,18 +584,20 @@ def encode8(exp_avg, exp_avg_sq, st):
     if dev.type != "cuda":
         raise ValueError("8-bit moments need a HIP device")
     plan, ns = _single(st, exp_avg.numel())
-    _lib.check(_on(dev, _lib.load().vcr_moments8_encode, 1, plan.data_ptr(), ns, _pointers([exp_avg.data_ptr()]),
-                   _pointers([exp_avg_sq.data_ptr()]), _lib.stream_of(st["exp_avg"])))
+    m, v = array("Q", [exp_avg.data_ptr()]), array("Q", [exp_avg_sq.data_ptr()])
+    _lib.check(_on(dev, _lib.load().vcr_moments8_encode, 1, plan.data_ptr(), _address(ns), _address(m), _address(v),
+                   _lib.stream_of(st["exp_avg"])))
 
 
-def decode8(st, p):
-    """-> the float32 values of the 8-bit moments in `st`, of `p`'s shape."""
+def decode8(st):
+    """-> the float32 values of the 8-bit moments in `st`, of their shape."""
     dev = st["exp_avg"].device
-    outs = [torch.empty(p.shape, device=dev) for _ in range(2)]
-    if p.numel():
+    outs = [torch.empty(st["exp_avg"].shape, device=dev) for _ in range(2)]
+    if outs[0].numel():
         if dev.type != "cuda":
             raise ValueError("8-bit moments need a HIP device")
-        plan, ns = _single(st, p.numel())
-        _lib.check(_on(dev, _lib.load().vcr_moments8_decode, 1, plan.data_ptr(), ns, *[_pointers([o.data_ptr()]) for o in outs], 0,
+        plan, ns = _single(st, outs[0].numel())
+        m, v = (array("Q", [o.data_ptr()]) for o in outs)
+        _lib.check(_on(dev, _lib.load().vcr_moments8_decode, 1, plan.data_ptr(), _address(ns), _address(m), _address(v), 0,
                        _lib.stream_of(st["exp_avg"])))
     return outs

@@ -21,6 +21,7 @@ from .gaussian_model import GaussianModel
 from .gaussian_renderer import count_render, render, visi_acc_render, visibility_counts
 from .loss_utils import (curv_loss, edge_aware_mean, entropy_regulariser, l1_ssim, normal_loss, scale_regulariser,
                          semantic_loss)
+from .optim import AdamW
 
 
 def load_capture(path):
@@ -71,6 +72,7 @@ class Trainer:
         self.visi_list = None
         self._stats_delta, self._visi_delta, self._stats_dirty = None, None, False     # data parallel: see _densify_stats
         self.last_stats = {}
+        self.last_grad_norm = None       # AdamW with `optim.max_grad_norm`: the last step's gradient norm (device scalar)
         self._picked = []
         # DP: exchange dL/drgb (12 B/Gaussian/view, all-gather) instead of all-reducing the 192 B/Gaussian SH gradients
         self.factorised_sh = world > 1 or force_factorised       # (forcing it at world 1 exercises the path in tests)
@@ -459,7 +461,7 @@ class Trainer:
                 self._pending_sh = rec.take_sh_factors() + (int(m.active_sh_degree),)
         else:
             self.join_side()
-            self._allreduce_grads(early_feature_step=not surgery, rec=rec, sink=sink)
+            self._allreduce_grads(early_feature_step=not surgery and not isinstance(m.optimizer, AdamW), rec=rec, sink=sink)
             collectives = self.world > 1 or getattr(self, "force_collectives", False)
             self.last_exchange = ("factorised" if self.factorised_sh else "dense") if collectives else "none"
             if collectives and self.exchange_algo == "rs_ag" and self.world > 1:
@@ -676,7 +678,9 @@ class Trainer:
         extra = self.active_extra_losses(it)
         fused = getattr(self, "use_fused_losses", True) and not extra
         from .rasterizer import RasterOptions
-        overlap = self.overlap_sh and m._xyz.shape[0] >= self.overlap_min_gaussians
+        # AdamW (`optim.optimizer = "adamw"`) takes whole gradients after the backward: the serial step with the modular tail
+        adamw = isinstance(m.optimizer, AdamW)
+        overlap = self.overlap_sh and m._xyz.shape[0] >= self.overlap_min_gaussians and not adamw
         self.factorised_sh = self._factorised_base or overlap
         if not overlap and self._pending_sh is not None:
             self.join_side()
@@ -688,7 +692,7 @@ class Trainer:
         # the fused static tail needs every gradient path into scaling / rotation / opacity to pass through the fused
         # activation node (the fused loss node guarantees that), un-reduced gradients (one process) and unchanged rows
         dp = self.world > 1 or getattr(self, "force_collectives", False)
-        armed = bool(self.fuse_geometry and fused and not surgery and m._xyz.is_cuda and m._xyz.shape[0] > 0
+        armed = bool(self.fuse_geometry and fused and not surgery and not adamw and m._xyz.is_cuda and m._xyz.shape[0] > 0
                      and not cfg.pipline.compute_cov3D_python)
         # the iteration's side channel (see GeometrySink): armed = the one-kernel static tail; the l1_scale gradient joins the
         # activation backward's kernel; the loss node's reduction buffer is this trainer's
@@ -794,7 +798,10 @@ class Trainer:
                 i = cfg.optim.prune.iterations.index(it)
                 m.prune_gaussians((cfg.optim.prune.decay ** i) * cfg.optim.prune.percent,
                                   self.v_imp_score(imp, cfg.optim.prune.v_pow))
-            m.optimizer.step()
+            if adamw:          # (the norm, or None where `optim.max_grad_norm` is not set: a device scalar, nothing waits for it)
+                self.last_grad_norm = m.optimizer.step(max_norm=getattr(cfg.optim, "max_grad_norm", None) or None)
+            else:
+                m.optimizer.step()
             m.optimizer.zero_grad(set_to_none=True)
         return data
 
