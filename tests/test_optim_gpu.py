@@ -557,6 +557,50 @@ def test_replaced_tensors_are_seen(device):
     assert not torch.equal(params[1], b)
 
 
+def test_masters_follow_only_when_asked(device):
+    from vcr_gaus_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.full((300,), 2.0, dtype=BF, device=device))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], lr=1e-3, weight_decay=0.0, master_weights=True)
+    opt.step()
+    p.data.fill_(5.0)
+    opt.step()
+    assert float(p[0]) == 2.0 and abs(float(opt.state["0"]["master"][0]) - (2 - 2e-3)) < 1e-6        # (lr each step: constant gradients)
+    p.data.fill_(5.0)
+    del opt.state["0"]["master"]
+    opt.step()
+    assert abs(float(opt.state["0"]["master"][0]) - (5 - 1e-3)) < 1e-6 and float(p[0]) == 5.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_past_32_bits(device, bits):
+    """A tensor of 2^32 + 4099 bf16 elements: its first, middle and last elements are stepped like those of a small tensor with the same
+    values, what lies between keeps its zeros; the norm counts every one."""
+    from vcr_gaus_amd.optim import AdamW, grad_norm
+    n, spots = (1 << 32) + 4099, [0, 4096, (1 << 31) + 77, (1 << 32) - 1, 1 << 32, (1 << 32) + 4098]
+    big = torch.nn.Parameter(torch.zeros(n, dtype=BF, device=device))
+    big.grad = torch.zeros(n, dtype=BF, device=device)
+    vals = torch.tensor([0.5, -1.0, 2.0, 0.25, -0.125, 1.0], device=device).to(BF)
+    small = torch.nn.Parameter(torch.zeros(6, dtype=BF, device=device))
+    small.grad = vals.clone()
+    for k, i in enumerate(spots):
+        big.grad[i] = vals[k]
+    assert float(grad_norm([big.grad])) == float(grad_norm([small.grad]))
+    opt, ref = AdamW([big], state_bits=bits, lr=0.01), AdamW([small], state_bits=bits, lr=0.01)
+    opt.step()
+    ref.step()
+    # (a first step: the update is lr * sign to 2^-20, whatever block the element lies in)
+    for k, i in enumerate(spots):
+        assert float(big[i]) == float(small[k]) != 0.0, i
+    assert int(opt.state["0"]["step"]) == 1
+    assert int(torch.count_nonzero(big.detach())) == len(spots)
+    if bits == 8:
+        st = opt.state["0"]
+        assert int(st["exp_avg_scale"][-1]) > 1 and int(st["exp_avg_scale"][1 << 23]) > 1 and int(st["exp_avg_scale"][1 << 22]) == 1
+    del opt, big
+    torch.cuda.empty_cache()
+
+
 # ---- checkpoints ----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("bits, dtype, master", [(32, F, False), (8, F, False), (8, BF, True), (32, HF, True)])
 def test_checkpoint_resumes_bit_for_bit(device, bits, dtype, master, tmp_path):
@@ -610,7 +654,7 @@ def test_moments_pass_between_the_two_forms(device):
 GROUPS = ["xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation"]
 
 
-def adamw_trainer(device, sem=0, **optim):
+def adamw_trainer(device, sem=0, factorised=False, **optim):
     from vcr_gaus_amd import synthetic
     from vcr_gaus_amd.trainer import make_synthetic_trainer
     raw = synthetic.make_gaussians(2500, seed=5, **({"sem_channels": sem} if sem else {}))
@@ -618,14 +662,14 @@ def adamw_trainer(device, sem=0, **optim):
     cams = synthetic.make_cameras(3, 96, 64, 80.0, device=device)
     ov = {"densify_from_iter": 10 ** 9, "prune": {"iterations": []}, "optimizer": "adamw"}
     ov.update(optim)
-    return make_synthetic_trainer(raw, cams, device, preset="dtu_c3", gt_jitter=0.3, optim=ov)
+    return make_synthetic_trainer(raw, cams, device, preset="dtu_c3", gt_jitter=0.3, force_factorised=factorised, optim=ov)
 
 
-@pytest.mark.parametrize("bits, max_norm", [(32, None), (32, 1e-3), (8, 1e-3)])
-def test_a_training_step_applies_the_formula_to_its_gradients(device, bits, max_norm):
+@pytest.mark.parametrize("bits, max_norm, factorised", [(32, None, False), (32, 1e-3, True), (8, 1e-3, False)])
+def test_a_training_step_applies_the_formula_to_its_gradients(device, bits, max_norm, factorised):
     """Three iterations of Trainer.train_step; before each optimizer step the parameters and gradients are recorded, after it every
     group holds what the definition gives for them (8 bits: the same codes)."""
-    tr = adamw_trainer(device, state_bits=bits, max_grad_norm=max_norm, weight_decay=0.01)
+    tr = adamw_trainer(device, factorised=factorised, state_bits=bits, max_grad_norm=max_norm, weight_decay=0.01)
     m, opt = tr.model, tr.model.optimizer
     assert opt.state_bits == bits and [g["name"] for g in opt.param_groups] == GROUPS
     real, seen = opt.step, {}

@@ -35,6 +35,7 @@ namespace {
 #define VCR_OPT_LDS_FP32 40000
 #define VCR_OPT_TENSORS 352        // tensors and ...
 #define VCR_OPT_GROUPS 14          // ... hyper-parameter groups per launch: both travel in the kernel arguments (4 KB)
+#define VCR_OPT_LAUNCH_CHUNKS 4194303   // plan entries per launch: a launch has fewer than 2^32 threads, 1024 an entry at most
 #define VCR_OPT_NORM_TENSORS 192   // tensors per launch of the norm kernel
 #define VCR_OPT_PAIRS 200          // tensors per launch of the code <-> value kernels
 #define VCR_OPT_NORM_BLOCKS 2048
@@ -306,9 +307,10 @@ __device__ __forceinline__ Coef coef_of(const Group& G, int t) {
     return c;
 }
 
-// Counts this workgroup out (its read of the counter is long done: the factors came from it).  Tickets on one address come at 12.5 ns each (a
-// tensor of 400 M elements in 195 000 workgroups would take 2.4 ms for them alone, measured), so a tensor with many chunks
-// has 64 first-level words, and only the last arrival of each goes to the second level.
+// Counts this workgroup out (its read of the counter is long done: the factors came from it), at the end, where nothing waits for the
+// ticket: drawn before the results are written it costs 3 to 6 %.  Tickets on one address come at 12.5 ns each (a tensor of
+// 400 M elements in 195 000 workgroups would take 2.4 ms for them alone, measured), so a tensor with many chunks has 64 first-level
+// words, and only the last arrival of each goes to the second level.
 #define TICKET_GROUPS 64
 #define TICKET_FLAT 64             // up to this many chunks: one level
 #define TICKET_STRIDE 16           // words between two tickets: a cache line of their own
@@ -345,7 +347,7 @@ __device__ __forceinline__ Entry enter(const VcrOptimTensor& R, const Group& G) 
     return entry;
 }
 
-// ---- update, moments in 32 bits: four consecutive elements per lane, 4096 per workgroup ------------------------------------
+// ---- update, moments in 32 bits: four consecutive elements per lane ----------------------------------------------------
 template <typename T, bool MASTER>
 __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
                                                                 uint32_t* __restrict__ words, const Clip* __restrict__ clip, float gscale,
@@ -689,6 +691,7 @@ int64_t plan_check(const char* who, const void* plan, int n, const int64_t* nume
     int64_t total = 0;
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0) { vcr_set_error("%s: tensor %d has numel %lld", who, k, (long long)numel[k]); return -1; }
+        if (chunks_of(numel[k], VCR_OPT_CHUNK) > VCR_OPT_LAUNCH_CHUNKS) { vcr_set_error("%s: tensor %d with %lld elements is too large", who, k, (long long)numel[k]); return -1; }
         total += chunks_of(numel[k], VCR_OPT_CHUNK);
     }
     if (total > 0x0FFFFFFF) { vcr_set_error("%s: %lld chunks", who, (long long)total); return -1; }
@@ -809,8 +812,10 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
         bool any = false;
         const int g0 = a.group_of[t0];
         for (; t1 < a.ntensors && t1 - t0 < VCR_OPT_TENSORS && a.group_of[t1] - g0 < VCR_OPT_GROUPS; ++t1) {
+            const int64_t c = chunks_of(a.numel[t1], VCR_OPT_CHUNK);
+            if (nchunks + c > VCR_OPT_LAUNCH_CHUNKS) break;
             pk.g[t1 - t0] = a.grads[t1];
-            nchunks += chunks_of(a.numel[t1], VCR_OPT_CHUNK);
+            nchunks += c;
             any |= a.grads[t1] != nullptr && a.numel[t1] > 0;
         }
         for (int k = g0; k <= a.group_of[t1 - 1]; ++k) {
@@ -845,14 +850,16 @@ static int pairs_call(const char* who, int n, const void* plan, const int64_t* n
     if (!a || !b || type < 0 || type > VCR_F16) { vcr_set_error("%s: inconsistent arguments", who); return 1; }
     const VcrOptimTensor* tensors = (const VcrOptimTensor*)plan;
     const uint2* chunks = plan_chunks(plan, n);
-    for (int t0 = 0; t0 < n; t0 += VCR_OPT_PAIRS) {
+    for (int t0 = 0, t1 = 0; t0 < n; t0 = t1) {
         PairPack pk = {};
         int64_t nchunks = 0;
-        for (int k = 0; k < VCR_OPT_PAIRS && t0 + k < n; ++k) {
-            pk.a[k] = a[t0 + k];
-            pk.b[k] = b[t0 + k];
-            if (encode && numel[t0 + k] > 0 && (!pk.a[k] || !pk.b[k])) { vcr_set_error("%s: values of tensor %d are missing", who, t0 + k); return 1; }
-            nchunks += chunks_of(numel[t0 + k], VCR_OPT_CHUNK);
+        for (; t1 < n && t1 - t0 < VCR_OPT_PAIRS; ++t1) {
+            const int64_t c = chunks_of(numel[t1], VCR_OPT_CHUNK);
+            if (nchunks + c > VCR_OPT_LAUNCH_CHUNKS) break;
+            pk.a[t1 - t0] = a[t1];
+            pk.b[t1 - t0] = b[t1];
+            if (encode && numel[t1] > 0 && (!a[t1] || !b[t1])) { vcr_set_error("%s: values of tensor %d are missing", who, t1); return 1; }
+            nchunks += c;
         }
         if (nchunks > 0) {
             const dim3 grid((uint32_t)(encode ? nchunks : nchunks * parts<1>())), block(VCR_OPT_THREADS);

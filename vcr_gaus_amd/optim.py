@@ -178,9 +178,13 @@ class AdamW:
     rounded into the 16-bit parameter.  `lr` may be a float32 device scalar (a captured step reads it at replay).
 
     `state[key]`: `step` (int32 on the device), `exp_avg`, `exp_avg_sq` (float32, or uint8 codes with `exp_avg_scale` /
-    `exp_avg_sq_scale`), `master`; key = the group's name if the group has one tensor, else "<name or number>.<i>".
+    `exp_avg_sq_scale`), `master`; key = the group's name if the group has one tensor, else "<name or number>.<i>".  A 16-bit
+    parameter that is changed from outside between steps does not change its master: delete `state[key]["master"]`, and the
+    next step takes it from the parameter again.
     Parameters must be contiguous; gradients of another layout are copied.  Tensors without a gradient are skipped, and so are
-    their counters, as in torch.  Memory: plan and state belong to the optimizer; a captured step keeps its plan alive."""
+    their counters, as in torch.  Memory: plan and state belong to the optimizer; a captured step keeps its plan alive (and holds
+    the rates of its groups as they were, but for those given as device scalars).  One optimizer's steps are one sequence: two that
+    run at the same time on two streams, or two of its captured graphs replayed so, race on the parameters."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False, seed=0):
         params = list(params)
@@ -288,6 +292,8 @@ class AdamW:
         plan.keys, plan.captured = keys, False
         plan.sizes, plan.numels = [len(g["params"]) for g in self.param_groups], list(map(_NUMEL, plan.params))
         plan.ids, plan.ptrs = list(map(id, plan.params)), list(map(_PTR, plan.params))
+        if len(set(plan.ids)) != len(plan.ids):
+            raise ValueError("AdamW: a parameter appears twice")
         by = {}
         for i, (p, key) in enumerate(zip(plan.params, keys)):
             if not p.is_contiguous():
@@ -296,7 +302,13 @@ class AdamW:
                 if i not in need:
                     continue
                 dict.__setitem__(self.state, key, self._fresh(p))
-            self._check_state(key, p, self.state[key])
+            st = self.state[key]
+            if type(st) is not _Watched:
+                st = _Watched(self, st)
+                dict.__setitem__(self.state, key, st)
+            if self._has_master(p) and "master" not in st:
+                dict.__setitem__(st, "master", p.detach().float().contiguous())
+            self._check_state(key, p, st)
             by.setdefault(_TYPES[p.dtype], []).append(i)
         plan.buckets, plan.covered = [], sum(map(len, by.values()))
         for kind, at in by.items():
@@ -356,7 +368,7 @@ class AdamW:
     # ---- the step -----------------------------------------------------------------------------------------------------
     def step(self, only=None, max_norm=None):
         """One update of every parameter that has a gradient (`only`: of the groups with these names; their gradients are released
-        afterwards, as in `FusedAdam.step`).  `max_norm`: the gradients count with the factor min(1, max_norm / (norm + 1e-6)), norm
+        afterwards, as in `FusedAdam.step`).  `max_norm` (infinity: measure and guard, never clip): the gradients count with the factor min(1, max_norm / (norm + 1e-6)), norm
         the 2-norm of all gradients of this step times `grad_scale`; -> the norm (0-dim float32; nothing waits for it), and if that is
         not finite in float32 the whole step is skipped on the device: parameters, moments and counters stay.  Without: -> None."""
         if max_norm is not None:
@@ -416,7 +428,6 @@ class AdamW:
                 p.grad.zero_()
 
     # ---- moments as values ---------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def moments(self, exp_avgs=None, exp_avg_sqs=None, dtype=torch.float32):
         """The moments as values, whatever they are held in: two lists, one tensor for each parameter in the groups' order.  Given
         lists are written to (contiguous, all of one type) instead of new tensors of `dtype`; a parameter that has not been stepped
@@ -440,13 +451,13 @@ class AdamW:
             held = {i for b in plan.buckets for i in b.at}
             for i in range(len(params)):
                 if i not in held:
-                    outs[0][i].zero_()
-                    outs[1][i].zero_()
+                    outs[0][i].detach().zero_()
+                    outs[1][i].detach().zero_()
         if self.state_bits == 32:
             for b in plan.buckets:
                 for i in b.at:
                     for o, k in zip(outs, ("exp_avg", "exp_avg_sq")):
-                        o[i].copy_(self.state[plan.keys[i]][k].view(o[i].shape))
+                        o[i].detach().copy_(self.state[plan.keys[i]][k].view(o[i].shape))
         else:
             kind = _TYPES[kinds.pop()]
             for b in plan.buckets:
