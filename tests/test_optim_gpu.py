@@ -253,11 +253,13 @@ def test_adamw8_extreme_blocks(device, eps):
     """Blocks of zeros, of tiny gradients (v below 2^-126, block exponents at the bottom), of huge ones, of all sizes at once, with NaN
     and infinities in single places: codes as defined, the other elements of a block untouched by what is not finite."""
     from vcr_gaus_amd.optim import AdamW
-    n = 24 * 256
-    base = torch.randn(n, generator=torch.Generator().manual_seed(1)).view(24, 256)
+    n = 26 * 256
+    base = torch.randn(n, generator=torch.Generator().manual_seed(1)).view(26, 256)
     scale = torch.tensor([0.0, 1.0, 1e-12, 1e-18, 1e-20, 1e-22, 1e-30, 1e-38, 1e-42, 1e4, 1e8, 1e12, 1e15, 1e17, 1e18, 3e18, 1e19, 1e25, 1e38,
-                          1.0, 1.0, 1.0, 1.0, 1.0])
+                          1.0, 1.0, 1.0, 1.0, 1.0, 1.0, 1e-6])
     grads = base * scale[:, None]
+    # ordinary sizes whose squares reach 2^-53 of the largest: the lowest code of v, at least 1
+    grads[24:] *= torch.logspace(-8, 0, 256)
     grads[20] *= torch.logspace(-30, 5, 256)
     grads[21, 7], grads[21, 200], grads[22, 0], grads[23, 255] = float("nan"), float("inf"), float("-inf"), float("nan")
     p = torch.nn.Parameter(torch.ones(n, device=device))
@@ -277,9 +279,9 @@ def test_adamw8_extreme_blocks(device, eps):
             q = np.abs(x - 1) + 1e-4
             off = 2.0 ** -22 + 2.0 ** -19 * q + q * np.where(v > 0, 2.0 ** -150 / np.maximum(v.astype(np.float64), 2.0 ** -149), 0)
             assert np.all(np.abs(got - x)[ok] <= off[ok])
-    untouched = np.ones(n, bool).reshape(24, 256)
+    untouched = np.ones(n, bool).reshape(26, 256)
     untouched[21, [7, 200]] = untouched[22, 0] = untouched[23, 255] = False
-    assert np.isfinite(host(p).reshape(24, 256)[[21, 22, 23]][untouched[[21, 22, 23]]]).all()
+    assert np.isfinite(host(p).reshape(26, 256)[[21, 22, 23]][untouched[[21, 22, 23]]]).all()
 
 
 def test_adamw8_is_the_same_on_every_run_and_unbiased(device):

@@ -25,14 +25,10 @@ namespace {
 
 #define VCR_OPT_BLOCK 256          // elements that share a scale
 #define VCR_OPT_CHUNK 4096         // elements per entry of a plan
-// Threads per workgroup, four elements each and no loop: a workgroup reads, computes, writes and is gone, so that the ones in
-// flight work on neighbouring memory (400 M elements: 2 008 us with four rounds of 1024 elements per workgroup, 1 929 us with one).
+// Threads per workgroup; four elements each and no loop in the 32-bit update: a workgroup reads, computes, writes and is gone, so that
+// the ones in flight work on neighbouring memory (1 M Gaussians: 289 us with four rounds of 1024 elements per workgroup, 279 us
+// with one; 1024 threads 291 us).
 #define VCR_OPT_THREADS 256
-// LDS that a workgroup of the fp32 update asks for and does not use: it leaves 4 workgroups on a compute unit instead of 8.  With
-// fewer waves the memory sees longer runs of reads and of writes: 400 M elements 1 929 -> 1 857 us, 1 M Gaussians 279 -> 265 us (6.2
-// TB/s).  16-bit parameters lose by it (9 M fp16 elements, one off alignment: 37 -> 43 us), the 8-bit update, which is bound by its
-// instructions, more still (771 -> 1 099 us).
-#define VCR_OPT_LDS_FP32 40000
 #define VCR_OPT_TENSORS 352        // tensors and ...
 #define VCR_OPT_GROUPS 14          // ... hyper-parameter groups per launch: both travel in the kernel arguments (4 KB)
 #define VCR_OPT_LAUNCH_CHUNKS 4194303   // plan entries per launch: a launch has fewer than 2^32 threads, 1024 an entry at most
@@ -67,7 +63,7 @@ __device__ __forceinline__ void store1(GLOBAL __half* p, float x) { *(GLOBAL uns
 
 // Four consecutive elements at any address that the element's type allows: the types below are aligned to one element, and the
 // hardware takes such addresses in its 8- and 16-byte accesses as they are.  NT: past the caches' retention, for what a step
-// touches once (all of it: parameters, gradients, moments).
+// touches once: parameters, gradients, moments (400 M elements 2 079 -> 1 868 us, 302 M bf16 elements with masters 1 599 -> 1 400 us).
 typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u2a __attribute__((ext_vector_type(2), aligned(2)));
@@ -125,12 +121,6 @@ template <int V, bool NT, typename T> __device__ __forceinline__ void storev(GLO
         for (int k = 0; k < 2; ++k) q[k] = narrow(r.x + 2 * k, p);
         stq<NT>(p, q);
     }
-}
-
-// whether 4-element accesses of p and g are naturally aligned: if not, they share cache lines with the neighbours', and the
-// non-temporal kind would move each line twice (fp16, one element off: 52 against 46 us for 9 M elements)
-template <typename T> __device__ __forceinline__ bool aligned(const GLOBAL T* p, const GLOBAL T* g) {
-    return (((uint32_t)(uintptr_t)p | (uint32_t)(uintptr_t)g) & (4 * sizeof(T) - 1)) == 0;
 }
 
 __device__ __forceinline__ void moments_one(float& m, float& v, float g, const Coef& c) {
@@ -362,14 +352,13 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
     GLOBAL float* mst = MASTER ? global(R.master) + off : nullptr;
     GLOBAL float *m = global((float*)R.m) + off, *v = global((float*)R.v) + off;
     g += off;
-    const bool fit = aligned(p, g);
     Vec<4> gg = {}, mm = {}, vv = {}, x = {};
     if (left >= 4) {
-        gg = fit ? loadv<4, true>(g) : loadv<4, false>(g);
+        gg = loadv<4, true>(g);
         mm = loadv<4, true>(m);
         vv = loadv<4, true>(v);
         if constexpr (MASTER) x = loadv<4, true>(mst);
-        else x = fit ? loadv<4, true>(p) : loadv<4, false>(p);
+        else x = loadv<4, true>(p);
     } else {
 #pragma unroll
         for (int k = 0; k < 3; ++k)
@@ -389,7 +378,7 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
         storev<4, true>(m, mm);
         storev<4, true>(v, vv);
         if constexpr (MASTER) storev<4, true>(mst, x);
-        if (fit) storev<4, true>(p, x); else storev<4, false>(p, x);
+        storev<4, true>(p, x);
     } else {
 #pragma unroll
         for (int k = 0; k < 3; ++k)
@@ -411,10 +400,16 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {
     x = max(x, dpp<0x141>(x));         // halves of 8 mirrored
     return max(x, dpp<0x140>(x));      // rows of 16 mirrored
 }
+// (the compiler would take these three to the vector side)
+__device__ __forceinline__ uint32_t smax(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("s_max_u32 %0, %1, %2" : "=s"(r) : "s"(a), "s"(b) : "scc");
+    return r;
+}
 __device__ __forceinline__ uint32_t rows_max(uint32_t x) {
     const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
     const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
-    return max(max(a, b), max(c, d));
+    return smax(smax(a, b), smax(c, d));
 }
 
 struct Lane8 { Vec<4> g, x; uint32_t cm, cv; };      // what a lane loads: gradient, parameter, codes
@@ -425,40 +420,68 @@ __device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0703u), __builtin_amdgcn_perm(b, a, 0x0C0C0703u), 0x05040100u);
 }
 __device__ __forceinline__ float power(int field) { return __uint_as_float((uint32_t)field << 23); }      // 2^(field - 127), 1 <= field <= 254
+// byte K of x at bits 20 ... 27
+template <int K> __device__ __forceinline__ float code_bits(uint32_t x, uint32_t twenty) {
+    uint32_t r;
+    if constexpr (K == 0) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(twenty), "v"(x));
+    if constexpr (K == 1) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(twenty), "v"(x));
+    if constexpr (K == 2) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(twenty), "v"(x));
+    if constexpr (K == 3) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(twenty), "v"(x));
+    return __uint_as_float(r);
+}
 // block exponents for which every power of two below is a normal number, and no value that the codes stand for is denormal
 #define M_LOW 40
 #define M_HIGH 139
 #define V_LOW 40
 #define V_HIGH 155
 
+// The factors once more, as the fast path takes them: p' = p decay - m' / (sqrt(v') root + eps), both divided by the step size.
+// `plain`: whether it applies at all (a step size of zero does not).  `guard`: whether eps is so small that a root flushed to
+// zero (v' below 2^-126: the root below 1e-19, 3e-18 with the largest factor that b2 = 0.999 gives) could be seen.
+struct Fast { float root, eps; bool plain, guard; };
+__device__ __forceinline__ Fast fast_of(const Coef& c) {
+    const float r = __builtin_amdgcn_rcpf(c.step_size);
+    const int ss = __builtin_amdgcn_readfirstlane(__float_as_int(c.step_size)), eps = __builtin_amdgcn_readfirstlane(__float_as_int(c.eps));
+    const int isq = __builtin_amdgcn_readfirstlane(__float_as_int(c.inv_sqrt_bc2));
+    return {c.inv_sqrt_bc2 * r, c.eps * r, __int_as_float(ss) > 1e-20f && __int_as_float(ss) < 1e20f,
+            !(__int_as_float(eps) >= 1e-10f && __int_as_float(isq) < 40.f)};
+}
+
 // A whole block of finite numbers of ordinary size: the definition above with its scalings as multiplications by powers of two
 // (exact, so that b2 and the scale of v are one factor), the first moment's codes decoded by the hardware (they are OCP e4m3:
 // bias 7, code exponent 14 = 2^7), and everything shifted up by 4 so that a code is the top byte of its word.  Returns false, with
 // nothing changed, where it does not apply: a code or a moment that is not finite, block exponents out of the ranges above, or a
-// second moment below 2^-126 (the square root instruction would flush it).
-__device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], float gs, const Coef& c) {
+// second moment below 2^-126 (the square root instruction would flush it).  Its 150 vector instructions, of 190 a block in all, are what
+// bounds the update of 16-bit parameters: in 92 % of the cycles one is at work.
+__device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], float gs, const Coef& c,
+                                           const Fast& f) {
 #pragma clang fp contract(off)
-    if (sm < M_LOW || sm > M_HIGH || sv < V_LOW || sv > V_HIGH) return false;
+    if (!f.plain || sm < M_LOW || sm > M_HIGH || sv < V_LOW || sv > V_HIGH) return false;
     // a byte 0x7F / 0xFF among the first moment's codes, a byte 0xFF among the second's
     uint32_t odd = ((r.cm & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
     odd |= ((r.cv & 0x7F7F7F7Fu) + 0x01010101u) & r.cv & 0x80808080u;
     const float m_scale = power(sm - 7), v_scale = power(sv - V_TOP + 127) * c.b2;
     const f2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(r.cm, m_scale, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(r.cm, m_scale, true);
-    float m[4] = {lo.x, lo.y, hi.x, hi.y}, v[4];
-    bool tiny = false;
+    float m[4] = {lo.x, lo.y, hi.x, hi.y};
+    float v[4] = {code_bits<0>(r.cv, 20), code_bits<1>(r.cv, 20), code_bits<2>(r.cv, 20), code_bits<3>(r.cv, 20)};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float g = r.g.x[k] * gs;
         m[k] = m[k] * c.b1 + g * c.omb1;
-        v[k] = __uint_as_float(k < 3 ? (r.cv << (20 - 8 * k)) & 0x0FF00000u : (r.cv >> 4) & 0x0FF00000u) * v_scale + (g * g) * c.omb2;
-        tiny |= __builtin_amdgcn_classf(v[k], 0x90);               // denormal
+        v[k] = v[k] * v_scale + (g * g) * c.omb2;
     }
     const float ma = fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])));
     const uint32_t va = max(max(__float_as_uint(v[0]), __float_as_uint(v[1])), max(__float_as_uint(v[2]), __float_as_uint(v[3])));
     const uint32_t mr = row_max(__float_as_uint(ma)), vr = row_max(va);
     const uint32_t mb = rows_max(mr), vb = rows_max(vr);                     // (m' is finite where v' is)
     const int nm = (int)(mb >> 23), nv = (int)(vb >> 23);
-    if (nm < M_LOW || nm > M_HIGH || nv < V_LOW || nv > V_HIGH || __any(tiny | (odd != 0))) return false;
+    if (nm < M_LOW || nm > M_HIGH || nv < V_LOW || nv > V_HIGH || __any(odd != 0)) return false;
+    if (f.guard) {
+        bool tiny = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tiny |= __builtin_amdgcn_classf(v[k], 0x90);               // denormal
+        if (__any(tiny)) return false;
+    }
     sm = nm;
     sv = nv;
     const float m_up = power(M_TOP - nm + 127), v_up = power(V_TOP - nv + 127);
@@ -467,13 +490,15 @@ __device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t 
     for (int k = 0; k < 4; ++k) {
         {
 #pragma clang fp contract(fast)
-            const float d = __builtin_amdgcn_sqrtf(v[k]) * c.inv_sqrt_bc2 + c.eps;
-            r.x.x[k] = r.x.x[k] * c.decay - c.step_size * (m[k] * __builtin_amdgcn_rcpf(d));
+            const float d = __builtin_amdgcn_sqrtf(v[k]) * f.root + f.eps;
+            r.x.x[k] = r.x.x[k] * c.decay - m[k] * __builtin_amdgcn_rcpf(d);
         }
+        // 16 r_m and 16 r_v: the word's upper and lower half at bits 8 ... 23, 0x80 below
         const uint32_t w = element_word(bkey, j_step[k]);
-        zm[k] = (__float_as_uint(fabsf(m[k]) * m_up) << 4) + ((w >> 8 & 0xFFFF00u) | 0x80u);
-        const uint32_t y = max(__float_as_uint(v[k] * v_up), min(__float_as_uint(v[k]), 1u << 20));          // (at least 1 where v' > 0)
-        zv[k] = (y << 4) + ((w << 8 & 0xFFFF00u) | 0x80u);
+        zm[k] = (__float_as_uint(fabsf(m[k]) * m_up) << 4) + __builtin_amdgcn_perm(w, 0x80u, 0x0C070600u);
+        // at least code 1 where v' > 0: the middle one of the scaled value, the value (larger, as its exponent is above 30) and code 1
+        const float y = __builtin_amdgcn_fmed3f(v[k] * v_up, v[k], __uint_as_float(1u << 20));
+        zv[k] = (__float_as_uint(y) << 4) + __builtin_amdgcn_perm(w, 0x80u, 0x0C050400u);
     }
     const uint32_t sign = top_bytes(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])) & 0x80808080u;
     r.cm = sign | top_bytes(zm[0], zm[1], zm[2], zm[3]);
@@ -511,16 +536,19 @@ template <typename T> struct Block8 {
     GLOBAL T* p;
     GLOBAL float* mst;
     GLOBAL uint8_t *mc, *vc;
-    bool whole, fit;
+    bool whole;
     int n;
 };
 template <typename T, bool MASTER>
 __device__ __forceinline__ Lane8 load_block(const Block8<T>& b, uint32_t j0) {
+    // (measured both ways: with the non-temporal kind 302 M bf16 elements take 523 instead of 564 us, but fp32 ones, 295 M, 776 instead
+    //  of 752, and bf16 ones with masters 821 instead of 803)
+    constexpr bool NT = sizeof(T) == 2 && !MASTER;
     Lane8 r = {};
     if (b.whole) {
-        r.g = b.fit ? loadv<4, true>(b.g + j0) : loadv<4, false>(b.g + j0);
+        r.g = loadv<4, NT>(b.g + j0);
         if constexpr (MASTER) r.x = loadv<4, true>(b.mst + j0);
-        else r.x = b.fit ? loadv<4, true>((const GLOBAL T*)b.p + j0) : loadv<4, false>((const GLOBAL T*)b.p + j0);
+        else r.x = loadv<4, NT>((const GLOBAL T*)b.p + j0);
         r.cm = ldq<true, u1a>(b.mc + j0);
         r.cv = ldq<true, u1a>(b.vc + j0);
     } else {
@@ -539,7 +567,7 @@ template <typename T, bool MASTER>
 __device__ __forceinline__ void store_block(const Block8<T>& b, uint32_t j0, const Lane8& r) {
     if (b.whole) {
         if constexpr (MASTER) storev<4, true>(b.mst + j0, r.x);
-        if (b.fit) storev<4, true>(b.p + j0, r.x); else storev<4, false>(b.p + j0, r.x);
+        storev<4, true>(b.p + j0, r.x);
         stq<true>(b.mc + j0, (u1a)r.cm);
         stq<true>(b.vc + j0, (u1a)r.cv);
     } else {
@@ -555,9 +583,9 @@ __device__ __forceinline__ void store_block(const Block8<T>& b, uint32_t j0, con
 }
 
 // Blocks of a wave, one after another.  What every wave does once (addresses, factors) is a third of its instructions with one block:
-// 16-bit parameters without masters (10 bytes an element) are bound by instructions and take four (302 M elements 763, 637, 593 us
+// 16-bit parameters without masters (10 bytes an element) are bound by instructions and take four (302 M elements 731, 601, 524 us
 // with 1, 2, 4 blocks), with masters two (19 M elements in odd sizes 57.5, 49.4, 51.0 us); fp32 (16 bytes) is bound by memory, which
-// favours short runs of a workgroup, and takes one (295 M elements 761, 862, 899 us; 6.2 TB/s).
+// favours short runs of a workgroup, and takes one (295 M elements 772, 777, 840 us).
 template <typename T, bool MASTER> constexpr int blocks8() { return sizeof(T) == 4 ? 1 : MASTER ? 2 : 4; }
 template <typename T, bool MASTER>
 __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
@@ -570,6 +598,7 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimT
     const VcrOptimTensor& R = tensors[at.tensor];
     const float gs = clip ? clip->gscale : gscale;
     const Entry e = enter(R, pk.group[R.group - g0]);
+    const Fast fast = fast_of(e.coef);
     const uint32_t j0 = (threadIdx.x & 63) * 4;
     const uint32_t j_step[4] = {j0 * LANE_STEP, (j0 + 1) * LANE_STEP, (j0 + 2) * LANE_STEP, (j0 + 3) * LANE_STEP};
     const uint32_t key = mix32(mix32(mix32(seed) + (uint32_t)__builtin_amdgcn_readfirstlane(e.step)) + (uint32_t)R.index);
@@ -588,13 +617,12 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimT
         b.mc = global((uint8_t*)R.m) + first;
         b.vc = global((uint8_t*)R.v) + first;
         b.whole = have >= VCR_OPT_BLOCK;
-        b.fit = aligned(b.p, b.g);
         b.n = b.whole ? 4 : have > j0 ? (int)min((long long)4, have - j0) : 0;
         Lane8 r = load_block<T, MASTER>(b, j0);
         GLOBAL uint8_t *ms = global(R.m_scale) + blk, *vs = global(R.v_scale) + blk;
         int sm = __builtin_amdgcn_readfirstlane(*ms), sv = __builtin_amdgcn_readfirstlane(*vs);
         const uint32_t bkey = mix32(key + blk);
-        if (!b.whole || !block_fast(r, sm, sv, bkey, j_step, gs, e.coef)) block_any(r, sm, sv, bkey, j_step, b.n, gs, e.coef);
+        if (!b.whole || !block_fast(r, sm, sv, bkey, j_step, gs, e.coef, fast)) block_any(r, sm, sv, bkey, j_step, b.n, gs, e.coef);
         store_block<T, MASTER>(b, j0, r);
         if (j0 == 0) { *ms = (uint8_t)sm; *vs = (uint8_t)sv; }
     }
@@ -825,9 +853,8 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
         }
         if (any) {
             const dim3 block(VCR_OPT_THREADS);
-            const size_t lds = a.param_type == VCR_F32 ? VCR_OPT_LDS_FP32 : 0;
             const float gs = (float)a.grad_scale;
-#define LAUNCH32(T, M) hipLaunchKernelGGL((adamw_kernel<T, M>), dim3((uint32_t)nchunks * parts<1>()), block, lds, st, tensors, chunks, words, clip, gs, pk, t0, g0)
+#define LAUNCH32(T, M) hipLaunchKernelGGL((adamw_kernel<T, M>), dim3((uint32_t)nchunks * parts<1>()), block, 0, st, tensors, chunks, words, clip, gs, pk, t0, g0)
 #define LAUNCH8(T, M) hipLaunchKernelGGL((adamw8_kernel<T, M>), dim3((uint32_t)nchunks * parts<blocks8<T, M>()>()), block, 0, st, tensors, chunks, words, clip, gs, pk, t0, g0, a.seed)
 #define LAUNCH(T, M) do { if (a.state_bits == 32) LAUNCH32(T, M); else LAUNCH8(T, M); } while (0)
             if (a.param_type == VCR_F32) LAUNCH(float, false);
