@@ -505,10 +505,10 @@ class AdamW:
         (uint8 codes and scales); `moments()` gives the values another optimizer could load."""
         template = torch.optim.AdamW([torch.zeros(1)]).param_groups[0]
         state, groups, idx = {}, [], 0
-        for i, (key, p) in enumerate(zip(self._keys(), self._tensors())):
-            st = self.state.get(key)
-            if st is not None:
-                state[i] = {k: torch.tensor(float(int(t))) if k == "step" else t for k, t in st.items()}
+        held = [(i, self.state[key]) for i, key in enumerate(self._keys()) if key in self.state]
+        steps = torch.stack([st["step"].reshape(()) for _, st in held]).tolist() if held else []          # (one wait for all)
+        for (i, st), t in zip(held, steps):
+            state[i] = {k: torch.tensor(float(t)) if k == "step" else v for k, v in st.items()}
         for g in self.param_groups:
             wg = {k: v for k, v in template.items() if k != "params"}
             wg.update({k: v for k, v in g.items() if k != "params"})
@@ -530,10 +530,11 @@ class AdamW:
                 raise ValueError(f"AdamW: group {k}: {len(wg['params'])} tensors saved, {len(g['params'])} here")
             order += list(wg["params"])
         new = {}
-        for i, key, p in zip(order, self._keys(), self._tensors()):
-            st = sd["state"].get(i)
-            if st is not None:
-                new[key] = self._converted(key, p, st)
+        held = [(key, p, sd["state"][i]) for i, key, p in zip(order, self._keys(), self._tensors()) if i in sd["state"]]
+        if held:
+            steps = torch.tensor([int(round(float(st["step"]))) for _, _, st in held], dtype=torch.int32).to(held[0][1].device).unbind()
+            for (key, p, st), t in zip(held, steps):
+                new[key] = self._converted(key, p, st, t)
         for wg, g in zip(sd["param_groups"], self.param_groups):
             for k in ("lr", "eps", "weight_decay"):
                 if k in wg:
@@ -542,12 +543,12 @@ class AdamW:
                 g["betas"] = tuple(wg["betas"])
         self.state = new
 
-    def _converted(self, key, p, st):
+    def _converted(self, key, p, st, step):
         dev, n, nb = p.device, p.numel(), -(-p.numel() // BLOCK)
         for k in ("exp_avg", "exp_avg_sq"):
             if st[k].numel() != n:
                 raise ValueError(f"optimizer state of {key!r} has shape {tuple(st[k].shape)}, parameter {tuple(p.shape)}")
-        out = dict(step=torch.tensor(int(round(float(st["step"]))), dtype=torch.int32).to(dev))
+        out = dict(step=step)
         as_held = lambda t, dt: t.detach().to(device=dev, dtype=dt).contiguous()  # noqa: E731
         codes = st["exp_avg"].dtype == torch.uint8
         if codes:
