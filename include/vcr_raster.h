@@ -300,10 +300,11 @@ int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, co
                         const float* const* exp_avg_sq, void* stream);
 /* 2-norm over all tensors, mixed types (HOST arrays): *norm = sqrt(sum of squares) * |grad_scale|, and with `clip` (8 bytes on the
  * device) the factor grad_scale * min(1, max_norm / (norm + 1e-6)) of a clipped step, which is skipped if the norm is not finite.
- * `partials`: scratch for `capacity` >= vcr_grad_norm_partials(ntensors, numel) doubles. */
+ * `partials`: scratch for `capacity` >= vcr_grad_norm_partials(ntensors, numel) doubles.  `read_again` != 0: the tensors are read
+ * again soon (a clipped step) and kept in the caches. */
 int vcr_grad_norm_partials(int ntensors, const int64_t* numel);
 int vcr_grad_norm(int ntensors, const void* const* tensors, const int64_t* numel, const int32_t* types, double* partials,
-                  int capacity, double grad_scale, double max_norm, float* norm, void* clip, void* stream);
+                  int capacity, double grad_scale, double max_norm, int read_again, float* norm, void* clip, void* stream);
 /* tensors *= min(1, max_norm / (*norm + 1e-6)), in place. */
 int vcr_clip_gradients(int ntensors, void* const* tensors, const int64_t* numel, const int32_t* types, const float* norm,
                        double max_norm, void* stream);

@@ -141,7 +141,7 @@ SYMBOLS = {
     "vcr_moments8_decode": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_void_p]),
     "vcr_moments8_encode": (C.c_int, [C.c_int] + [C.c_void_p] * 5),
     "vcr_grad_norm_partials": (C.c_int, [C.c_int, C.c_void_p]),
-    "vcr_grad_norm": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_double, C.c_double] + [C.c_void_p] * 3),
+    "vcr_grad_norm": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_double, C.c_double, C.c_int] + [C.c_void_p] * 3),
     "vcr_clip_gradients": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_double, C.c_void_p]),
     "vcr_densify_stats": (C.c_int, [C.c_int] + [C.c_void_p] * 6),
     "vcr_depth_to_normal_forward": (C.c_int, [C.c_int, C.c_int] + [C.c_float] * 4 + [C.c_void_p] * 3),

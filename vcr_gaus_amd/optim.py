@@ -73,14 +73,16 @@ class _List:
         return self.n, _address(self.ptrs), _address(self.numels), _address(self.kinds)
 
 
-def _norm(args, out, grad_scale=1.0, max_norm=0.0, clip=False):
+def _norm(args, out, again=False, grad_scale=1.0, max_norm=0.0, clip=False):
     """Launches the norm of the listed tensors into `out`; -> with `clip` the buffer whose first 8 bytes are the clipped step's factor.
+    `again`: the tensors are read again right behind.
     The scratch belongs to this call (allocated on the current stream): two captured calls share nothing."""
     lib = _lib.load()
     room = lib.vcr_grad_norm_partials(args[0], args[2])
     buffer = torch.empty(room + 1, dtype=torch.float64, device=out.device)
     at = buffer.data_ptr()
-    _lib.check(lib.vcr_grad_norm(*args, at + 8, room, grad_scale, max_norm, out.data_ptr(), at if clip else None, _lib.stream_of(out)))
+    _lib.check(lib.vcr_grad_norm(*args, at + 8, room, grad_scale, max_norm, int(again), out.data_ptr(),
+                                 at if clip else None, _lib.stream_of(out)))
     return buffer
 
 
@@ -116,7 +118,7 @@ def clip_grad_norm_(parameters, max_norm):
     norm, words = torch.empty((), device=dev), _List(work, dtypes)
 
     def both():
-        _norm(words.args(), norm)
+        _norm(words.args(), norm, True)
         _lib.check(_lib.load().vcr_clip_gradients(*words.args(), norm.data_ptr(), max_norm, _lib.stream_of(norm)))
 
     _on(dev, both)
@@ -411,7 +413,7 @@ class AdamW:
             else:
                 words = (array("Q", [ptrs[i] for i in live]), array("q", [plan.numels[i] for i in live]),
                          array("i", [_TYPES[plan.dtypes[i]] for i in live]))
-            clip = _norm((len(words[0]), *map(_address, words)), norm, float(self.grad_scale), max_norm, True)
+            clip = _norm((len(words[0]), *map(_address, words)), norm, True, float(self.grad_scale), max_norm, True)
         for b in plan.buckets:
             mine = ptrs if b.every else array("Q", [ptrs[i] for i in b.at])
             a = b.args
