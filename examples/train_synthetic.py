@@ -22,6 +22,9 @@ def main():
     ap.add_argument("--views", type=int, default=24)
     ap.add_argument("--iters", type=int, default=1500)
     ap.add_argument("--preset", default="dtu_c3")
+    ap.add_argument("--optimizer", choices=["adam", "adamw"], default="adam")
+    ap.add_argument("--state-bits", type=int, choices=[8, 32], default=32, help="of AdamW's moments")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="AdamW: clip the gradients' norm")
     args = ap.parse_args()
     from vcr_gaus_amd import synthetic
     from vcr_gaus_amd.gaussian_renderer import render
@@ -33,7 +36,8 @@ def main():
     tr = make_synthetic_trainer(raw, cams, dev, preset=args.preset, gt_jitter=0.3,
                                 optim={"densify_from_iter": 100, "densification_interval": 100, "densify_until_iter": 1000,
                                        "opacity_reset_interval": 600, "prune": {"iterations": [1200]},
-                                       "consistent_normal_from_iter": 500})
+                                       "consistent_normal_from_iter": 500, "optimizer": args.optimizer,
+                                       "state_bits": args.state_bits, "max_grad_norm": args.max_grad_norm})
 
     def eval_psnr():
         tr.join_side()          # the last SH update may still be pending on / running on the trainer's second stream

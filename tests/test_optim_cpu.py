@@ -110,6 +110,26 @@ def test_replacing_state_makes_the_optimizer_look_again():
         assert opt._plan is None
 
 
+def test_copies_and_added_groups():
+    import copy
+    import pickle
+    opt = AdamW([P(3)], lr=0.5, state_bits=8)
+    opt.state = {"0": dict(step=torch.zeros((), dtype=torch.int32))}
+    opt._plan = lambda: None                            # (something that cannot be copied)
+    for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert twin._plan is None and twin.state_bits == 8 and int(twin.state["0"]["step"]) == 0
+        twin._plan = "built"
+        twin.state["0"]["step"] = torch.ones((), dtype=torch.int32)
+        assert twin._plan is None and int(opt.state["0"]["step"]) == 0
+    q = P(4)
+    opt.add_param_group(dict(params=q, name="late", lr=0.1))
+    assert opt._keys() == ["0", "late"] and opt.param_groups[1]["weight_decay"] == 1e-2
+    for bad in (dict(params=[q]), dict(params=[P(1)], lr=-1.0), dict(lr=1.0)):
+        with pytest.raises((ValueError, TypeError)):
+            opt.add_param_group(bad)
+        assert len(opt.param_groups) == 2
+
+
 # ---- C entries: refused before anything reaches a device -----------------------------------------------------------------
 def _words(kind, values):
     a = array(kind, values)

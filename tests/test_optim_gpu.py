@@ -185,6 +185,8 @@ def test_refusals_on_the_device(device):
         grad_norm([torch.ones(3, device=device), torch.ones(3)])
     with pytest.raises(ValueError, match="`out`"):
         grad_norm([p], out=torch.empty(2, device=device))
+    with pytest.raises(ValueError, match="one float32 element on the device"):
+        AdamW([p], lr=torch.tensor(1e-3))
     # a parameter shortened in place: the gradient no longer fits what the plan holds, and the plan is looked at before any launch
     opt = AdamW([p])
     p.grad = torch.ones_like(p)

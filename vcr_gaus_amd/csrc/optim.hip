@@ -349,6 +349,8 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
     const GLOBAL T* g = global((const T*)pk.g[at.tensor - t0]);
     if (!g || (clip && clip->skip)) return;
     const VcrOptimTensor& R = tensors[at.tensor];
+    const uint32_t group = (uint32_t)(R.group - g0);
+    if (group >= VCR_OPT_GROUPS || (MASTER && !R.master)) return;             // (a plan that was made for another call)
     const float gs = clip ? clip->gscale : gscale;
     const long long off = at.first + threadIdx.x * 4, left = R.numel - off;
     GLOBAL T* p = global((T*)R.p) + off;
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
                 x.x[k] = MASTER ? mst[k] : load1(p + k);
             }
     }
-    const Entry e = enter(R, pk.group[R.group - g0]);
+    const Entry e = enter(R, pk.group[group]);
     const Coef c = e.coef;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -599,8 +601,10 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimT
     const T* grad = (const T*)pk.g[at.tensor - t0];
     if (!grad || (clip && clip->skip)) return;
     const VcrOptimTensor& R = tensors[at.tensor];
+    const uint32_t group = (uint32_t)(R.group - g0);
+    if (group >= VCR_OPT_GROUPS || !R.m_scale || (MASTER && !R.master)) return;       // (a plan that was made for another call)
     const float gs = clip ? clip->gscale : gscale;
-    const Entry e = enter(R, pk.group[R.group - g0]);
+    const Entry e = enter(R, pk.group[group]);
     const Fast fast = fast_of(e.coef);
     const uint32_t j0 = (threadIdx.x & 63) * 4;
     const uint32_t j_step[4] = {j0 * LANE_STEP, (j0 + 1) * LANE_STEP, (j0 + 2) * LANE_STEP, (j0 + 3) * LANE_STEP};
@@ -639,7 +643,7 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) decode_kernel(const VcrOptimT
     const Place at = place<1>(chunks);
     const VcrOptimTensor& R = tensors[at.tensor];
     const long long off = at.first + threadIdx.x * 4, left = R.numel - off;
-    if (left <= 0) return;
+    if (left <= 0 || !R.m_scale) return;
     GLOBAL T *mo = global((T*)out.a[at.tensor - t0]), *vo = global((T*)out.b[at.tensor - t0]);
     const GLOBAL uint8_t *mc = global((const uint8_t*)R.m) + off, *vc = global((const uint8_t*)R.v) + off;
     const int sm = global(R.m_scale)[off / VCR_OPT_BLOCK], sv = global(R.v_scale)[off / VCR_OPT_BLOCK];
@@ -683,6 +687,7 @@ __global__ void __launch_bounds__(256) encode_kernel(const VcrOptimTensor* __res
                                                      PairPack in, int t0) {
     const uint2 cw = chunks[blockIdx.x];
     const VcrOptimTensor& R = tensors[cw.x];
+    if (!R.m_scale) return;
     const GLOBAL float *mi = global((const float*)in.a[cw.x - t0]), *vi = global((const float*)in.b[cw.x - t0]);
     GLOBAL uint8_t *mc = global((uint8_t*)R.m), *vc = global((uint8_t*)R.v);
     const uint32_t lane = threadIdx.x & 63;

@@ -165,7 +165,7 @@ class _Bucket:
 
 
 class _Plan:
-    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "numels", "buckets", "device", "stream", "captured", "covered")
+    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "numels", "buckets", "device", "stream", "captured", "covered", "keep")
 
 
 class AdamW:
@@ -196,19 +196,14 @@ class AdamW:
             raise ValueError(f"AdamW: state_bits = {state_bits}: 8 or 32")
         self.defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay)
         groups = params if isinstance(params[0], dict) else [dict(params=params)]
-        self.param_groups = []
-        for g in groups:
-            if not isinstance(g, dict) or "params" not in g:
-                raise TypeError("AdamW: groups are dictionaries with `params`")
-            ps = g["params"]
-            g["params"] = [ps] if isinstance(ps, torch.Tensor) else list(ps)
-            for k, v in self.defaults.items():
-                g.setdefault(k, v)
-            self.param_groups.append(g)
+        self.param_groups = [self._filled(g) for g in groups]
         self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed) & 0xFFFFFFFF
         self.grad_scale = 1.0
         self._plan, self._captured, self._rates = None, [], None
         self._state_dict = _Watched(self)
+        self._check_groups()
+
+    def _check_groups(self):
         for k, g in enumerate(self.param_groups):
             self._hyper(k, g)
         seen = set()
@@ -218,6 +213,31 @@ class AdamW:
             if id(p) in seen:
                 raise ValueError("AdamW: a parameter appears twice")
             seen.add(id(p))
+
+    def add_param_group(self, group):
+        """One more group (a dict with `params`), with this optimizer's defaults for what it does not say."""
+        self.param_groups.append(self._filled(group))
+        try:
+            self._check_groups()
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
+
+    def _filled(self, g):
+        if not isinstance(g, dict) or "params" not in g:
+            raise TypeError("AdamW: groups are dictionaries with `params`")
+        ps = g["params"]
+        g["params"] = [ps] if isinstance(ps, torch.Tensor) else list(ps)
+        for k, v in self.defaults.items():
+            g.setdefault(k, v)
+        return g
+
+    def __getstate__(self):          # (copies and pickles: plans hold addresses and are made anew)
+        return dict(self.__dict__, _plan=None, _captured=[], _rates=None, _state_dict={k: dict(v) for k, v in self.state.items()})
+
+    def __setstate__(self, d):
+        self.__dict__.update(d)
+        self.state = d["_state_dict"]
 
     # ---- what is trained ---------------------------------------------------------------------------------------------
     @property
@@ -313,6 +333,7 @@ class AdamW:
             self._check_state(key, p, st)
             by.setdefault(_TYPES[p.dtype], []).append(i)
         plan.buckets, plan.covered = [], sum(map(len, by.values()))
+        plan.keep = [t for at in by.values() for i in at for t in self.state[keys[i]].values()]          # (a graph may hold their addresses)
         for kind, at in by.items():
             b = _Bucket()
             b.type, b.at, b.n, b.every = kind, at, len(at), len(at) == len(plan.params)
@@ -359,11 +380,14 @@ class AdamW:
             self._captured.append(plan)          # the graph holds its addresses
         return plan, stream.cuda_stream
 
-    def _group_table(self):
+    def _group_table(self, device):
         """The groups' rates as the library takes them, formed anew only where one has changed."""
         key = [(g["lr"].data_ptr() if isinstance(g["lr"], torch.Tensor) else float(g["lr"]), g["betas"], g["eps"], g["weight_decay"])
                for g in self.param_groups]
         if self._rates is None or self._rates[0] != key:
+            for k, g in enumerate(self.param_groups):
+                if isinstance(g["lr"], torch.Tensor) and g["lr"].device != device:
+                    raise ValueError(f"AdamW: group {k}: `lr` is on {g['lr'].device}, the parameters are on {device}")
             self._rates = key, (_lib.VcrOptimGroup * len(key))(*[self._hyper(k, g) for k, g in enumerate(self.param_groups)])
         return self._rates[1]
 
@@ -404,7 +428,7 @@ class AdamW:
         return norm
 
     def _launch(self, plan, ptrs, live, max_norm, stream):
-        groups, lib, norm, clip = self._group_table(), _lib.load(), None, None
+        groups, lib, norm, clip = self._group_table(plan.device), _lib.load(), None, None
         if max_norm is not None:
             norm = torch.empty((), device=plan.device)
             if len(live) == len(ptrs) and len(plan.buckets) == 1:
@@ -436,6 +460,7 @@ class AdamW:
         yet has zeros.  8-bit moments are exact in bfloat16."""
         params = self._tensors()
         outs = []
+        dtype = next((o[0].dtype for o in (exp_avgs, exp_avg_sqs) if o), dtype)
         for given in (exp_avgs, exp_avg_sqs):
             if given is None:
                 given = [torch.empty(p.shape, dtype=dtype, device=p.device) for p in params]
