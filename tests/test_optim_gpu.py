@@ -787,3 +787,117 @@ def test_model_checkpoints_pass_between_optimizers(device, bits):
         assert all(torch.equal(m4.optimizer.state[k]["exp_avg_sq"], tr.model.optimizer.state[k]["exp_avg_sq"]) for k in GROUPS)
     with pytest.raises(ValueError, match="optim.optimizer"):
         restored(cap, optimizer="sgd")
+
+
+def test_settings_of_adamw_are_refused_with_adam(device):
+    for kw in (dict(max_grad_norm=1.0), dict(weight_decay=0.1), dict(state_bits=8)):
+        with pytest.raises(ValueError, match="need optim.optimizer"):
+            adamw_trainer(device, optimizer="adam", **kw)
+
+
+# ---- what is shared, kept and changed behind a caller's back -------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [32, 8])
+def test_set_moments_copies(device, bits):
+    """One tensor given for both moments, and changed afterwards: each moment has its own memory with the values as given."""
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([700], F, device, seed=91)
+    opt = AdamW(params, state_bits=bits)
+    z = torch.full((700,), 0.25, device=device)
+    opt.set_moments("0", z, z, step=4)
+    z.fill_(9.0)
+    m, v = opt.moments()
+    assert bool((m[0] == 0.25).all()) and bool((v[0] == 0.25).all()) and int(opt.state["0"]["step"]) == 4
+    assert opt.state["0"]["exp_avg"].data_ptr() != opt.state["0"]["exp_avg_sq"].data_ptr()
+    opt.step()
+    m, v = opt.moments_of("0")
+    g = params[0].grad
+    want = (0.9 * 0.25 + 0.1 * g, 0.999 * 0.25 + 0.001 * g * g)
+    for got, w in zip((m, v), want):           # (8 bits: less than one code step, 2^-3 of the value, and the smallest code)
+        off = 2.0 ** -22 * (w.abs() + 0.25 + g.abs()) if bits == 32 else w.abs() * 2.0 ** -3 + 2.0 ** -16
+        assert bool(((got - w).abs() <= off).all())
+    assert int(opt.state["0"]["step"]) == 5
+    with pytest.raises(KeyError, match="no parameter"):
+        opt.set_moments("1", z, z)
+    with pytest.raises(ValueError, match="values for"):
+        opt.set_moments("0", z[:3], z)
+
+
+def test_rates_changed_in_place_are_seen(device):
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([300], F, device, seed=92)
+    twin = [torch.nn.Parameter(params[0].detach().clone())]
+    twin[0].grad = params[0].grad.clone()
+    betas = [0.9, 0.999]
+    opt, ref = AdamW([dict(params=params, betas=betas)]), AdamW(twin)
+    opt.step()
+    ref.step()
+    betas[0] = 0.5
+    ref.param_groups[0]["betas"] = (0.5, 0.999)
+    opt.step()
+    ref.step()
+    assert torch.equal(params[0], twin[0]) and torch.equal(opt.state["0"]["exp_avg"], ref.state["0"]["exp_avg"])
+    opt.param_groups[0]["lr"] = torch.tensor(1e-3, device=device)
+    opt.step()
+    opt.param_groups[0]["lr"] = torch.tensor(1e-3, device=device, dtype=torch.float64)
+    with pytest.raises(ValueError, match="one float32 element"):
+        opt.step()
+
+
+def test_a_captured_rate_stays_alive(device):
+    import weakref
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([64], F, device, seed=93)
+    opt = AdamW(params, lr=torch.tensor(1e-3, device=device))
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    alive = weakref.ref(opt.param_groups[0]["lr"])
+    opt.param_groups[0]["lr"] = 0.5
+    opt.step()
+    assert alive() is not None and float(alive()) == np.float32(1e-3)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(opt.state["0"]["step"]) == 3
+
+
+def test_a_step_between_forward_and_backward_is_noticed(device):
+    from vcr_gaus_amd.optim import AdamW, clip_grad_norm_
+    a, b = (torch.nn.Parameter(torch.ones(5, device=device)) for _ in range(2))
+    a.grad = torch.ones_like(a)
+    opt = AdamW([a, b])
+    y, z = (a * a).sum(), (b * b).sum()
+    opt.step()
+    z.backward()                                  # b had no gradient and is as it was
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    before = a.grad._version
+    clip_grad_norm_([a], 1e-3)
+    assert a.grad._version > before
+
+
+def test_state_freed_while_another_stream_uses_it(device):
+    """The optimizer goes while its last step still runs on a side stream: its memory is not handed out before that step is done."""
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([1 << 20], F, device, seed=94)
+    opt = AdamW(params)
+    opt.step()
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)             # (of the order of 10 ms)
+        opt.step()
+    del opt
+    fresh = [torch.full((1 << 20,), 7.0, device=device) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(bool((t == 7.0).all()) for t in fresh)
+
+
+def test_one_name_is_a_name(device):
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([8, 8], F, device, seed=95)
+    opt = AdamW([dict(params=[params[0]], name="f"), dict(params=[params[1]], name="f_dc")])
+    old = params[0].detach().clone()
+    opt.step(only="f_dc")
+    assert torch.equal(params[0], old) and params[0].grad is not None and params[1].grad is None

@@ -630,6 +630,9 @@ class GaussianModel:
                                "aux": True})
         kind = getattr(training_args, "optimizer", "adam")
         if kind == "adam":
+            if getattr(training_args, "max_grad_norm", None) or float(getattr(training_args, "weight_decay", 0.0)) or \
+                    int(getattr(training_args, "state_bits", 32)) != 32:
+                raise ValueError("optim.max_grad_norm, weight_decay and state_bits need optim.optimizer = \"adamw\"")
             self.optimizer = FusedAdam(groups, eps=1e-15)
         elif kind == "adamw":
             self.optimizer = GaussianAdamW(groups, eps=1e-15, weight_decay=float(getattr(training_args, "weight_decay", 0.0)),

@@ -19,6 +19,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TENSORS = {torch.Tensor, torch.nn.Parameter}
 _PTR, _CONTIGUOUS, _NUMEL, _DEVICE = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.get_device
 _GRAD, _DTYPE = attrgetter("grad"), attrgetter("dtype")
+_changed = torch.autograd.graph.increment_version        # (a backward that needs the old values says so instead of using the new ones)
 # Lists of many tensors are looked at attribute by attribute, not tensor by tensor, and go to the library as arrays of words: at 200
 # tensors the host's share of a call is what a user sees (a loop with the same checks took 94 us, the kernels 10).
 
@@ -122,6 +123,7 @@ def clip_grad_norm_(parameters, max_norm):
         _lib.check(_lib.load().vcr_clip_gradients(*words.args(), norm.data_ptr(), max_norm, _lib.stream_of(norm)))
 
     _on(dev, both)
+    _changed(grads)
     for g, w in zip(grads, work):
         if g is not w:
             g.copy_(w)
@@ -165,7 +167,7 @@ class _Bucket:
 
 
 class _Plan:
-    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "numels", "buckets", "device", "stream", "captured", "covered", "keep")
+    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "numels", "buckets", "device", "streams", "captured", "covered", "keep")
 
 
 class AdamW:
@@ -357,7 +359,7 @@ class AdamW:
             plan.buckets.append(b)
         stream = torch.cuda.current_stream(plan.device)
         stream.synchronize()                     # (the upload is finished whatever stream the steps use)
-        plan.stream = stream.cuda_stream
+        plan.streams = {stream.cuda_stream}
         self._plan = plan
         return plan
 
@@ -372,18 +374,21 @@ class AdamW:
             if any(i not in known for i in need):
                 plan = self._build(set(need))
         stream = torch.cuda.current_stream(plan.device)
-        if stream.cuda_stream != plan.stream:
-            for b in plan.buckets:
-                b.plan.record_stream(stream)
-        if not plan.captured and torch.cuda.is_current_stream_capturing():
-            plan.captured = True
-            self._captured.append(plan)          # the graph holds its addresses
+        if stream.cuda_stream not in plan.streams:          # (what is freed later is not given away before this stream is done with it)
+            plan.streams.add(stream.cuda_stream)
+            for t in plan.keep + [b.plan for b in plan.buckets]:
+                t.record_stream(stream)
+        if torch.cuda.is_current_stream_capturing():        # the graph holds these addresses
+            plan.keep += [g["lr"] for g in self.param_groups if isinstance(g["lr"], torch.Tensor)]
+            if not plan.captured:
+                plan.captured = True
+                self._captured.append(plan)
         return plan, stream.cuda_stream
 
     def _group_table(self, device):
         """The groups' rates as the library takes them, formed anew only where one has changed."""
-        key = [(g["lr"].data_ptr() if isinstance(g["lr"], torch.Tensor) else float(g["lr"]), g["betas"], g["eps"], g["weight_decay"])
-               for g in self.param_groups]
+        key = [(float(lr) if not isinstance(lr, torch.Tensor) else (lr.data_ptr(), lr.dtype, lr.numel(), lr.device), *g["betas"], g["eps"],
+                g["weight_decay"]) for g in self.param_groups for lr in (g["lr"],)]
         if self._rates is None or self._rates[0] != key:
             for k, g in enumerate(self.param_groups):
                 if isinstance(g["lr"], torch.Tensor) and g["lr"].device != device:
@@ -394,14 +399,16 @@ class AdamW:
     # ---- the step -----------------------------------------------------------------------------------------------------
     def step(self, only=None, max_norm=None):
         """One update of every parameter that has a gradient (`only`: of the groups with these names; their gradients are released
-        afterwards, as in `FusedAdam.step`).  `max_norm` (infinity: measure and guard, never clip): the gradients count with the factor min(1, max_norm / (norm + 1e-6)), norm
-        the 2-norm of all gradients of this step times `grad_scale`; -> the norm (0-dim float32; nothing waits for it), and if that is
-        not finite in float32 the whole step is skipped on the device: parameters, moments and counters stay.  Without: -> None."""
+        afterwards, as in `FusedAdam.step`).  `max_norm`: the gradients count with the factor min(1, max_norm / (norm + 1e-6)), norm the
+        2-norm of all gradients of this step times `grad_scale`; -> the norm (0-dim float32; nothing waits for it), and if that is not
+        finite in float32 the whole step is skipped on the device: parameters, moments and counters stay.  Infinity as `max_norm`
+        measures and guards, and never clips.  Without `max_norm`: -> None."""
         if max_norm is not None:
             max_norm = _positive(max_norm, "max_norm")
         params = self._tensors()
         grads = list(map(_GRAD, params))
         if only is not None:
+            only = {only} if isinstance(only, str) else set(only)
             flags = [g.get("name") in only for g in self.param_groups for _ in g["params"]]
             grads = [g if f else None for g, f in zip(grads, flags)]
         live = [i for i, g in enumerate(grads) if g is not None]
@@ -415,6 +422,7 @@ class AdamW:
             some = _dense([grads[i] for i in live], "AdamW: gradients")
             fits = all(g.dtype is plan.dtypes[i] and g.numel() == plan.numels[i] for i, g in zip(live, some))
             ptrs = array("Q", bytes(8 * len(grads)))
+            params = [params[i] for i in live]
             for i, g in zip(live, some):
                 ptrs[i], grads[i] = g.data_ptr(), g              # (grads: alive until the launch)
         if not fits:
@@ -422,9 +430,10 @@ class AdamW:
             raise ValueError(f"AdamW: the gradient of {plan.keys[i]!r} has type {grads[i].dtype} and {grads[i].numel()} elements, "
                              f"the parameter {plan.dtypes[i]} and {plan.numels[i]}")
         norm = _on(plan.device, self._launch, plan, ptrs, live, max_norm, stream)
+        _changed(params)
         if only is not None:
-            for i in live:
-                params[i].grad = None
+            for p in params:
+                p.grad = None
         return norm
 
     def _launch(self, plan, ptrs, live, max_norm, stream):
@@ -441,7 +450,7 @@ class AdamW:
         for b in plan.buckets:
             mine = ptrs if b.every else array("Q", [ptrs[i] for i in b.at])
             a = b.args
-            a.grads, a.groups, a.ngroups, a.grad_scale = _address(mine), groups, len(groups), self.grad_scale
+            a.grads, a.groups, a.ngroups, a.grad_scale = _address(mine), groups, len(groups), float(self.grad_scale)
             a.clip = None if clip is None else clip.data_ptr()
             _lib.check(lib.vcr_adamw_step(C.byref(a), stream))
         return norm
@@ -519,11 +528,12 @@ class AdamW:
                 st["master"] = old["master"]
         if step is not None:
             st["step"].fill_(int(step))
-        m, v = (t.detach().to(device=p.device, dtype=torch.float32).reshape(p.shape).contiguous() for t in (exp_avg, exp_avg_sq))
-        if self.state_bits == 32:
-            st["exp_avg"], st["exp_avg_sq"] = m, v
+        given = [t.detach().reshape(p.shape) for t in (exp_avg, exp_avg_sq)]
+        if self.state_bits == 32:                            # (copied: the caller's tensors stay the caller's, also one given twice)
+            for k, t in zip(("exp_avg", "exp_avg_sq"), given):
+                st[k].copy_(t)
         elif p.numel():
-            encode8(m, v, st)
+            encode8(*(t.to(device=p.device, dtype=torch.float32).contiguous() for t in given), st)
         self.state[key] = st
 
     # ---- checkpoints -----------------------------------------------------------------------------------------------------
