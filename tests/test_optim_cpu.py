@@ -253,3 +253,22 @@ def test_random_words_do_not_repeat_between_steps_tensors_and_blocks():
     for other in (R.words(2, 1, 0, 4096), R.words(1, 2, 0, 4096), R.words(1, 1, 1, 4096)):
         assert np.mean(base == other) < 0.01 and abs(np.corrcoef(base.astype(float), other.astype(float))[0, 1]) < 0.1
     assert np.unique(R.words(1, 1, 0, 1 << 16)).size > (1 << 16) * 0.99
+
+
+# ---- native lists, on the host -----------------------------------------------------------------------------------------------
+def test_native_lists_leave_host_tensors_to_the_checks():
+    native = _lib.tensor_list()
+    p = P(3)
+    p.grad = torch.ones(3)
+    assert native.words([p]) is None and native.words([]) is None and native.words(p) is None and native.words([None]) is None
+    assert native.gradients([p], None) is None and native.gradients([], None) is None
+    before = p._version
+    native.changed([p, p.grad, 3], None)
+    assert p._version == before + 1
+    native.changed([p, p.grad], bytes(8) + b"\1" + bytes(7))
+    assert p._version == before + 1 and p.grad._version == 2
+    with torch.inference_mode():
+        q = torch.ones(2)
+    native.changed([q], None)
+    with pytest.raises(TypeError):
+        native.changed((p,), None)

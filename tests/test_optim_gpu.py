@@ -901,3 +901,61 @@ def test_one_name_is_a_name(device):
     old = params[0].detach().clone()
     opt.step(only="f_dc")
     assert torch.equal(params[0], old) and params[0].grad is not None and params[1].grad is None
+
+
+# ---- lists ---------------------------------------------------------------------------------------------------------------------------
+class Named(torch.Tensor):
+    """A tensor of another Python type: not an ordinary list for the native module."""
+
+
+def test_lists_are_the_same_however_they_are_looked_at(device):
+    """Native arrays against the attributes; what is not ordinary is left to the other path, which gives the same results."""
+    from vcr_gaus_amd import _lib
+    from vcr_gaus_amd.optim import grad_norm
+    native = _lib.tensor_list()
+    x = [torch.randn(n, device=device).to(t) for n, t in ((5, F), (0, F), (1000, BF), (77, torch.float16), (300001, F))]
+    index, blob, _ = native.words(x)
+    n = len(x)
+    assert index == device.index and len(blob) == 20 * n
+    assert np.frombuffer(blob, np.uint64, n).tolist() == [t.data_ptr() for t in x]
+    assert np.frombuffer(blob, np.int64, n, 8 * n).tolist() == [t.numel() for t in x]
+    assert np.frombuffer(blob, np.int32, n, 16 * n).tolist() == [0, 0, 1, 2, 0]
+    odd = [x[:1] + [torch.ones(3)], x[:1] + [torch.ones(4, 4, device=device).t()[:2]], x[:1] + [torch.ones(2, device=device).double()], [1.0],
+           [x[0].as_subclass(Named)], [], tuple(x), [torch.ones(3, device=device).to_sparse()], [torch._neg_view(x[0])]]
+    assert all(native.words(o) is None for o in odd)
+    for o in ([x[0].as_subclass(Named)] + x[1:], [torch._neg_view(x[0])] + x[1:]):
+        assert torch.equal(grad_norm(o), grad_norm(x))
+
+
+def test_parameters_are_the_same_however_they_are_looked_at(device):
+    """Gradients that are negated views, not contiguous, or of a subclass: the step of plain ones; flags and missing gradients."""
+    from vcr_gaus_amd import _lib
+    from vcr_gaus_amd.optim import AdamW
+    native = _lib.tensor_list()
+    a, b, c = (torch.nn.Parameter(torch.randn(6, 4, device=device, generator=gen(97, device))) for _ in range(3))
+    g = [torch.randn(6, 4, device=device, generator=gen(98 + k, device)) for k in range(2)]
+    a.grad, b.grad = g
+    index, live, blob, _ = native.gradients([a, b, c], None)
+    assert (index, live) == (device.index, 2)
+    assert np.frombuffer(blob, np.uint64, 9).tolist() == [g[0].data_ptr(), g[1].data_ptr(), 0] + [id(p) for p in (a, b, c)] + [p.data_ptr() for p in (a, b, c)]
+    assert np.frombuffer(blob, np.int64, 3, 72).tolist() == [24] * 3 and np.frombuffer(blob, np.int32, 3, 96).tolist() == [0] * 3
+    assert native.gradients([a, b, c], b"\0\1\1")[1] == 1
+    with pytest.raises(ValueError, match="one flag"):
+        native.gradients([a], b"")
+    with pytest.raises(ValueError, match="one word"):
+        native.changed([a], b"")
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in (a, b, c)]
+    opt, ref = AdamW([a, b, c]), AdamW(twins)
+    for t in range(3):
+        for p, q, x in zip((a, b), twins, g):
+            q.grad = x.clone()
+            p.grad = (x, torch._neg_view(-x), x.t().contiguous().t())[t]
+        assert (native.gradients([a, b, c], None) is None) == (t > 0)
+        assert torch.equal(opt.step(max_norm=0.5), ref.step(max_norm=0.5))
+    assert all(torch.equal(p, q) for p, q in zip((a, b, c), twins)) and list(opt.state) == ["0.0", "0.1"]
+    # the same storage under the same parameter, in another order: refused, not read in the wrong one
+    a.grad = b.grad = None
+    a.data = a.data.view(4, 6).t()
+    a.grad = torch.ones(6, 4, device=device)
+    with pytest.raises(ValueError, match="not contiguous"):
+        opt.step()

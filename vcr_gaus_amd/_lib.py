@@ -208,6 +208,23 @@ def load():
     return lib
 
 
+_lists = None
+
+
+def tensor_list():
+    """Load (once) the native module that turns lists of torch tensors into arrays (csrc/tensor_list.cpp)."""
+    global _lists
+    if _lists is None:
+        import torch  # noqa: F401  (maps the libraries that the module needs)
+        try:
+            from . import _tensor_list
+        except ImportError as e:
+            raise ImportError(f"vcr_gaus_amd/_tensor_list.so is missing or does not load ({e}): run "
+                              "`python -c 'import __graft_entry__ as g; g.build()'`.") from e
+        _lists = _tensor_list
+    return _lists
+
+
 def check(rc):
     if rc != 0:
         raise RuntimeError("vcr_raster: " + last_error())

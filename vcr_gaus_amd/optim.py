@@ -7,21 +7,19 @@ step replays), and moments in a quarter of the memory.  The reference trains wit
 (`scene/gaussian_model.py:258`); the update is torch.optim.AdamW's.  All arithmetic runs in csrc/optim.hip; there is no fallback.
 """
 import ctypes as C
+import sys
 from array import array
-from operator import attrgetter
 
 import torch
 
 from . import _lib
+from ._lib import tensor_list as _native
 
 BLOCK = 256                                    # elements that share the scale of an 8-bit moment
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_TENSORS = {torch.Tensor, torch.nn.Parameter}
-_PTR, _CONTIGUOUS, _NUMEL, _DEVICE = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.get_device
-_GRAD, _DTYPE = attrgetter("grad"), attrgetter("dtype")
-_changed = torch.autograd.graph.increment_version        # (a backward that needs the old values says so instead of using the new ones)
-# Lists of many tensors are looked at attribute by attribute, not tensor by tensor, and go to the library as arrays of words: at 200
-# tensors the host's share of a call is what a user sees (a loop with the same checks took 94 us, the kernels 10).
+# Lists of many tensors go to the library as arrays of words.  Ordinary lists (plain dense contiguous tensors of the supported types on
+# one device) are turned into them in one native call: at 160 tensors the host's share of a call is what a user sees (a loop over the
+# tensors took 94 us, attribute by attribute 41 us, the kernels 10).  Any other list is looked at here, tensor by tensor.
 
 
 def _address(words):
@@ -37,12 +35,7 @@ def _on(dev, call, *args):
 
 
 def _check_list(tensors, what):
-    """The list, its types and its device; every tensor dense, of a supported type and on the device of the first."""
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if set(map(type, tensors)) <= _TENSORS or all(isinstance(t, torch.Tensor) for t in tensors):
-        dtypes, devices = list(map(_DTYPE, tensors)), set(map(_DEVICE, tensors))
-        if _TYPES.keys() >= set(dtypes) and len(devices) <= 1 and -1 not in devices:
-            return tensors, dtypes, tensors[0].device if tensors else None
+    """The types and the device of a list; every tensor dense, of a supported type and on the device of the first."""
     for k, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}[{k}] is a {type(t).__name__}, not a tensor")
@@ -52,29 +45,40 @@ def _check_list(tensors, what):
             raise ValueError(f"{what}[{k}] is not a dense tensor on a HIP device")
         if t.device != tensors[0].device:
             raise ValueError(f"{what}[{k}] is on {t.device}, {what}[0] on {tensors[0].device}")
+    return [t.dtype for t in tensors], tensors[0].device if tensors else None
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _dense(tensors, what):
-    """The tensors, contiguous."""
+    """The tensors, contiguous and stored as they are read."""
     try:
-        return tensors if all(map(_CONTIGUOUS, tensors)) else [t.detach().contiguous() for t in tensors]
+        return [t if t.is_contiguous() and not t.is_neg() else t.detach().resolve_neg().contiguous() for t in tensors]
     except (RuntimeError, NotImplementedError) as e:          # (layouts that have no strides)
         raise ValueError(f"{what}: dense tensors are needed: {e}") from None
 
 
 class _List:
-    """Dense tensors as the library takes them: addresses, sizes, types."""
-    __slots__ = ("n", "ptrs", "numels", "kinds")
+    """Tensors as the library takes them: how many, addresses, sizes, types (`args`), on `device`.  `work`: the tensors that were
+    listed, dense copies where the given ones are not dense; `holds`: what the addresses are of."""
+    __slots__ = ("work", "device", "args", "holds")
 
-    def __init__(self, tensors, dtypes):
-        self.n, self.ptrs, self.numels = len(tensors), array("Q", map(_PTR, tensors)), array("q", map(_NUMEL, tensors))
-        self.kinds = array("i", [_TYPES[dtypes[0]]]) * self.n if len(set(dtypes)) == 1 else array("i", [_TYPES[d] for d in dtypes])
+    def __init__(self, tensors, what, where):
+        n, found = len(tensors), _native().words(tensors)
+        if found is not None:
+            index, blob, at = found
+            self.work, self.device, self.args, self.holds = tensors, tensors[0].device, (n, at, at + 8 * n, at + 16 * n), blob
+            return
+        dtypes, self.device = _check_list(tensors, what)
+        self.work = _dense(tensors, where)
+        self.holds = (array("Q", [t.data_ptr() for t in self.work]), array("q", [t.numel() for t in self.work]),
+                      array("i", [_TYPES[d] for d in dtypes]))
+        self.args = (n, *map(_address, self.holds))
 
-    def args(self):
-        return self.n, _address(self.ptrs), _address(self.numels), _address(self.kinds)
 
-
-def _norm(args, out, again=False, grad_scale=1.0, max_norm=0.0, clip=False):
+def _norm(args, out, stream, again=False, grad_scale=1.0, max_norm=0.0, clip=False):
     """Launches the norm of the listed tensors into `out`; -> with `clip` the buffer whose first 8 bytes are the clipped step's factor.
     `again`: the tensors are read again right behind.
     The scratch belongs to this call (allocated on the current stream): two captured calls share nothing."""
@@ -82,8 +86,7 @@ def _norm(args, out, again=False, grad_scale=1.0, max_norm=0.0, clip=False):
     room = lib.vcr_grad_norm_partials(args[0], args[2])
     buffer = torch.empty(room + 1, dtype=torch.float64, device=out.device)
     at = buffer.data_ptr()
-    _lib.check(lib.vcr_grad_norm(*args, at + 8, room, grad_scale, max_norm, int(again), out.data_ptr(),
-                                 at if clip else None, _lib.stream_of(out)))
+    _lib.check(lib.vcr_grad_norm(*args, at + 8, room, grad_scale, max_norm, int(again), out.data_ptr(), at if clip else None, stream))
     return buffer
 
 
@@ -91,15 +94,16 @@ def grad_norm(tensors, out=None):
     """2-norm over all elements of all `tensors` (a list, or one tensor; float32 / bfloat16 / float16, mixed as they come) as a 0-dim
     float32 tensor on their device.  Sums in 64 bits in a fixed order: the same result on every run; NaN or infinity anywhere gives
     NaN or infinity.  No tensors: an error, as there is no device to put the result on -- unless `out` is given."""
-    tensors, dtypes, dev = _check_list(tensors, "tensors")
+    words = _List([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), "tensors", "grad_norm")
+    dev = words.device
     if out is None:
         if dev is None:
             raise ValueError("grad_norm: no tensors and no `out`")
         out = torch.empty((), device=dev)
     elif out.dtype != torch.float32 or out.numel() != 1 or not out.is_cuda or dev not in (None, out.device):
         raise ValueError("grad_norm: `out` must be one float32 element on the tensors' device")
-    words = _List(_dense(tensors, "grad_norm"), dtypes)
-    _on(out.device, _norm, words.args(), out)
+    dev = out.device
+    _on(dev, _norm, words.args, out, _stream(dev.index))
     return out
 
 
@@ -110,23 +114,26 @@ def clip_grad_norm_(parameters, max_norm):
     factor inside the update instead, without writing the gradients again."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = _positive(max_norm, "max_norm")
-    grads, dtypes, dev = _check_list([p.grad for p in parameters if p.grad is not None], "gradients")
+    grads = [p.grad for p in parameters]
+    grads = [g for g in grads if g is not None]
     if not grads:
         raise ValueError("clip_grad_norm_: no parameter has a gradient")
     if len(set(map(id, grads))) != len(grads):
         raise ValueError("clip_grad_norm_: a gradient appears twice")
-    work = _dense(grads, "clip_grad_norm_")
-    norm, words = torch.empty((), device=dev), _List(work, dtypes)
+    words = _List(grads, "gradients", "clip_grad_norm_")
+    dev = words.device
+    norm, stream = torch.empty((), device=dev), _stream(dev.index)
 
     def both():
-        _norm(words.args(), norm, True)
-        _lib.check(_lib.load().vcr_clip_gradients(*words.args(), norm.data_ptr(), max_norm, _lib.stream_of(norm)))
+        _norm(words.args, norm, stream, True)
+        _lib.check(_lib.load().vcr_clip_gradients(*words.args, norm.data_ptr(), max_norm, stream))
 
     _on(dev, both)
-    _changed(grads)
-    for g, w in zip(grads, work):
-        if g is not w:
-            g.copy_(w)
+    _native().changed(grads, None)
+    if words.work is not grads:
+        for g, w in zip(grads, words.work):
+            if g is not w:
+                g.copy_(w)
     return norm
 
 
@@ -167,7 +174,7 @@ class _Bucket:
 
 
 class _Plan:
-    __slots__ = ("params", "ids", "ptrs", "dtypes", "keys", "sizes", "numels", "buckets", "device", "streams", "captured", "covered", "keep")
+    __slots__ = ("params", "identity", "dtypes", "keys", "sizes", "numels", "buckets", "device", "streams", "captured", "covered", "keep")
 
 
 class AdamW:
@@ -305,23 +312,22 @@ class AdamW:
             if not isinstance(t, torch.Tensor) or t.dtype != dt or t.numel() != m or t.device != p.device or not t.is_contiguous():
                 raise ValueError(f"AdamW: state[{key!r}][{k!r}] must be {m} contiguous elements of {dt} on {p.device}")
 
-    def _build(self, need):
-        """Plan of all parameters that have a state, and of those in `need`, which get one."""
+    def _build(self, identity, need):
+        """Plan of all parameters that have a state, and of those in `need`, which get one.  `identity`: the native lists' words."""
         lib = _lib.load()
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the first step after its tensors changed cannot be captured; take one step before the capture")
         keys, groups_of = self._keys(), [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
         plan = _Plan()
-        plan.params, plan.dtypes, plan.device = _check_list(self._tensors(), "params")
+        plan.params = self._tensors()
+        plan.dtypes, plan.device = _check_list(plan.params, "params")
         plan.keys, plan.captured = keys, False
-        plan.sizes, plan.numels = [len(g["params"]) for g in self.param_groups], list(map(_NUMEL, plan.params))
-        plan.ids, plan.ptrs = list(map(id, plan.params)), list(map(_PTR, plan.params))
-        if len(set(plan.ids)) != len(plan.ids):
+        plan.sizes, plan.numels, plan.identity = [len(g["params"]) for g in self.param_groups], [p.numel() for p in plan.params], identity
+        if len(set(map(id, plan.params))) != len(plan.params):
             raise ValueError("AdamW: a parameter appears twice")
+        self._check_dense(plan.params)
         by = {}
         for i, (p, key) in enumerate(zip(plan.params, keys)):
-            if not p.is_contiguous():
-                raise ValueError(f"AdamW: parameter {key!r} is not contiguous")
             if key not in self.state:
                 if i not in need:
                     continue
@@ -363,27 +369,26 @@ class AdamW:
         self._plan = plan
         return plan
 
-    def _current(self, params, need=()):
-        """The plan, rebuilt where a parameter or a state entry is another tensor than it holds; `need`: indices that must be in it."""
-        plan = self._plan
-        if plan is None or list(map(id, params)) != plan.ids or list(map(_PTR, params)) != plan.ptrs \
-                or [len(g["params"]) for g in self.param_groups] != plan.sizes:
-            plan = self._build(set(need))
-        elif plan.covered < len(params):
-            known = {i for b in plan.buckets for i in b.at}
-            if any(i not in known for i in need):
-                plan = self._build(set(need))
-        stream = torch.cuda.current_stream(plan.device)
-        if stream.cuda_stream not in plan.streams:          # (what is freed later is not given away before this stream is done with it)
-            plan.streams.add(stream.cuda_stream)
+    def _current(self, params, words, flags):
+        """The plan, rebuilt where a parameter or a state entry is another tensor than it holds, or where one that is to be stepped
+        (has a gradient and a flag) is not in it."""
+        plan, identity = self._plan, words[8 * len(params):]
+        fits = plan is not None and plan.identity == identity and [len(g["params"]) for g in self.param_groups] == plan.sizes
+        if not fits or plan.covered < len(params):
+            need = {i for i, p in enumerate(params) if p.grad is not None and (flags is None or flags[i])}
+            if not fits or not need <= {i for b in plan.buckets for i in b.at}:
+                plan = self._build(identity, need)
+        stream = _stream(plan.device.index)
+        if stream not in plan.streams:          # (what is freed later is not given away before this stream is done with it)
+            plan.streams.add(stream)
             for t in plan.keep + [b.plan for b in plan.buckets]:
-                t.record_stream(stream)
+                t.record_stream(torch.cuda.current_stream(plan.device))
         if torch.cuda.is_current_stream_capturing():        # the graph holds these addresses
             plan.keep += [g["lr"] for g in self.param_groups if isinstance(g["lr"], torch.Tensor)]
             if not plan.captured:
                 plan.captured = True
                 self._captured.append(plan)
-        return plan, stream.cuda_stream
+        return plan, stream
 
     def _group_table(self, device):
         """The groups' rates as the library takes them, formed anew only where one has changed."""
@@ -405,52 +410,65 @@ class AdamW:
         measures and guards, and never clips.  Without `max_norm`: -> None."""
         if max_norm is not None:
             max_norm = _positive(max_norm, "max_norm")
-        params = self._tensors()
-        grads = list(map(_GRAD, params))
+        params, flags = self._tensors(), None
         if only is not None:
             only = {only} if isinstance(only, str) else set(only)
-            flags = [g.get("name") in only for g in self.param_groups for _ in g["params"]]
-            grads = [g if f else None for g, f in zip(grads, flags)]
-        live = [i for i, g in enumerate(grads) if g is not None]
+            flags = bytes(g.get("name") in only for g in self.param_groups for _ in g["params"])
+        found = _native().gradients(params, flags)
+        if found is None:
+            if all(p.grad is None or (flags and not f) for p, f in zip(params, flags or params)):
+                return None
+            found = self._looked_at(params, flags)
+        _, live, words, at, *_holds = found
         if not live:
             return None
-        plan, stream = self._current(params, live)
-        if len(live) == len(grads):
-            grads = _dense(grads, "AdamW: gradients")
-            fits, ptrs = list(map(_NUMEL, grads)) == plan.numels and list(map(_DTYPE, grads)) == plan.dtypes, array("Q", map(_PTR, grads))
-        else:
-            some = _dense([grads[i] for i in live], "AdamW: gradients")
-            fits = all(g.dtype is plan.dtypes[i] and g.numel() == plan.numels[i] for i, g in zip(live, some))
-            ptrs = array("Q", bytes(8 * len(grads)))
-            params = [params[i] for i in live]
-            for i, g in zip(live, some):
-                ptrs[i], grads[i] = g.data_ptr(), g              # (grads: alive until the launch)
-        if not fits:
-            i = next(i for i in live if grads[i].dtype is not plan.dtypes[i] or grads[i].numel() != plan.numels[i])
-            raise ValueError(f"AdamW: the gradient of {plan.keys[i]!r} has type {grads[i].dtype} and {grads[i].numel()} elements, "
-                             f"the parameter {plan.dtypes[i]} and {plan.numels[i]}")
-        norm = _on(plan.device, self._launch, plan, ptrs, live, max_norm, stream)
-        _changed(params)
+        plan, stream = self._current(params, words, flags)
+        norm = _on(plan.device, self._launch, plan, words, at, live, max_norm, stream)
+        _native().changed(params, words)
         if only is not None:
-            for p in params:
-                p.grad = None
+            for p, f in zip(params, flags):
+                if f:
+                    p.grad = None
         return norm
 
-    def _launch(self, plan, ptrs, live, max_norm, stream):
-        groups, lib, norm, clip = self._group_table(plan.device), _lib.load(), None, None
+    def _looked_at(self, params, flags):
+        """What `gradients` of the native lists gives, for lists that are not ordinary: dense copies of gradients, or what is wrong."""
+        dtypes, dev = _check_list(params, "params")
+        self._check_dense(params)
+        live = [i for i, p in enumerate(params) if p.grad is not None and (flags is None or flags[i])]
+        work = _dense([params[i].grad for i in live], "AdamW: gradients")
+        grads = array("Q", bytes(8 * len(params)))
+        for i, g in zip(live, work):
+            if g.dtype is not dtypes[i] or g.numel() != params[i].numel() or g.device != dev:
+                raise ValueError(f"AdamW: the gradient of {self._keys()[i]!r} has type {g.dtype} and {g.numel()} elements on {g.device}, "
+                                 f"the parameter {dtypes[i]} and {params[i].numel()} on {dev}")
+            grads[i] = g.data_ptr()
+        words = b"".join(a.tobytes() for a in (grads, array("Q", map(id, params)), array("Q", [p.data_ptr() for p in params]),
+                                               array("q", [p.numel() for p in params]), array("i", [_TYPES[d] for d in dtypes])))
+        return dev.index, len(live), words, C.cast(words, C.c_void_p).value, work
+
+    def _check_dense(self, params):
+        for key, p in zip(self._keys(), params):
+            if not p.is_contiguous() or p.is_neg():
+                raise ValueError(f"AdamW: parameter {key!r} is not contiguous")
+
+    def _launch(self, plan, words, at, live, max_norm, stream):
+        groups, lib, norm, clip, n = self._group_table(plan.device), _lib.load(), None, None, len(plan.params)
+        grads = None if live == n and len(plan.buckets) == 1 else memoryview(words)[:8 * n].cast("Q")
         if max_norm is not None:
             norm = torch.empty((), device=plan.device)
-            if len(live) == len(ptrs) and len(plan.buckets) == 1:
-                b = plan.buckets[0]
-                words = ptrs, b.numels, b.kinds
+            if live == n:
+                args = n, at, at + 24 * n, at + 32 * n
             else:
-                words = (array("Q", [ptrs[i] for i in live]), array("q", [plan.numels[i] for i in live]),
-                         array("i", [_TYPES[plan.dtypes[i]] for i in live]))
-            clip = _norm((len(words[0]), *map(_address, words)), norm, True, float(self.grad_scale), max_norm, True)
+                some = [i for i in range(n) if grads[i]]
+                lists = (array("Q", [grads[i] for i in some]), array("q", [plan.numels[i] for i in some]),
+                         array("i", [_TYPES[plan.dtypes[i]] for i in some]))
+                args = len(some), *map(_address, lists)
+            clip = _norm(args, norm, stream, True, float(self.grad_scale), max_norm, True)
         for b in plan.buckets:
-            mine = ptrs if b.every else array("Q", [ptrs[i] for i in b.at])
+            mine = None if b.every else array("Q", [grads[i] for i in b.at])
             a = b.args
-            a.grads, a.groups, a.ngroups, a.grad_scale = _address(mine), groups, len(groups), float(self.grad_scale)
+            a.grads, a.groups, a.ngroups, a.grad_scale = at if b.every else _address(mine), groups, len(groups), float(self.grad_scale)
             a.clip = None if clip is None else clip.data_ptr()
             _lib.check(lib.vcr_adamw_step(C.byref(a), stream))
         return norm
@@ -476,13 +494,16 @@ class AdamW:
             elif len(given) != len(params):
                 raise ValueError(f"moments: {len(given)} tensors for {len(params)} parameters")
             outs.append(given)
-        kinds = set(map(_DTYPE, outs[0])) | set(map(_DTYPE, outs[1]))
-        if len(kinds) != 1 or not kinds <= _TYPES.keys():
-            raise ValueError(f"moments: the outputs must be of one type among float32, bfloat16, float16: {kinds}")
-        plan, stream = self._current(params)
-        for o in outs:
-            if list(map(_NUMEL, o)) != plan.numels or set(map(_DEVICE, o)) != {plan.device.index} or not all(map(_CONTIGUOUS, o)):
-                raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
+        n, none = len(params), bytes(len(params))
+        found = [_native().words(list(o)) for o in outs]          # device, words, their address
+        kind = None if None in found else found[0][1][16 * n:16 * n + 4]
+        if kind is None or any(f[1][16 * n:] != kind * n for f in found):
+            kinds = {t.dtype for o in outs for t in o}
+            if len(kinds) != 1 or not kinds <= _TYPES.keys():
+                raise ValueError(f"moments: the outputs must be of one type among float32, bfloat16, float16: {kinds}")
+        plan, stream = self._current(params, (_native().gradients(params, none) or self._looked_at(params, none))[2], none)
+        if any(f is None or f[0] != plan.device.index or f[1][8 * n:16 * n] != plan.identity[16 * n:24 * n] for f in found):
+            raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
         if plan.covered < len(params):
             held = {i for b in plan.buckets for i in b.at}
             for i in range(len(params)):
@@ -495,11 +516,11 @@ class AdamW:
                     for o, k in zip(outs, ("exp_avg", "exp_avg_sq")):
                         o[i].detach().copy_(self.state[plan.keys[i]][k].view(o[i].shape))
         else:
-            kind = _TYPES[kinds.pop()]
+            kind = int.from_bytes(kind, sys.byteorder)
             for b in plan.buckets:
-                m, v = (array("Q", map(_PTR, o if b.every else [o[i] for i in b.at])) for o in outs)
-                _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), _address(b.numels), _address(m),
-                               _address(v), kind, stream))
+                some = None if b.every else [array("Q", [o[i].data_ptr() for i in b.at]) for o in outs]
+                m, v = (f[2] for f in found) if b.every else map(_address, some)
+                _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), _address(b.numels), m, v, kind, stream))
         return outs
 
     @torch.no_grad()
