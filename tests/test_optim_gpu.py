@@ -959,3 +959,36 @@ def test_parameters_are_the_same_however_they_are_looked_at(device):
     a.grad = torch.ones(6, 4, device=device)
     with pytest.raises(ValueError, match="not contiguous"):
         opt.step()
+
+
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+def test_grad_norm_of_few_elements(device, dtype):
+    """Sizes around those that one workgroup sums alone (4 pieces of 16384), alone and after other types; eager, captured, in a step."""
+    from vcr_gaus_amd.optim import AdamW, grad_norm
+    g = gen(99, device)
+    for sizes in ((1,), (7, 1), (16384,), (16385, 5), (65536,), (65535, 0), (65537,), (20000, 20000), (20000, 20000, 3), (16384,) * 4, (3,) * 4, (3,) * 5):
+        x = [torch.randn(n + 1, device=device, generator=g).to(dtype)[1:] for n in sizes]
+        want = math.sqrt(sum(float(t.double().square().sum()) for t in x))
+        off = 2.0 ** -24 * want * (1 + 1e-6)
+        assert abs(float(grad_norm(x)) - want) <= off, sizes
+        more = x + [torch.full((2,), 0.5, device=device, dtype=F if dtype != F else BF)]
+        assert abs(float(grad_norm(more)) - math.sqrt(want * want + 0.5)) <= 2.0 ** -24 * (want + 1) * (1 + 1e-6), sizes
+        out = torch.empty((), device=device)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            grad_norm(x, out=out)
+        for r in range(3):
+            x[0].mul_(-2.0)
+            graph.replay()
+            assert torch.equal(out, grad_norm(x)), (sizes, r)
+        params = [torch.nn.Parameter(torch.ones_like(t)) for t in x]
+        for p, t in zip(params, x):
+            p.grad = t
+        opt = AdamW(params)
+        opt.grad_scale = 0.5
+        norm = opt.step(max_norm=1e-3)
+        assert abs(float(norm) - 0.5 * float(grad_norm(x))) <= 2.0 ** -23 * float(norm)
+        m = torch.cat([t.flatten() for t in opt.moments()[0]])
+        clipped = torch.cat([t.float() for t in x]) * (0.5 * min(1.0, 1e-3 / (float(norm) + 1e-6)))
+        assert bool(((m - 0.1 * clipped).abs() <= 2.0 ** -21 * clipped.abs() + 2.0 ** -148).all()), sizes

@@ -37,6 +37,9 @@ namespace {
 // The norm's workgroups stride over chunks (800 M fp32 elements: 459 us with 1024 workgroups, 469 with 2048, 468 with 4096).
 #define VCR_OPT_NORM_BLOCKS 1024
 #define NORM_CHUNK 16384
+// Up to this many chunks in all, of one type: one workgroup and one launch (64 K fp32 elements, 4 chunks: 8.9 instead of 11.8 us from
+// Python, 4.8 us either way in a captured graph; 8 chunks 8.9 instead of 12.0, but 8.5 instead of 4.9 captured).
+#define VCR_OPT_NORM_ONE 4
 
 struct Group { double lr, wd, log_b1, log_b2; const float* lr_dev; float eps, b1, omb1, b2, omb2; int pad; };
 struct StepPack { const void* g[VCR_OPT_TENSORS]; Group group[VCR_OPT_GROUPS]; };
@@ -188,11 +191,26 @@ __device__ __forceinline__ int scale_of(uint32_t bits) { const int s = (int)(bit
 // ---- norm -------------------------------------------------------------------------------------------------------
 // The sum of squares runs in fp64: neither an fp32 gradient near 1e38 nor 1e9 small ones leave its range, and one partial per
 // workgroup, summed in a fixed order, makes the result the same from run to run (no atomics).
-__device__ __forceinline__ double block_sum(double x, double* lds) {
+template <int THREADS> __device__ __forceinline__ double block_sum(double x) {
+    __shared__ double lds[THREADS / 64];
     for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
     __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+    x = lds[0];
+    for (int k = 1; k < THREADS / 64; ++k) x += lds[k];
+    return x;
+}
+
+// norm = sqrt(sum) |scale|; with `clip`: the factor of a clipped step, and skip where the norm is not finite in fp32
+struct Finish { double scale, max_norm; float* out; Clip* clip; };
+__device__ __forceinline__ void finish(double sum, const Finish& f) {
+    const float norm = (float)(sqrt(sum) * fabs(f.scale));
+    if (f.out) *f.out = norm;
+    if (f.clip) {
+        const double q = f.max_norm / ((double)norm + 1e-6);
+        f.clip->gscale = q < 1.0 ? (float)(f.scale * q) : (float)f.scale;
+        f.clip->skip = (__float_as_uint(norm) & 0x7FFFFFFFu) >= INF_BITS;
+    }
 }
 
 struct Piece { int tensor; long long off; uint32_t cnt; };
@@ -207,10 +225,12 @@ __device__ __forceinline__ Piece piece_of(const NormPack& pk, int n, uint32_t ch
 }
 // NT: gradients that nothing reads soon again pass the caches (800 M fp32 elements 520 -> 459 us, 7.0 TB/s; 302 M bf16 106 -> 95 us);
 // those of a clipped step stay in them for the update behind (75 M fp32 elements, norm and update together: 379 against 420 us).
-template <typename T, bool NT>
-__global__ void __launch_bounds__(256) norm_kernel(NormPack pk, int n, uint32_t chunk, double* __restrict__ partials) {
-    __shared__ double lds[4];
-    constexpr int V = 16 / sizeof(T);
+// ONE: few elements in all, one large workgroup that writes the norm itself: one launch instead of two.
+template <typename T, bool NT, bool ONE> constexpr int norm_threads() { return ONE ? 1024 : 256; }
+template <typename T, bool NT, bool ONE>
+__global__ void __launch_bounds__((norm_threads<T, NT, ONE>())) norm_kernel(NormPack pk, int n, uint32_t chunk, double* __restrict__ partials,
+                                                                          Finish f) {
+    constexpr int V = 16 / sizeof(T), THREADS = norm_threads<T, NT, ONE>();
     double sum[V] = {};
     for (uint32_t c = blockIdx.x; c < pk.start[n]; c += gridDim.x) {
         const Piece q = piece_of(pk, n, chunk, c);
@@ -218,7 +238,7 @@ __global__ void __launch_bounds__(256) norm_kernel(NormPack pk, int n, uint32_t 
         const uint32_t vecs = q.cnt / V, tail = vecs * V;
         if (threadIdx.x < q.cnt - tail) { const double x = (double)load1(g + tail + threadIdx.x); sum[0] += x * x; }
 #pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < vecs; i += 256) {
+        for (uint32_t i = threadIdx.x; i < vecs; i += THREADS) {
             const Vec<V> x = loadv<V, NT>(g + (size_t)i * V);
 #pragma unroll
             for (int k = 0; k < V; ++k) { const double y = (double)x.x[k]; sum[k] += y * y; }
@@ -226,28 +246,17 @@ __global__ void __launch_bounds__(256) norm_kernel(NormPack pk, int n, uint32_t 
     }
 #pragma unroll
     for (int k = 1; k < V; ++k) sum[0] += sum[k];
-    const double total = block_sum(sum[0], lds);
-    if (threadIdx.x == 0) partials[blockIdx.x] = total;
+    const double total = block_sum<THREADS>(sum[0]);
+    if (threadIdx.x != 0) return;
+    if constexpr (ONE) finish(total, f);
+    else partials[blockIdx.x] = total;
 }
 
-__device__ __forceinline__ double sum_partials(const double* __restrict__ partials, int n, double* lds) {
+__global__ void __launch_bounds__(256) finish_kernel(const double* __restrict__ partials, int n, Finish f) {
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) s += partials[i];
-    return block_sum(s, lds);
-}
-
-// norm = sqrt(sum) |scale|; with `clip`: the factor of a clipped step, and skip where the norm is not finite in fp32
-__global__ void __launch_bounds__(256) finish_kernel(const double* __restrict__ partials, int n, double scale, double max_norm,
-                                                     float* __restrict__ out, Clip* __restrict__ clip) {
-    __shared__ double lds[4];
-    const float norm = (float)(sqrt(sum_partials(partials, n, lds)) * fabs(scale));
-    if (threadIdx.x != 0) return;
-    if (out) *out = norm;
-    if (clip) {
-        const double q = max_norm / ((double)norm + 1e-6);
-        clip->gscale = q < 1.0 ? (float)(scale * q) : (float)scale;
-        clip->skip = (__float_as_uint(norm) & 0x7FFFFFFFu) >= INF_BITS;
-    }
+    s = block_sum<256>(s);
+    if (threadIdx.x == 0) finish(s, f);
 }
 
 // g *= min(1, max_norm / (norm + 1e-6)); a norm that is not finite leaves NaN or zero as the formula says
@@ -934,25 +943,30 @@ extern "C" int vcr_grad_norm(int ntensors, const void* const* tensors, const int
     if (!partials || (!norm && !clip)) { vcr_set_error("vcr_grad_norm: partials or norm is NULL"); return 1; }
     if (clip && !(max_norm > 0.0)) { vcr_set_error("vcr_grad_norm: max_norm is %g", max_norm); return 1; }
     hipStream_t st = (hipStream_t)stream;
-    int used_partials = 0;
+    const Finish f{grad_scale, max_norm, norm, (Clip*)clip};
+    int used_partials = 0, types_seen = 0;
+    int64_t all = 0, listed = 0;
+    for (int k = 0; k < ntensors; ++k)
+        if (numel[k] > 0) { types_seen |= 1 << types[k]; all += chunks_of(numel[k], NORM_CHUNK); ++listed; }
+    const bool one = all <= VCR_OPT_NORM_ONE && listed <= VCR_OPT_NORM_TENSORS && (types_seen & (types_seen - 1)) == 0 && all > 0;
     for (int type = VCR_F32; type <= VCR_F16; ++type) {
         const int rc = each_norm_pack(ntensors, tensors, numel, types, type, [&](const NormPack& pk, int used, uint32_t chunks) {
-            const int blocks = chunks < VCR_OPT_NORM_BLOCKS ? (int)chunks : VCR_OPT_NORM_BLOCKS;
+            const int blocks = one ? 1 : chunks < VCR_OPT_NORM_BLOCKS ? (int)chunks : VCR_OPT_NORM_BLOCKS;
             if (used_partials + blocks > capacity) { vcr_set_error("vcr_grad_norm: room for %d partial sums is too little", capacity); return 1; }
-            const dim3 grid(blocks), block(256);
             double* out = partials + used_partials;
-#define LAUNCH(T) do { if (read_again) hipLaunchKernelGGL((norm_kernel<T, false>), grid, block, 0, st, pk, used, NORM_CHUNK, out); \
-                       else hipLaunchKernelGGL((norm_kernel<T, true>), grid, block, 0, st, pk, used, NORM_CHUNK, out); } while (0)
-            if (type == VCR_F32) LAUNCH(float);
-            else if (type == VCR_BF16) LAUNCH(__hip_bfloat16);
-            else LAUNCH(__half);
+#define LAUNCH(T, NT, ONE) hipLaunchKernelGGL((norm_kernel<T, NT, ONE>), dim3(blocks), dim3(norm_threads<T, NT, ONE>()), 0, st, pk, used, NORM_CHUNK, out, f)
+#define LAUNCH_ANY(T) do { if (one) LAUNCH(T, false, true); else if (read_again) LAUNCH(T, false, false); else LAUNCH(T, true, false); } while (0)
+            if (type == VCR_F32) LAUNCH_ANY(float);
+            else if (type == VCR_BF16) LAUNCH_ANY(__hip_bfloat16);
+            else LAUNCH_ANY(__half);
+#undef LAUNCH_ANY
 #undef LAUNCH
             used_partials += blocks;
             return 0;
         });
         if (rc) return 1;
     }
-    hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, st, partials, used_partials, grad_scale, max_norm, norm, (Clip*)clip);
+    if (!one) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, st, partials, used_partials, f);
     VCR_HIP_CHECK(hipGetLastError());
     return 0;
 }
