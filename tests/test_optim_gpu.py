@@ -992,3 +992,25 @@ def test_grad_norm_of_few_elements(device, dtype):
         m = torch.cat([t.flatten() for t in opt.moments()[0]])
         clipped = torch.cat([t.float() for t in x]) * (0.5 * min(1.0, 1e-3 / (float(norm) + 1e-6)))
         assert bool(((m - 0.1 * clipped).abs() <= 2.0 ** -21 * clipped.abs() + 2.0 ** -148).all()), sizes
+
+
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_moments_into_given_tensors(device, dtype, shift):
+    """Values of the codes at sizes around what a lane, a block and a workgroup hold, into tensors off their alignment: the codes'
+    values rounded to the type, and nothing beside them."""
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([1, 2, 3, 4, 5, 7, 8, 9, 255, 257, 2047, 2049, 4095, 4097, 12291], F, device, seed=96, grad=1.0)
+    opt = AdamW(params, state_bits=8)
+    opt.step()
+    bufs = [[torch.full((p.numel() + 32,), 7.0, dtype=dtype, device=device) for p in params] for _ in range(2)]
+    outs = [[b[8 + shift:8 + shift + p.numel()] for b, p in zip(bs, params)] for bs in bufs]
+    got = opt.moments(*outs)
+    for i, p in enumerate(params):
+        n, st = p.numel(), opt.state[f"0.{i}"]
+        for signed, k, b in ((True, "exp_avg", bufs[0][i]), (False, "exp_avg_sq", bufs[1][i])):
+            want = R.decode(st[k].cpu().numpy().reshape(-1), st[k + "_scale"].cpu().numpy(), signed)
+            a = 8 + shift
+            assert torch.equal(b[a:a + n].cpu(), torch.from_numpy(np.asarray(want, np.float64)).to(dtype)), (n, k)
+            assert bool((b[:a] == 7).all()) and bool((b[a + n:] == 7).all()), (n, k)
+    assert got[0] is outs[0]
