@@ -1014,3 +1014,19 @@ def test_moments_into_given_tensors(device, dtype, shift):
             assert torch.equal(b[a:a + n].cpu(), torch.from_numpy(np.asarray(want, np.float64)).to(dtype)), (n, k)
             assert bool((b[:a] == 7).all()) and bool((b[a + n:] == 7).all()), (n, k)
     assert got[0] is outs[0]
+
+
+def test_a_gradient_without_memory_is_refused(device):
+    from vcr_gaus_amd.optim import AdamW, grad_norm
+    params, _ = make([64, 8], F, device, seed=100)
+    opt = AdamW(params)
+    opt.step()
+    before = [p.detach().clone() for p in params]
+    freed = torch.ones(64, device=device)
+    freed.untyped_storage().resize_(0)
+    params[0].grad = freed
+    with pytest.raises(ValueError, match="no memory"):
+        opt.step()
+    with pytest.raises(RuntimeError, match="pointer"):
+        grad_norm([freed, params[1]])
+    assert all(torch.equal(p, q) for p, q in zip(params, before)) and int(opt.state["0.1"]["step"]) == 1

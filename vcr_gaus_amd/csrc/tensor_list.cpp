@@ -4,6 +4,7 @@
 // tensors) is not judged here: the answer is None, and the caller looks at the tensors one by one and says what is wrong.
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 #include <ATen/core/Tensor.h>
 
 namespace {
@@ -35,22 +36,22 @@ PyObject* words(PyObject*, PyObject* list) {
     return guarded([&]() -> PyObject* {
         if (!PyList_CheckExact(list) || PyList_GET_SIZE(list) == 0) Py_RETURN_NONE;
         const Py_ssize_t n = PyList_GET_SIZE(list);
-        PyObject* blob = PyBytes_FromStringAndSize(nullptr, n * 20);
+        THPObjectPtr blob(PyBytes_FromStringAndSize(nullptr, n * 20));
         if (!blob) return nullptr;
-        uint64_t* at_ = (uint64_t*)PyBytes_AS_STRING(blob);
+        uint64_t* at_ = (uint64_t*)PyBytes_AS_STRING(blob.get());
         int64_t* numel = (int64_t*)(at_ + n);
         int32_t* kind = (int32_t*)(numel + n);
         int device = -1;
         for (Py_ssize_t i = 0; i < n; ++i) {
             const at::Tensor* t = plain(PyList_GET_ITEM(list, i));
             const int k = t ? kind_of(*t) : -1;
-            if (k < 0 || (i > 0 && t->device().index() != device)) { Py_DECREF(blob); Py_RETURN_NONE; }
+            if (k < 0 || (i > 0 && t->device().index() != device)) Py_RETURN_NONE;
             device = t->device().index();
             at_[i] = (uint64_t)(uintptr_t)t->const_data_ptr();
             numel[i] = t->numel();
             kind[i] = k;
         }
-        return Py_BuildValue("iNK", device, blob, (unsigned long long)(uintptr_t)at_);
+        return Py_BuildValue("iNK", device, blob.release(), (unsigned long long)(uintptr_t)at_);
     });
 }
 
@@ -68,9 +69,9 @@ PyObject* gradients(PyObject*, PyObject* args) {
             if (!PyBytes_Check(flags) || PyBytes_GET_SIZE(flags) != n) { PyErr_SetString(PyExc_ValueError, "gradients: one flag for each tensor"); return nullptr; }
             wanted = PyBytes_AS_STRING(flags);
         }
-        PyObject* blob = PyBytes_FromStringAndSize(nullptr, n * 36);
+        THPObjectPtr blob(PyBytes_FromStringAndSize(nullptr, n * 36));
         if (!blob) return nullptr;
-        uint64_t* grad = (uint64_t*)PyBytes_AS_STRING(blob);
+        uint64_t* grad = (uint64_t*)PyBytes_AS_STRING(blob.get());
         uint64_t *object = grad + n, *at_ = object + n;
         int64_t* numel = (int64_t*)(at_ + n);
         int32_t* kind = (int32_t*)(numel + n);
@@ -91,11 +92,12 @@ PyObject* gradients(PyObject*, PyObject* args) {
                 if (g.defined() && (!wanted || wanted[i])) {
                     good = kind_of(g) == k && g.numel() == numel[i] && g.device().index() == device;
                     if (good) { grad[i] = (uint64_t)(uintptr_t)g.const_data_ptr(); ++live; }
+                    good = good && (grad[i] || numel[i] == 0);
                 }
             }
-            if (!good) { Py_DECREF(blob); Py_RETURN_NONE; }
+            if (!good) Py_RETURN_NONE;
         }
-        return Py_BuildValue("iiNK", device, live, blob, (unsigned long long)(uintptr_t)grad);
+        return Py_BuildValue("iiNK", device, live, blob.release(), (unsigned long long)(uintptr_t)grad);
     });
 }
 
