@@ -1030,3 +1030,20 @@ def test_a_gradient_without_memory_is_refused(device):
     with pytest.raises(RuntimeError, match="pointer"):
         grad_norm([freed, params[1]])
     assert all(torch.equal(p, q) for p, q in zip(params, before)) and int(opt.state["0.1"]["step"]) == 1
+
+
+def test_codes_are_not_loaded_as_values(device):
+    """A checkpoint with 8-bit moments is refused by the Adam that holds values, before anything of it is taken."""
+    from vcr_gaus_amd.gaussian_model import GaussianModel
+    tr = adamw_trainer(device, state_bits=8)
+    tr.train_step()
+    cap = tr.model.capture()
+    args = type(tr.cfg.optim)(tr.cfg.optim)
+    args.update(optimizer="adam", state_bits=32)
+    with pytest.raises(ValueError, match="8-bit codes"):
+        GaussianModel(tr.cfg.model).restore(cap, args)
+    args.update(optimizer="adamw", state_bits=32)                      # (the same optimizer in 32 bits expands them)
+    m = GaussianModel(tr.cfg.model)
+    m.restore(cap, args)
+    for k in GROUPS:
+        assert torch.equal(m.optimizer.state[k]["exp_avg"], tr.model.optimizer.moments_of(k)[0])

@@ -468,7 +468,7 @@ __device__ __forceinline__ Fast fast_of(const Coef& c) {
 // bias 7, code exponent 14 = 2^7), and everything shifted up by 4 so that a code is the top byte of its word.  Returns false, with
 // nothing changed, where it does not apply: a code or a moment that is not finite, block exponents out of the ranges above, or a
 // second moment below 2^-126 (the square root instruction would flush it).  Its 150 vector instructions, of 190 a block in all, are what
-// bounds the update of 16-bit parameters: in 92 % of the cycles one is at work.
+// bounds the update of 16-bit parameters: in 90 % of the cycles one is at work.
 __device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], float gs, const Coef& c,
                                            const Fast& f) {
 #pragma clang fp contract(off)

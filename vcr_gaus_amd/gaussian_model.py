@@ -399,6 +399,8 @@ class FusedAdam:
     def load_state_dict(self, sd):
         """Accepts what the reference's `torch.optim.Adam.state_dict()` holds (and, for older files of this repo, the
         name-keyed form).  Groups are matched by name; moments land on the device of the parameter they belong to."""
+        if any(not v["exp_avg"].dtype.is_floating_point for v in sd["state"].values() if "exp_avg" in v):
+            raise ValueError("optimizer state holds 8-bit codes of GaussianAdamW: load it with optim.optimizer = \"adamw\"")
         by_wire = {}
         for g in self.param_groups:
             by_wire.setdefault(self._wire_name(g["name"]), []).append(g)
