@@ -1,0 +1,42 @@
+"""`vcr_gaus_amd.optim` where a call is allowed but rare: values at the bottom of the number range, tensors that share or change their memory,
+other streams, lists with empty tensors.  Definitions and bounds as in tests/test_optim_gpu.py."""
+import numpy as np
+import pytest
+import torch
+
+from tests import optim_reference as R
+from tests.test_optim_gpu import blank8, host, same8, state8
+
+pytestmark = pytest.mark.gpu
+BF, HF, F = torch.bfloat16, torch.float16, torch.float32
+
+
+def quiet_lanes(n, seed, late):
+    """Gradients of three steps: ordinary ones; every fifth element has none in the first two, and `late` in the third."""
+    g = torch.Generator().manual_seed(seed)
+    steps = [torch.randn(n, generator=g) for _ in range(3)]
+    quiet = torch.arange(n) % 5 == 0
+    for t in range(2):
+        steps[t][quiet] = 0.0
+    steps[2][quiet] = late(int(quiet.sum()))
+    return steps, quiet
+
+
+@pytest.mark.parametrize("dtype", [F, BF])
+@pytest.mark.parametrize("eps", [1e-8, 1e-4, 1e-15])
+def test_second_moments_below_the_lowest_code(device, dtype, eps):
+    """Elements of ordinary blocks whose first gradients (1e-23 ... 1e-15) come late, so that v' goes from 0 to below 2^-129: code 1 at
+    least wherever v' > 0, as defined, in whole blocks and in the partial one at the end alike."""
+    from vcr_gaus_amd.optim import AdamW
+    n = 8 * 256 + 100
+    steps, quiet = quiet_lanes(n, 3, lambda k: torch.logspace(-23.5, -15, k) * (torch.arange(k) % 2 * 2 - 1))
+    p = torch.nn.Parameter(torch.ones(n, dtype=dtype, device=device))
+    opt, st = AdamW([p], lr=1e-3, eps=eps, state_bits=8, seed=9), blank8(n)
+    for t, x in enumerate(steps + steps[2:]):
+        p.grad = x.to(device).to(dtype)
+        _, _, v = R.step8(np.ones(n), host(p.grad), st, lr=1e-3, b1=0.9, b2=0.999, eps=eps, wd=0.01, seed=9)
+        opt.step()
+        got = state8(opt, "0")
+        assert same8(got, st) == [], t
+        assert np.all((got["vc"] > 0) == (v > 0))
+        assert t != 2 or int(((v > 0) & (v < 2.0 ** -129)).sum()) > 20

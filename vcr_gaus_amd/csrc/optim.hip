@@ -466,8 +466,8 @@ __device__ __forceinline__ Fast fast_of(const Coef& c) {
 // A whole block of finite numbers of ordinary size: the definition above with its scalings as multiplications by powers of two
 // (exact, so that b2 and the scale of v are one factor), the first moment's codes decoded by the hardware (they are OCP e4m3:
 // bias 7, code exponent 14 = 2^7), and everything shifted up by 4 so that a code is the top byte of its word.  Returns false, with
-// nothing changed, where it does not apply: a code or a moment that is not finite, block exponents out of the ranges above, or a
-// second moment below 2^-126 (the square root instruction would flush it).  Its 150 vector instructions, of 190 a block in all, are what
+// nothing changed, where it does not apply: a code or a moment that is not finite, block exponents out of the ranges above, or, where
+// eps is small enough for it to be seen (`guard`), a second moment below 2^-126, which the square root instruction would flush.  Its 150 vector instructions, of 190 a block in all, are what
 // bounds the update of 16-bit parameters: in 90 % of the cycles one is at work.
 __device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], float gs, const Coef& c,
                                            const Fast& f) {
@@ -512,8 +512,9 @@ __device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t 
         // 16 r_m and 16 r_v: the word's upper and lower half at bits 8 ... 23, 0x80 below
         const uint32_t w = element_word(bkey, j_step[k]);
         zm[k] = (__float_as_uint(fabsf(m[k]) * m_up) << 4) + __builtin_amdgcn_perm(w, 0x80u, 0x0C070600u);
-        // at least code 1 where v' > 0: the middle one of the scaled value, the value (larger, as its exponent is above 30) and code 1
-        const float y = __builtin_amdgcn_fmed3f(v[k] * v_up, v[k], __uint_as_float(1u << 20));
+        // at least code 1 (2^-129) where v' > 0: the middle one of the scaled value, of 2^20 v' -- larger than either, as v_up is
+        // 2^-10 at most and the smallest v' is 2^-149; 0 where v' is 0 -- and of code 1
+        const float y = __builtin_amdgcn_fmed3f(v[k] * v_up, v[k] * 0x1p+20f, __uint_as_float(1u << 20));
         zv[k] = (__float_as_uint(y) << 4) + __builtin_amdgcn_perm(w, 0x80u, 0x0C050400u);
     }
     const uint32_t sign = top_bytes(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])) & 0x80808080u;
