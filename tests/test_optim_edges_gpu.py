@@ -40,3 +40,27 @@ def test_second_moments_below_the_lowest_code(device, dtype, eps):
         assert same8(got, st) == [], t
         assert np.all((got["vc"] > 0) == (v > 0))
         assert t != 2 or int(((v > 0) & (v < 2.0 ** -129)).sum()) > 20
+
+
+@pytest.mark.parametrize("lr, eps", [(8.0, 1.25 * 2.0 ** -126), (8.0, 2.0 ** -120), (1e18, 1e-12), (1e3, 0.0)])
+def test_small_eps_under_a_large_rate(device, lr, eps):
+    """eps / step size below the normal numbers (first case) or just above: elements with m = v = 0 stay where eps > 0 (0 / 0 where it is
+    not, by the formula), the others follow the formula."""
+    from vcr_gaus_amd.optim import AdamW
+    n = 1024
+    steps, quiet = quiet_lanes(n, 4, lambda k: torch.zeros(k))
+    quiet = quiet.numpy()
+    p = torch.nn.Parameter(torch.ones(n, device=device))
+    opt, st, x = AdamW([p], lr=lr, eps=eps, weight_decay=0.0, state_bits=8), blank8(n), np.ones(n)
+    for g in steps:
+        p.grad = g.to(device)
+        x, _, _ = R.step8(x, host(p.grad), st, lr=lr, b1=0.9, b2=0.999, eps=eps, wd=0.0)
+        opt.step()
+        assert same8(state8(opt, "0"), st) == []
+        got = host(p)
+        if eps:
+            assert np.array_equal(got[quiet], np.ones(quiet.sum()))
+        else:
+            assert np.isnan(got[quiet]).all() and np.isnan(x[quiet]).all()
+        # three steps: two roundings of p each, and 2^-20 of an update of at most 4 lr
+        assert np.abs(got - x)[~quiet].max() <= 3 * (2.0 ** -23 * np.abs(x[~quiet]).max() + 2.0 ** -20 * lr * 4)

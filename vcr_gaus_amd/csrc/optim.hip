@@ -47,7 +47,7 @@ struct PairPack { const void* a[VCR_OPT_PAIRS]; const void* b[VCR_OPT_PAIRS]; };
 struct NormPack { const void* g[VCR_OPT_NORM_TENSORS]; long long n[VCR_OPT_NORM_TENSORS]; uint32_t start[VCR_OPT_NORM_TENSORS + 1]; };
 static_assert(sizeof(StepPack) <= 4000 && sizeof(NormPack) <= 4000 && sizeof(PairPack) <= 4000, "kernel arguments are 4 KB at most");
 
-struct Coef { float decay, step_size, inv_sqrt_bc2, eps, b1, omb1, b2, omb2; };
+struct Coef { float decay, step_size, inv_sqrt_bc2, eps, b1, omb1, b2, omb2; int plain; };
 struct Clip { float gscale; int skip; };       // of a clipped step, written by the finish kernel
 
 // Pointers read from memory are generic to the compiler (flat_* accesses, which wait on two counters); these are global.
@@ -308,6 +308,12 @@ __device__ __forceinline__ Coef coef_of(const Group& G, int t) {
     c.inv_sqrt_bc2 = from_lane(f, 1);
     c.decay = (float)(1.0 - lr * G.wd);
     c.eps = G.eps; c.b1 = G.b1; c.omb1 = G.omb1; c.b2 = G.b2; c.omb2 = G.omb2;
+    // Whether the 8-bit fast path, which divides by the step size, applies: not with a step size of zero, nor where its denominator
+    // could leave the normal numbers, whose reciprocal is infinite (m' = 0 would become NaN).  eps / step size is 0 or normal by the
+    // test (which has room for the reciprocal's rounding); with eps = 0 the root of a v' of 2^-126 or more (`Fast::guard`), times a
+    // factor of 1 or more, over a step size below 2^60 is above 2^-123.  (Formed here once, not in every wave, where it delays the
+    // loads: 295 M fp32 elements and their values 1 036 instead of 1 156 us.)
+    c.plain = c.step_size > 1e-20f && c.step_size < 0x1p+60f && (c.eps == 0.f || c.eps >= 0x1.01p-126f * c.step_size);
     return c;
 }
 
@@ -452,15 +458,13 @@ template <int K> __device__ __forceinline__ float code_bits(uint32_t x, uint32_t
 #define V_HIGH 155
 
 // The factors once more, as the fast path takes them: p' = p decay - m' / (sqrt(v') root + eps), both divided by the step size.
-// `plain`: whether it applies at all (a step size of zero does not).  `guard`: whether eps is so small that a root flushed to
-// zero (v' below 2^-126: the root below 1e-19, 3e-18 with the largest factor that b2 = 0.999 gives) could be seen.
-struct Fast { float root, eps; bool plain, guard; };
+// `guard`: whether eps is so small that a root flushed to zero (v' below 2^-126: the root below 1e-19, 3e-18 with the largest factor
+// that b2 = 0.999 gives) could be seen.
+struct Fast { float root, eps; bool guard; };
 __device__ __forceinline__ Fast fast_of(const Coef& c) {
     const float r = __builtin_amdgcn_rcpf(c.step_size);
-    const int ss = __builtin_amdgcn_readfirstlane(__float_as_int(c.step_size)), eps = __builtin_amdgcn_readfirstlane(__float_as_int(c.eps));
-    const int isq = __builtin_amdgcn_readfirstlane(__float_as_int(c.inv_sqrt_bc2));
-    return {c.inv_sqrt_bc2 * r, c.eps * r, __int_as_float(ss) > 1e-20f && __int_as_float(ss) < 1e20f,
-            !(__int_as_float(eps) >= 1e-10f && __int_as_float(isq) < 40.f)};
+    const int eps = __builtin_amdgcn_readfirstlane(__float_as_int(c.eps)), isq = __builtin_amdgcn_readfirstlane(__float_as_int(c.inv_sqrt_bc2));
+    return {c.inv_sqrt_bc2 * r, c.eps * r, !(__int_as_float(eps) >= 1e-10f && __int_as_float(isq) < 40.f)};
 }
 
 // A whole block of finite numbers of ordinary size: the definition above with its scalings as multiplications by powers of two
@@ -472,7 +476,7 @@ __device__ __forceinline__ Fast fast_of(const Coef& c) {
 __device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], float gs, const Coef& c,
                                            const Fast& f) {
 #pragma clang fp contract(off)
-    if (!f.plain || sm < M_LOW || sm > M_HIGH || sv < V_LOW || sv > V_HIGH) return false;
+    if (!__builtin_amdgcn_readfirstlane(c.plain) || sm < M_LOW || sm > M_HIGH || sv < V_LOW || sv > V_HIGH) return false;
     // a byte 0x7F / 0xFF among the first moment's codes, a byte 0xFF among the second's
     uint32_t odd = ((r.cm & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
     odd |= ((r.cv & 0x7F7F7F7Fu) + 0x01010101u) & r.cv & 0x80808080u;
