@@ -291,7 +291,10 @@ typedef struct VcrAdamWStep {
 } VcrAdamWStep;
 size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel);
 int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, void* host_plan, size_t bytes);
-/* One AdamW step (decoupled weight decay, torch.optim.AdamW's arithmetic) on every tensor with a gradient; see csrc/optim.hip. */
+/* One AdamW step (decoupled weight decay, torch.optim.AdamW's arithmetic) on every tensor with a gradient; see csrc/optim.hip.
+ * `numel`, `group_of`, `param_type` must be what the plan was made for: the plan lies on the device, where the host cannot compare
+ * them.  A record of the other `state_bits`, or without the master that `masters` asks for, is left alone, and so is its counter;
+ * that is no error. */
 int vcr_adamw_step(const VcrAdamWStep* args, void* stream);
 /* Values of the 8-bit moments (a NULL pointer leaves that output out), and 8-bit moments from fp32 values (to the nearest). */
 int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, void* const* exp_avg,

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import optim_reference as R
-from tests.test_optim_gpu import blank8, host, same8, state8
+from tests.test_optim_gpu import blank8, host, make, same8, state8
 
 pytestmark = pytest.mark.gpu
 BF, HF, F = torch.bfloat16, torch.float16, torch.float32
@@ -64,3 +64,30 @@ def test_small_eps_under_a_large_rate(device, lr, eps):
             assert np.isnan(got[quiet]).all() and np.isnan(x[quiet]).all()
         # three steps: two roundings of p each, and 2^-20 of an update of at most 4 lr
         assert np.abs(got - x)[~quiet].max() <= 3 * (2.0 ** -23 * np.abs(x[~quiet]).max() + 2.0 ** -20 * lr * 4)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_plan_of_the_other_state_is_left_alone(device, bits):
+    """vcr_adamw_step with the other `state_bits` than its plan's records: nothing is written.  (The moments lie in memory that an fp32
+    update of the 8-bit kind, four times as long, would stay in.)"""
+    import ctypes as C
+    from vcr_gaus_amd import _lib
+    from vcr_gaus_amd.optim import AdamW
+    n = 5000
+    whole = torch.full((16 * n,), 3, dtype=torch.uint8, device=device)
+    params, _ = make([n], F, device, seed=110)
+    opt = AdamW(params, state_bits=bits)
+    opt.step()
+    if bits == 8:
+        for k, key in enumerate(("exp_avg", "exp_avg_sq")):
+            opt.state["0"][key] = whole[8 * n * k:8 * n * k + n]
+        opt.step()
+    snap = lambda: [t.clone() for t in (params[0], whole, *opt.state["0"].values())]  # noqa: E731
+    before = snap()
+    bucket = opt._plan.buckets[0]
+    a = _lib.VcrAdamWStep.from_buffer_copy(bucket.args)
+    grads = (C.c_uint64 * 1)(params[0].grad.data_ptr())
+    a.grads, a.state_bits, a.ngroups = C.addressof(grads), 40 - bits, 1
+    a.groups, a.grad_scale = opt._group_table(device), 1.0
+    assert _lib.load().vcr_adamw_step(C.byref(a), torch.cuda.current_stream(device).cuda_stream) == 0
+    assert all(torch.equal(x, y) for x, y in zip(before, snap()))

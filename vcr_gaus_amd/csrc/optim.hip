@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
     if (!g || (clip && clip->skip)) return;
     const VcrOptimTensor& R = tensors[at.tensor];
     const uint32_t group = (uint32_t)(R.group - g0);
-    if (group >= VCR_OPT_GROUPS || (MASTER && !R.master)) return;             // (a plan that was made for another call)
+    if (group >= VCR_OPT_GROUPS || R.m_scale || (MASTER && !R.master)) return;             // (a plan that was made for another call)
     const float gs = clip ? clip->gscale : gscale;
     const long long off = at.first + threadIdx.x * 4, left = R.numel - off;
     GLOBAL T* p = global((T*)R.p) + off;
