@@ -91,3 +91,41 @@ def test_a_plan_of_the_other_state_is_left_alone(device, bits):
     a.groups, a.grad_scale = opt._group_table(device), 1.0
     assert _lib.load().vcr_adamw_step(C.byref(a), torch.cuda.current_stream(device).cuda_stream) == 0
     assert all(torch.equal(x, y) for x, y in zip(before, snap()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits):
+    """The optimizer goes, without the collector, while its last step waits on a side stream: the allocator may reuse its moments only
+    when that step is done.  Blocks of the same sizes are taken in between and hold what was written to them."""
+    import gc
+    import weakref
+    from vcr_gaus_amd.optim import AdamW
+    n = (1 << 22) + 512                               # (sizes of its own: no other block of the allocator's fits better)
+    params, _ = make([n], F, device, seed=111)
+    opt = AdamW(params, state_bits=bits)
+    opt.step()
+    torch.cuda.synchronize()
+    sizes = [t.numel() * t.element_size() for t in opt.state["0"].values()]
+    old = {t.data_ptr() for t in opt.state["0"].values() if t.numel() > 1 << 20}
+    before = [t.clone() for t in (params[0], *opt.state["0"].values())]
+    held = torch.cuda.memory_allocated(device)
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    gc.collect()
+    gc.disable()
+    try:
+        gone = weakref.ref(opt)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)             # (tens of milliseconds)
+            opt.step()
+        waiting = not side.query()
+        del opt
+        assert gone() is None and torch.cuda.memory_allocated(device) < held
+        fresh = [torch.full((max(s, 1),), 7, dtype=torch.uint8, device=device) for s in sizes for _ in range(2)]
+        still = waiting and not side.query()
+    finally:
+        gc.enable()
+    torch.cuda.synchronize()
+    assert all(bool((t == 7).all()) for t in fresh) and not torch.equal(params[0], before[0])
+    assert not still or not old & {t.data_ptr() for t in fresh}
+    assert still                                      # (else nothing was tested)

@@ -8,6 +8,7 @@ step replays), and moments in a quarter of the memory.  The reference trains wit
 """
 import ctypes as C
 import sys
+import weakref
 from array import array
 
 import torch
@@ -146,16 +147,19 @@ def _positive(x, what):
 
 class _Watched(dict):
     """A dictionary of the optimizer's state: an entry that is replaced, added or removed makes the optimizer look at its tensors anew
-    (their addresses are on the device).  Values may be changed in place freely."""
+    (their addresses are on the device).  Values may be changed in place freely.  The optimizer is held weakly: with what it trains and
+    its moments it goes when its last user lets go of it, not when the cyclic collector runs."""
     __slots__ = ("_owner",)
 
     def __init__(self, owner, items=()):
         dict.__init__(self, items)
-        self._owner = owner
+        self._owner = weakref.ref(owner)
 
     def _touch(name):
         def method(self, *a, **k):
-            self._owner._plan = None
+            owner = self._owner()
+            if owner is not None:
+                owner._plan = None
             return getattr(dict, name)(self, *a, **k)
         method.__name__ = name
         return method
