@@ -129,3 +129,75 @@ def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits):
     assert all(bool((t == 7).all()) for t in fresh) and not torch.equal(params[0], before[0])
     assert not still or not old & {t.data_ptr() for t in fresh}
     assert still                                      # (else nothing was tested)
+
+
+@pytest.mark.parametrize("bits, dtype, master", [(32, F, False), (8, F, False), (8, BF, True)])
+@pytest.mark.parametrize("how", ["data", "set_"])
+def test_replaced_storage_of_the_state_is_seen(device, bits, dtype, master, how):
+    """A state tensor gets another storage under the same object (`.data = ...`, `set_`), as a loop that offloads moments does: the next
+    step reads and writes the new one, like an optimizer that was loaded with it, and leaves the old one alone."""
+    from vcr_gaus_amd.optim import AdamW
+
+    def built():
+        params, _ = make([3000], dtype, device, seed=112, grad=1.0)
+        opt = AdamW(params, state_bits=bits, master_weights=master, seed=2)
+        opt.step()
+        return params[0], opt, opt.state["0"]
+
+    names = list(built()[2])
+    for name in names:
+        (p, opt, st), (q, ref, sr) = built(), built()
+        old = st[name].detach()                        # (holds the old storage)
+        kept = old.clone()
+        new = old + 1 if old.dtype != torch.uint8 else old.clone().fill_(120)
+        sr[name] = new.clone()
+        if how == "data":
+            st[name].data = new
+        else:
+            st[name].set_(new)
+        opt.step()
+        ref.step()
+        assert torch.equal(old, kept), name
+        assert torch.equal(p, q) and all(torch.equal(t, sr[k]) for k, t in st.items()), name
+        if name in ("exp_avg", "exp_avg_sq"):
+            assert all(torch.equal(a[0], b[0]) for a, b in zip(opt.moments(), ref.moments()))
+
+
+def test_storage_that_no_longer_fits_is_refused(device):
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([300], F, device, seed=113)
+    opt = AdamW(params)
+    opt.step()
+    good = opt.state["0"]["exp_avg"].data
+    before = params[0].detach().clone()
+    for bad in (good.cpu(), good[:299], good.double(), torch.zeros(600, device=device)[::2]):
+        opt.state["0"]["exp_avg"].data = bad
+        with pytest.raises(ValueError, match="exp_avg"):
+            opt.step()
+    opt.state["0"]["exp_avg"].data = good
+    assert torch.equal(params[0], before)
+    opt.state["0"]["note"] = "anything"                # (entries of the caller's own are let alone)
+    opt.step()
+    with torch.cuda.stream(torch.cuda.Stream(device)):
+        opt.step()
+    assert int(opt.state["0"]["step"]) == 3
+
+
+def test_a_graph_keeps_the_storages_it_writes(device):
+    """After a capture, parameter and moments get other storages: a replay writes the captured ones, which nothing else was given."""
+    from vcr_gaus_amd.optim import AdamW
+    n = (1 << 21) + 256
+    params, _ = make([n], F, device, seed=114)
+    params[0].data = params[0].data.clone()            # (a storage of its own)
+    opt = AdamW(params)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for t in (params[0], *opt.state["0"].values()):
+        t.data = t.data.clone()
+    fresh = [torch.full((4 * n,), 7, dtype=torch.uint8, device=device) for _ in range(6)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(bool((t == 7).all()) for t in fresh) and int(opt.state["0"]["step"]) == 1

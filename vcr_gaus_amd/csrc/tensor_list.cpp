@@ -101,6 +101,52 @@ PyObject* gradients(PyObject*, PyObject* args) {
     });
 }
 
+// What a tensor's memory is: address, elements, and type, device and layout.
+struct Memory {
+    uint64_t at;
+    int64_t numel;
+    int32_t type, device, dense, pad;
+    explicit Memory(const at::Tensor& t)
+        : at((uint64_t)(uintptr_t)t.const_data_ptr()), numel(t.numel()), type((int32_t)t.scalar_type()),
+          device(t.is_cuda() ? (int32_t)t.device().index() : -1), dense(t.is_contiguous()), pad(0) {}
+    bool operator!=(const Memory& o) const {
+        return at != o.at || numel != o.numel || type != o.type || device != o.device || dense != o.dense;
+    }
+};
+
+// memory(list) -> bytes: the Memory of each tensor
+PyObject* memory(PyObject*, PyObject* list) {
+    return guarded([&]() -> PyObject* {
+        if (!PyList_CheckExact(list)) { PyErr_SetString(PyExc_TypeError, "memory: a list of tensors"); return nullptr; }
+        const Py_ssize_t n = PyList_GET_SIZE(list);
+        THPObjectPtr blob(PyBytes_FromStringAndSize(nullptr, n * sizeof(Memory)));
+        if (!blob) return nullptr;
+        Memory* m = (Memory*)PyBytes_AS_STRING(blob.get());
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* o = PyList_GET_ITEM(list, i);
+            if (!THPVariable_Check(o)) { PyErr_SetString(PyExc_TypeError, "memory: a list of tensors"); return nullptr; }
+            m[i] = Memory(THPVariable_Unpack(o));
+        }
+        return blob.release();
+    });
+}
+
+// in_place(list, bytes) -> whether every tensor's memory is what `memory` of this list gave
+PyObject* in_place(PyObject*, PyObject* args) {
+    return guarded([&]() -> PyObject* {
+        PyObject *list, *known;
+        if (!PyArg_ParseTuple(args, "O!S", &PyList_Type, &list, &known)) return nullptr;
+        const Py_ssize_t n = PyList_GET_SIZE(list);
+        if (PyBytes_GET_SIZE(known) != n * (Py_ssize_t)sizeof(Memory)) Py_RETURN_FALSE;
+        const Memory* m = (const Memory*)PyBytes_AS_STRING(known);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* o = PyList_GET_ITEM(list, i);
+            if (!THPVariable_Check(o) || Memory(THPVariable_Unpack(o)) != m[i]) Py_RETURN_FALSE;
+        }
+        Py_RETURN_TRUE;
+    });
+}
+
 // changed(list, words): the tensors (words: those whose 64-bit word in these bytes is not 0) have been written to behind torch's back:
 // their version counters move, so that a backward that needs the old values says so instead of using the new ones
 PyObject* changed(PyObject*, PyObject* args) {
@@ -124,6 +170,7 @@ PyObject* changed(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"words", words, METH_O, nullptr}, {"gradients", gradients, METH_VARARGS, nullptr},
+                         {"memory", memory, METH_O, nullptr}, {"in_place", in_place, METH_VARARGS, nullptr},
                          {"changed", changed, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_list", nullptr, -1, methods};
 

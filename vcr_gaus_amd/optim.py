@@ -178,7 +178,8 @@ class _Bucket:
 
 
 class _Plan:
-    __slots__ = ("params", "identity", "dtypes", "keys", "sizes", "numels", "buckets", "device", "streams", "captured", "covered", "keep")
+    __slots__ = ("params", "identity", "dtypes", "keys", "sizes", "numels", "buckets", "device", "streams", "captured", "covered", "state",
+                 "memory", "keep")
 
 
 class AdamW:
@@ -303,6 +304,7 @@ class AdamW:
         return self.master_weights and p.dtype != torch.float32
 
     def _check_state(self, key, p, st):
+        """-> the tensors of the parameter's state that a step reads and writes."""
         n, nb = p.numel(), -(-p.numel() // BLOCK)
         want = {"step": (torch.int32, 1)}
         kind = torch.float32 if self.state_bits == 32 else torch.uint8
@@ -315,6 +317,7 @@ class AdamW:
             t = st.get(k)
             if not isinstance(t, torch.Tensor) or t.dtype != dt or t.numel() != m or t.device != p.device or not t.is_contiguous():
                 raise ValueError(f"AdamW: state[{key!r}][{k!r}] must be {m} contiguous elements of {dt} on {p.device}")
+        return [st[k] for k in want]
 
     def _build(self, identity, need):
         """Plan of all parameters that have a state, and of those in `need`, which get one.  `identity`: the native lists' words."""
@@ -330,7 +333,7 @@ class AdamW:
         if len(set(map(id, plan.params))) != len(plan.params):
             raise ValueError("AdamW: a parameter appears twice")
         self._check_dense(plan.params)
-        by = {}
+        by, plan.state, plan.keep = {}, [], []
         for i, (p, key) in enumerate(zip(plan.params, keys)):
             if key not in self.state:
                 if i not in need:
@@ -342,10 +345,10 @@ class AdamW:
                 dict.__setitem__(self.state, key, st)
             if self._has_master(p) and "master" not in st:
                 dict.__setitem__(st, "master", p.detach().float().contiguous())
-            self._check_state(key, p, st)
+            plan.state += self._check_state(key, p, st)
             by.setdefault(_TYPES[p.dtype], []).append(i)
         plan.buckets, plan.covered = [], sum(map(len, by.values()))
-        plan.keep = [t for at in by.values() for i in at for t in self.state[keys[i]].values()]          # (a graph may hold their addresses)
+        plan.memory = _native().memory(plan.state)
         for kind, at in by.items():
             b = _Bucket()
             b.type, b.at, b.n, b.every = kind, at, len(at), len(at) == len(plan.params)
@@ -374,10 +377,11 @@ class AdamW:
         return plan
 
     def _current(self, params, words, flags):
-        """The plan, rebuilt where a parameter or a state entry is another tensor than it holds, or where one that is to be stepped
-        (has a gradient and a flag) is not in it."""
+        """The plan, rebuilt where a parameter or a state entry is another tensor than it holds or has other memory, or where one that is
+        to be stepped (has a gradient and a flag) is not in it."""
         plan, identity = self._plan, words[8 * len(params):]
-        fits = plan is not None and plan.identity == identity and [len(g["params"]) for g in self.param_groups] == plan.sizes
+        fits = (plan is not None and plan.identity == identity and [len(g["params"]) for g in self.param_groups] == plan.sizes
+                and _native().in_place(plan.state, plan.memory))
         if not fits or plan.covered < len(params):
             need = {i for i, p in enumerate(params) if p.grad is not None and (flags is None or flags[i])}
             if not fits or not need <= {i for b in plan.buckets for i in b.at}:
@@ -385,12 +389,13 @@ class AdamW:
         stream = _stream(plan.device.index)
         if stream not in plan.streams:          # (what is freed later is not given away before this stream is done with it)
             plan.streams.add(stream)
-            for t in plan.keep + [b.plan for b in plan.buckets]:
+            for t in plan.state + [b.plan for b in plan.buckets]:
                 t.record_stream(torch.cuda.current_stream(plan.device))
         if torch.cuda.is_current_stream_capturing():        # the graph holds these addresses
             plan.keep += [g["lr"] for g in self.param_groups if isinstance(g["lr"], torch.Tensor)]
-            if not plan.captured:
+            if not plan.captured:                           # (aliases: they hold the memory whatever becomes of the tensors)
                 plan.captured = True
+                plan.keep += [t.detach() for t in plan.state + plan.params]
                 self._captured.append(plan)
         return plan, stream
 
