@@ -94,9 +94,11 @@ def test_a_plan_of_the_other_state_is_left_alone(device, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits):
+@pytest.mark.parametrize("loaded", [False, True])
+def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits, loaded):
     """The optimizer goes, without the collector, while its last step waits on a side stream: the allocator may reuse its moments only
-    when that step is done.  Blocks of the same sizes are taken in between and hold what was written to them."""
+    when that step is done.  Blocks of the same sizes are taken in between and hold what was written to them.  `loaded`: the state
+    comes from a checkpoint read on the main stream, and the side stream's step is its first."""
     import gc
     import weakref
     from vcr_gaus_amd.optim import AdamW
@@ -104,6 +106,12 @@ def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits):
     params, _ = make([n], F, device, seed=111)
     opt = AdamW(params, state_bits=bits)
     opt.step()
+    if loaded:
+        sd = opt.state_dict()
+        sd["state"][0] = {k: t.clone() for k, t in sd["state"][0].items()}
+        opt = AdamW(params, state_bits=bits)
+        opt.load_state_dict(sd)
+        del sd
     torch.cuda.synchronize()
     sizes = [t.numel() * t.element_size() for t in opt.state["0"].values()]
     old = {t.data_ptr() for t in opt.state["0"].values() if t.numel() > 1 << 20}
@@ -116,6 +124,8 @@ def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits):
     try:
         gone = weakref.ref(opt)
         with torch.cuda.stream(side):
+            if loaded:
+                opt.moments()                          # (builds the plan, and waits for this stream once)
             torch.cuda._sleep(50_000_000)             # (tens of milliseconds)
             opt.step()
         waiting = not side.query()

@@ -370,9 +370,8 @@ class AdamW:
                                        masters=int(self.master_weights and kind != 0), seed=self.seed, plan=b.plan.data_ptr(),
                                        numel=_address(b.numels), group_of=_address(b.group_of))
             plan.buckets.append(b)
-        stream = torch.cuda.current_stream(plan.device)
-        stream.synchronize()                     # (the upload is finished whatever stream the steps use)
-        plan.streams = {stream.cuda_stream}
+        torch.cuda.current_stream(plan.device).synchronize()          # (the upload is finished whatever stream the steps use)
+        plan.streams = set()                     # (those that use it: none yet, the state may come from another than this one)
         self._plan = plan
         return plan
 
