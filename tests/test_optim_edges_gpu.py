@@ -211,3 +211,25 @@ def test_a_graph_keeps_the_storages_it_writes(device):
     graph.replay()
     torch.cuda.synchronize()
     assert all(bool((t == 7).all()) for t in fresh) and int(opt.state["0"]["step"]) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_outputs_that_are_given_are_seen_to_change(device, bits):
+    """Version counters move, so that a backward that saved such a tensor says so: the norm's `out`, lists for the moments."""
+    from vcr_gaus_amd.optim import AdamW, grad_norm
+    params, _ = make([300, 5], F, device, seed=115)
+    w = torch.ones((), device=device, requires_grad=True)
+    out = torch.zeros((), device=device)
+    loss = w * out
+    grad_norm([p.grad for p in params], out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    opt = AdamW(params, state_bits=bits)
+    for late in (True, False):                        # before the first step (zeros), and after it
+        outs = [[torch.ones_like(p) for p in params] for _ in range(2)]
+        before = [t._version for o in outs for t in o]
+        opt.moments(*outs)
+        assert all(t._version > v for t, v in zip(outs[0] + outs[1], before))
+        assert [t._version for t in opt.moments(outs[0])[0]] > [v + 1 for v in before[:2]]
+        if late:
+            opt.step()

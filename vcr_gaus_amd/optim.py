@@ -96,8 +96,8 @@ def grad_norm(tensors, out=None):
     float32 tensor on their device.  Sums in 64 bits in a fixed order: the same result on every run; NaN or infinity anywhere gives
     NaN or infinity.  No tensors: an error, as there is no device to put the result on -- unless `out` is given."""
     words = _List([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), "tensors", "grad_norm")
-    dev = words.device
-    if out is None:
+    dev, own = words.device, out is None
+    if own:
         if dev is None:
             raise ValueError("grad_norm: no tensors and no `out`")
         out = torch.empty((), device=dev)
@@ -105,6 +105,8 @@ def grad_norm(tensors, out=None):
         raise ValueError("grad_norm: `out` must be one float32 element on the tensors' device")
     dev = out.device
     _on(dev, _norm, words.args, out, _stream(dev.index))
+    if not own:
+        _native().changed([out], None)
     return out
 
 
@@ -531,6 +533,9 @@ class AdamW:
                 some = None if b.every else [array("Q", [o[i].data_ptr() for i in b.at]) for o in outs]
                 m, v = (f[2] for f in found) if b.every else map(_address, some)
                 _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), _address(b.numels), m, v, kind, stream))
+            for given, o in zip((exp_avgs, exp_avg_sqs), outs):
+                if given is not None:
+                    _native().changed(list(o), None)
         return outs
 
     @torch.no_grad()
