@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from vcr_gaus_amd import _lib
+from vcr_gaus_amd.gaussian_model import FusedAdam, GaussianAdamW
 from vcr_gaus_amd.optim import AdamW
 
 
@@ -60,3 +61,42 @@ def test_native_lists_know_a_tensors_memory():
     assert not native.in_place([a, 1], known)
     with pytest.raises(TypeError):
         native.in_place((a, b), known)
+
+
+def model_groups():
+    """(as `GaussianModel` makes them, with a classifier)"""
+    shapes = dict(xyz=(4, 3), f_dc=(4, 1, 3), opacity=(4, 1))
+    groups = [dict(params=[P(*s)], lr=0.1, name=k) for k, s in shapes.items()]
+    return groups + [dict(params=[P(2, 3)], lr=0.1, name="classifier.weight", aux=True), dict(params=[P(2)], lr=0.1, name="classifier.bias", aux=True)]
+
+
+def state_of(shape, first=0.0, **other):
+    n = int(torch.tensor(shape).prod())
+    return dict(step=torch.tensor(7.0), exp_avg=torch.arange(first, first + n).view(shape), exp_avg_sq=torch.ones(shape), **other)
+
+
+@pytest.mark.parametrize("of", ["exp_avg", "exp_avg_sq", "master"])
+def test_moments_of_another_shape_are_refused(of):
+    """As many values in another order: refused, and the optimizer stays as it was."""
+    opt = AdamW([torch.nn.Parameter(torch.zeros(4, 3, dtype=torch.bfloat16))], master_weights=True)
+    sd = opt.state_dict()
+    sd["state"] = {0: state_of((4, 3), master=torch.zeros(4, 3))}
+    opt.load_state_dict(sd)
+    before = opt.state["0"]
+    bad = copy.deepcopy(sd)
+    bad["state"][0][of] = bad["state"][0][of].t()
+    bad["param_groups"][0]["lr"] = 9.0
+    with pytest.raises(ValueError, match="shape"):
+        opt.load_state_dict(bad)
+    assert opt.state["0"] is before and opt.param_groups[0]["lr"] == 1e-3
+
+
+@pytest.mark.parametrize("cls", [GaussianAdamW, FusedAdam])
+def test_model_optimizers_refuse_moments_of_another_shape(cls):
+    opt = cls(model_groups())
+    sd = dict(state={0: state_of((3, 4))}, param_groups=[dict(name="xyz", lr=0.5, params=[0])])
+    with pytest.raises(ValueError, match="shape"):
+        opt.load_state_dict(sd)
+    sd["state"][0] = state_of((4, 3))
+    opt.load_state_dict(sd)
+    assert torch.equal(opt.state["xyz"]["exp_avg"], torch.arange(12.0).view(4, 3)) and opt.param_groups[0]["lr"] == 0.5

@@ -618,8 +618,8 @@ class AdamW:
 
     def _converted(self, key, p, st, step):
         dev, n, nb = p.device, p.numel(), -(-p.numel() // BLOCK)
-        for k in ("exp_avg", "exp_avg_sq"):
-            if st[k].numel() != n:
+        for k in ("exp_avg", "exp_avg_sq"):              # (the shape: moments in another order fit by their number alone)
+            if tuple(st[k].shape) != tuple(p.shape):
                 raise ValueError(f"optimizer state of {key!r} has shape {tuple(st[k].shape)}, parameter {tuple(p.shape)}")
         out = dict(step=step)
         as_held = lambda t, dt: t.detach().to(device=dev, dtype=dt).contiguous()  # noqa: E731
@@ -641,6 +641,8 @@ class AdamW:
                 out.update({k: torch.ones(nb, dtype=torch.uint8, device=dev) for k in ("exp_avg_scale", "exp_avg_sq_scale")})
                 encode8(m, v, out)
         if self._has_master(p):
+            if "master" in st and tuple(st["master"].shape) != tuple(p.shape):
+                raise ValueError(f"optimizer state of {key!r}: the master has shape {tuple(st['master'].shape)}, parameter {tuple(p.shape)}")
             out["master"] = as_held(st["master"], torch.float32) if "master" in st else p.detach().float().contiguous()
         return out
 
