@@ -100,3 +100,19 @@ def test_model_optimizers_refuse_moments_of_another_shape(cls):
     sd["state"][0] = state_of((4, 3))
     opt.load_state_dict(sd)
     assert torch.equal(opt.state["xyz"]["exp_avg"], torch.arange(12.0).view(4, 3)) and opt.param_groups[0]["lr"] == 0.5
+
+
+@pytest.mark.parametrize("cls", [GaussianAdamW, FusedAdam])
+def test_model_optimizers_read_files_keyed_by_group_name(cls):
+    """The older form: state by group name, the classifier's tensors by their own; groups that the file lacks keep rate and no state."""
+    opt = cls(model_groups())
+    sd = dict(state={"xyz": state_of((4, 3)), "classifier.bias": state_of((2,), 5.0), "gone": state_of((9,))},
+              param_groups=[dict(name="xyz", lr=0.5), dict(name="f_dc", lr=0.25), dict(name="gone", lr=1.0)])
+    opt.load_state_dict(sd)
+    assert sorted(opt.state) == ["classifier.bias", "xyz"] and int(opt.state["xyz"]["step"]) == 7
+    assert torch.equal(opt.state["xyz"]["exp_avg"], torch.arange(12.0).view(4, 3))
+    assert torch.equal(opt.state["classifier.bias"]["exp_avg"], torch.tensor([5.0, 6.0]))
+    assert [g["lr"] for g in opt.param_groups] == [0.5, 0.25, 0.1, 0.1, 0.1]
+    sd["state"]["xyz"] = state_of((3, 4))
+    with pytest.raises(ValueError, match="shape"):
+        opt.load_state_dict(sd)

@@ -378,6 +378,11 @@ class FusedAdam:
     def _wire_name(name):
         return name.split(".", 1)[0] if name.startswith("classifier.") else name
 
+    @staticmethod
+    def _keyed_by_name(sd):
+        """Older files of this repo: state keyed by group name, groups without `params`."""
+        return any("params" not in g for g in sd["param_groups"]) or not all(isinstance(k, int) for k in sd["state"])
+
     def state_dict(self):
         template = torch.optim.Adam([torch.zeros(1)], lr=0.0, eps=self.eps, betas=self.betas).param_groups[0]
         state, groups, idx = {}, [], 0
@@ -405,9 +410,7 @@ class FusedAdam:
         for g in self.param_groups:
             by_wire.setdefault(self._wire_name(g["name"]), []).append(g)
         self.state = {}
-        legacy = any("params" not in g for g in sd["param_groups"]) or \
-            (sd["state"] and not all(isinstance(k, int) for k in sd["state"]))
-        if legacy:                                              # older files of this repo: state keyed by group name
+        if self._keyed_by_name(sd):
             mine = {g["name"]: g for g in self.param_groups}
             for k, v in sd["state"].items():
                 if k not in mine:
@@ -457,7 +460,14 @@ class GaussianAdamW(AdamW):
         return dict(state=sd["state"], param_groups=groups)
 
     def load_state_dict(self, sd):
-        """Takes the learning rates and moments of the groups that the file has; the other hyper-parameters are the configuration's."""
+        """Takes the learning rates and moments of the groups that the file has; the other hyper-parameters are the configuration's.
+        Reads what `FusedAdam.load_state_dict` reads."""
+        if FusedAdam._keyed_by_name(sd):
+            lrs = {wg["name"]: float(wg["lr"]) for wg in sd["param_groups"]}
+            names = [g["name"] for g in self.param_groups]
+            groups = [dict(params=[i], **(dict(lr=lrs[k]) if k in lrs else {})) for i, k in enumerate(names)]
+            state = {i: sd["state"][k] for i, k in enumerate(names) if k in sd["state"]}
+            return super().load_state_dict(dict(state=state, param_groups=groups))
         saved = {wg.get("name"): wg for wg in sd["param_groups"]}
         taken, state, groups = {}, {}, []
         for i, g in enumerate(self.param_groups):
