@@ -233,3 +233,26 @@ def test_outputs_that_are_given_are_seen_to_change(device, bits):
         assert [t._version for t in opt.moments(outs[0])[0]] > [v + 1 for v in before[:2]]
         if late:
             opt.step()
+
+
+@pytest.mark.parametrize("kind", ["cuda", "cpu", "double"])
+def test_a_saved_device_rate_is_loaded_as_one(device, kind, tmp_path):
+    """A rate that is a device scalar, saved and read to the host or kept: the loading optimizer has one of its own on its device."""
+    from vcr_gaus_amd.optim import AdamW
+    both = []
+    for _ in range(2):
+        params, _ = make([300, 5], F, device, seed=116)
+        both.append((params, AdamW(params, lr=torch.tensor(0.25, device=device))))
+        both[-1][1].step()
+    (pa, a), (pb, b) = both
+    torch.save(a.state_dict(), tmp_path / "o.pth")
+    sd = torch.load(tmp_path / "o.pth", weights_only=True, map_location="cpu" if kind == "cpu" else None)
+    if kind == "double":
+        sd["param_groups"][0]["lr"] = sd["param_groups"][0]["lr"].double()
+    c = AdamW(pb, lr=7.0)
+    c.load_state_dict(sd)
+    a.step()
+    c.step()
+    assert all(torch.equal(x, y) for x, y in zip(pa, pb))
+    c.param_groups[0]["lr"].fill_(9.0)
+    assert float(sd["param_groups"][0]["lr"]) == 0.25 and c.param_groups[0]["lr"].device == device

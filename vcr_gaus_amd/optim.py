@@ -612,6 +612,9 @@ class AdamW:
             for k in ("lr", "eps", "weight_decay"):
                 if k in wg:
                     g[k] = wg[k]
+            if "lr" in wg and isinstance(g["lr"], torch.Tensor):            # (the optimizer's own, on its device, wherever the file was read to)
+                dev = g["params"][0].device if g["params"] else g["lr"].device
+                g["lr"] = g["lr"].detach().to(device=dev, dtype=torch.float32, copy=True)
             if "betas" in wg:
                 g["betas"] = tuple(wg["betas"])
         self.state = new
