@@ -256,3 +256,19 @@ def test_a_saved_device_rate_is_loaded_as_one(device, kind, tmp_path):
     assert all(torch.equal(x, y) for x, y in zip(pa, pb))
     c.param_groups[0]["lr"].fill_(9.0)
     assert float(sd["param_groups"][0]["lr"]) == 0.25 and c.param_groups[0]["lr"].device == device
+
+
+def test_a_changed_seed_counts_from_the_next_step(device):
+    """Whether the optimizer looks at its tensors anew in between or not, and for any whole number."""
+    from vcr_gaus_amd.optim import AdamW
+    codes = []
+    for seed, again in ((2, False), (2, True), (2 - (1 << 40), False), (1, False)):
+        params, _ = make([3000], F, device, seed=117)
+        opt = AdamW(params, state_bits=8, seed=1)
+        opt.step()
+        opt.seed = seed
+        if again:
+            opt.state = dict(opt.state)
+        opt.step()
+        codes.append(opt.state["0"]["exp_avg"].clone())
+    assert torch.equal(codes[0], codes[1]) and torch.equal(codes[0], codes[2]) and not torch.equal(codes[0], codes[3])

@@ -369,7 +369,7 @@ class AdamW:
             _lib.check(lib.vcr_optim_plan(b.n, rec, host.data_ptr(), size))
             b.plan = host.to(plan.device)
             b.args = _lib.VcrAdamWStep(ntensors=b.n, param_type=kind, state_bits=self.state_bits,
-                                       masters=int(self.master_weights and kind != 0), seed=self.seed, plan=b.plan.data_ptr(),
+                                       masters=int(self.master_weights and kind != 0), plan=b.plan.data_ptr(),
                                        numel=_address(b.numels), group_of=_address(b.group_of))
             plan.buckets.append(b)
         torch.cuda.current_stream(plan.device).synchronize()          # (the upload is finished whatever stream the steps use)
@@ -481,6 +481,7 @@ class AdamW:
             mine = None if b.every else array("Q", [grads[i] for i in b.at])
             a = b.args
             a.grads, a.groups, a.ngroups, a.grad_scale = at if b.every else _address(mine), groups, len(groups), float(self.grad_scale)
+            a.seed = self.seed & 0xFFFFFFFF
             a.clip = None if clip is None else clip.data_ptr()
             _lib.check(lib.vcr_adamw_step(C.byref(a), stream))
         return norm
