@@ -116,3 +116,13 @@ def test_model_optimizers_read_files_keyed_by_group_name(cls):
     sd["state"]["xyz"] = state_of((3, 4))
     with pytest.raises(ValueError, match="shape"):
         opt.load_state_dict(sd)
+
+
+def test_the_kind_of_the_state_is_fixed():
+    """Codes would be read as values, or the other way round."""
+    opt = copy.deepcopy(AdamW([P(3)], state_bits=8, master_weights=True))
+    assert opt.state_bits == 8 and opt.master_weights is True
+    with pytest.raises(AttributeError):
+        opt.state_bits = 32
+    with pytest.raises(AttributeError):
+        opt.master_weights = False

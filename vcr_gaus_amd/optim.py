@@ -213,7 +213,7 @@ class AdamW:
         self.defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay)
         groups = params if isinstance(params[0], dict) else [dict(params=params)]
         self.param_groups = [self._filled(g) for g in groups]
-        self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed) & 0xFFFFFFFF
+        self._state_bits, self._master_weights, self.seed = int(state_bits), bool(master_weights), int(seed) & 0xFFFFFFFF
         self.grad_scale = 1.0
         self._plan, self._captured, self._rates = None, [], None
         self._state_dict = _Watched(self)
@@ -256,6 +256,10 @@ class AdamW:
         self.state = d["_state_dict"]
 
     # ---- what is trained ---------------------------------------------------------------------------------------------
+    # (what the state is held in: fixed, as the tensors of `state` are of that kind)
+    state_bits = property(lambda self: self._state_bits)
+    master_weights = property(lambda self: self._master_weights)
+
     @property
     def state(self):
         return self._state_dict
