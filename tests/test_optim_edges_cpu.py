@@ -126,3 +126,16 @@ def test_the_kind_of_the_state_is_fixed():
         opt.state_bits = 32
     with pytest.raises(AttributeError):
         opt.master_weights = False
+
+
+@pytest.mark.parametrize("kw", [dict(amsgrad=True), dict(maximize=True)])
+def test_checkpoints_of_another_update_are_refused(kw):
+    """torch.optim.AdamW's variants that this update does not have: not continued as something else without a word."""
+    p = P(3)
+    p.grad = torch.ones(3)
+    ref = torch.optim.AdamW([dict(params=[p], name="xyz")], **kw)
+    ref.step()
+    for opt in (AdamW([p]), GaussianAdamW([dict(params=[p], name="xyz")])):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            opt.load_state_dict(ref.state_dict())
+        assert opt.state == {}

@@ -479,6 +479,7 @@ class GaussianAdamW(AdamW):
                 continue
             if j >= len(wg["params"]):
                 raise ValueError(f"optimizer group {wire!r}: {len(wg['params'])} tensors saved, more here")
+            self._check_saved(wg)
             groups.append(dict(params=[i], lr=float(wg["lr"])))
             if wg["params"][j] in sd["state"]:
                 state[i] = sd["state"][wg["params"][j]]

@@ -606,6 +606,7 @@ class AdamW:
         for k, (wg, g) in enumerate(zip(sd["param_groups"], self.param_groups)):
             if len(wg["params"]) != len(g["params"]):
                 raise ValueError(f"AdamW: group {k}: {len(wg['params'])} tensors saved, {len(g['params'])} here")
+            self._check_saved(wg)
             order += list(wg["params"])
         new = {}
         held = [(key, p, sd["state"][i]) for i, key, p in zip(order, self._keys(), self._tensors()) if i in sd["state"]]
@@ -623,6 +624,12 @@ class AdamW:
             if "betas" in wg:
                 g["betas"] = tuple(wg["betas"])
         self.state = new
+
+    @staticmethod
+    def _check_saved(wg):
+        for k in ("amsgrad", "maximize"):
+            if wg.get(k):
+                raise ValueError(f"AdamW: the checkpoint's optimizer ran with {k}=True, which this one does not do")
 
     def _converted(self, key, p, st, step):
         dev, n, nb = p.device, p.numel(), -(-p.numel() // BLOCK)
