@@ -9,7 +9,7 @@ import torch
 
 from vcr_gaus_amd import _lib
 from vcr_gaus_amd.gaussian_model import FusedAdam, GaussianAdamW
-from vcr_gaus_amd.optim import AdamW
+from vcr_gaus_amd.optim import AdamW, decode8, encode8
 
 
 def P(*shape):
@@ -139,3 +139,29 @@ def test_checkpoints_of_another_update_are_refused(kw):
         with pytest.raises(ValueError, match=next(iter(kw))):
             opt.load_state_dict(ref.state_dict())
         assert opt.state == {}
+
+
+def test_codes_and_values_that_do_not_fit_are_refused():
+    """Before anything reaches a device: the kernels go by the number of codes alone."""
+    def state(**other):
+        st = {k: torch.zeros(300 if "scale" not in k else 2, dtype=torch.uint8) for k in
+              ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
+        st.update(other)
+        return st
+
+    x = torch.zeros(300)
+    for k in state():
+        n = state()[k].numel()
+        for bad in (torch.zeros(n - 1, dtype=torch.uint8), torch.zeros(n), torch.zeros(2 * n, dtype=torch.uint8)[::2]):
+            with pytest.raises(ValueError, match="exp_avg"):
+                decode8(state(**{k: bad}))
+            with pytest.raises(ValueError, match="exp_avg"):
+                encode8(x, x, state(**{k: bad}))
+    for bad in (x[:299], x.double(), torch.zeros(600)[::2], torch.zeros(0)):
+        for m, v in ((bad, x), (x, bad)):
+            with pytest.raises(ValueError, match="values of"):
+                encode8(m, v, state())
+    with pytest.raises(ValueError, match="HIP device"):
+        encode8(x, x, state())
+    with pytest.raises(ValueError, match="HIP device"):
+        decode8(state())

@@ -662,10 +662,22 @@ class AdamW:
         return out
 
 
-def _single(st, n):
+def _check_codes(st):
+    """-> elements and device of the 8-bit moments in `st`, whose four tensors must fit each other."""
+    n, dev = st["exp_avg"].numel(), st["exp_avg"].device
+    nb = -(-n // BLOCK)
+    for k, m in (("exp_avg", n), ("exp_avg_sq", n), ("exp_avg_scale", nb), ("exp_avg_sq_scale", nb)):
+        t = st[k]
+        if t.dtype != torch.uint8 or t.numel() != m or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"8-bit moments: {k!r} must be {m} contiguous elements of torch.uint8 on {dev}")
+    if dev.type != "cuda":
+        raise ValueError("8-bit moments need a HIP device")
+    return n, dev
+
+
+def _single(st, n, dev):
     """A plan of one tensor's 8-bit moments, for the code <-> value kernels."""
     lib = _lib.load()
-    dev = st["exp_avg"].device
     rec = (_lib.VcrOptimTensor * 1)()
     rec[0].p = rec[0].m = st["exp_avg"].data_ptr()
     rec[0].v, rec[0].m_scale, rec[0].v_scale = (st[k].data_ptr() for k in ("exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"))
@@ -680,25 +692,24 @@ def _single(st, n):
 
 def encode8(exp_avg, exp_avg_sq, st):
     """float32 moments into the uint8 tensors `exp_avg`, `exp_avg_sq`, `exp_avg_scale`, `exp_avg_sq_scale` of `st`, to the nearest."""
-    if exp_avg.numel() == 0:
-        return
-    dev = st["exp_avg"].device
-    if dev.type != "cuda":
-        raise ValueError("8-bit moments need a HIP device")
-    plan, ns = _single(st, exp_avg.numel())
-    m, v = array("Q", [exp_avg.data_ptr()]), array("Q", [exp_avg_sq.data_ptr()])
-    _lib.check(_on(dev, _lib.load().vcr_moments8_encode, 1, plan.data_ptr(), _address(ns), _address(m), _address(v),
-                   _lib.stream_of(st["exp_avg"])))
+    for k, t in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)):
+        if t.dtype != torch.float32 or t.numel() != st["exp_avg"].numel() or t.device != st["exp_avg"].device or not t.is_contiguous():
+            raise ValueError(f"encode8: the values of {k!r} must be {st['exp_avg'].numel()} contiguous elements of torch.float32 on "
+                             f"{st['exp_avg'].device}")
+    n, dev = _check_codes(st)
+    if n:
+        plan, ns = _single(st, n, dev)
+        m, v = array("Q", [exp_avg.data_ptr()]), array("Q", [exp_avg_sq.data_ptr()])
+        _lib.check(_on(dev, _lib.load().vcr_moments8_encode, 1, plan.data_ptr(), _address(ns), _address(m), _address(v),
+                       _lib.stream_of(st["exp_avg"])))
 
 
 def decode8(st):
     """-> the float32 values of the 8-bit moments in `st`, of their shape."""
-    dev = st["exp_avg"].device
+    n, dev = _check_codes(st)
     outs = [torch.empty(st["exp_avg"].shape, device=dev) for _ in range(2)]
-    if outs[0].numel():
-        if dev.type != "cuda":
-            raise ValueError("8-bit moments need a HIP device")
-        plan, ns = _single(st, outs[0].numel())
+    if n:
+        plan, ns = _single(st, n, dev)
         m, v = (array("Q", [o.data_ptr()]) for o in outs)
         _lib.check(_on(dev, _lib.load().vcr_moments8_decode, 1, plan.data_ptr(), _address(ns), _address(m), _address(v), 0,
                        _lib.stream_of(st["exp_avg"])))
