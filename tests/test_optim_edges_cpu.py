@@ -165,3 +165,15 @@ def test_codes_and_values_that_do_not_fit_are_refused():
         encode8(x, x, state())
     with pytest.raises(ValueError, match="HIP device"):
         decode8(state())
+
+
+def test_native_lists_find_shared_memory():
+    native, x = _lib.tensor_list(), torch.zeros(100)
+    far = torch.zeros(100)
+    for tensors, want in (([], None), ([x], None), ([x, far], None), ([x, x], (0, 1)), ([x[:50], x[50:]], None), ([x[:51], far, x[50:]], (0, 2)),
+                          ([x[10:20], x[30:40], x[:35]], (0, 2)), ([x, x[5:6], x[90:91]], (0, 1)), ([x[:0], x, x[50:50]], None),
+                          ([x[20:40], x[:20].view(torch.bfloat16), x[40:].view(torch.uint8)], None), ([x[:21].view(torch.uint8), x[20:40]], (0, 1))):
+        assert native.sharing(tensors) == want, want
+    for bad in ((x,), [x, 1]):
+        with pytest.raises(TypeError):
+            native.sharing(bad)

@@ -272,3 +272,30 @@ def test_a_changed_seed_counts_from_the_next_step(device):
         opt.step()
         codes.append(opt.state["0"]["exp_avg"].clone())
     assert torch.equal(codes[0], codes[1]) and torch.equal(codes[0], codes[2]) and not torch.equal(codes[0], codes[3])
+
+
+def test_memory_that_a_step_would_write_twice_is_refused(device):
+    """Two parameters, or a parameter's two moments, in the same memory: refused before a launch whose result had no order; a parameter
+    that is never stepped may be an alias."""
+    from vcr_gaus_amd.optim import AdamW
+    x = torch.ones(1000, device=device)
+    a, b = torch.nn.Parameter(x[:600]), torch.nn.Parameter(x[599:])
+    opt = AdamW([dict(params=[a], name="a"), dict(params=[b], name="b")])
+    a.grad = torch.ones_like(a)
+    opt.step()
+    before = x.clone()
+    b.grad = torch.ones_like(b)
+    with pytest.raises(ValueError, match="parameter 'a' and parameter 'b' share memory"):
+        opt.step()
+    assert list(opt.state) == ["a"]
+    b.grad = None
+    opt.state = {"a": dict(opt.state["a"], exp_avg_sq=opt.state["a"]["exp_avg"])}
+    with pytest.raises(ValueError, match=r"\['exp_avg'\] and state\['a'\]\['exp_avg_sq'\] share memory"):
+        opt.step()
+    assert torch.equal(x, before)
+    c = torch.nn.Parameter(x[:599])
+    opt = AdamW([c, torch.nn.Parameter(x[599:])])            # (side by side)
+    for p in opt.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert not torch.equal(x[598:600], before[598:600]) and int(opt.state["0.1"]["step"]) == 1

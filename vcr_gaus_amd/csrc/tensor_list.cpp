@@ -6,6 +6,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 #include <ATen/core/Tensor.h>
+#include <algorithm>
+#include <vector>
 
 namespace {
 
@@ -147,6 +149,34 @@ PyObject* in_place(PyObject*, PyObject* args) {
     });
 }
 
+// sharing(list) -> None, or the indices of two contiguous tensors of the list that have memory in common: a launch over the list
+// would write it twice, in no order
+PyObject* sharing(PyObject*, PyObject* list) {
+    return guarded([&]() -> PyObject* {
+        if (!PyList_CheckExact(list)) { PyErr_SetString(PyExc_TypeError, "sharing: a list of tensors"); return nullptr; }
+        struct Range { uint64_t at, end; Py_ssize_t index; };
+        std::vector<Range> ranges;
+        const Py_ssize_t n = PyList_GET_SIZE(list);
+        ranges.reserve(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* o = PyList_GET_ITEM(list, i);
+            if (!THPVariable_Check(o)) { PyErr_SetString(PyExc_TypeError, "sharing: a list of tensors"); return nullptr; }
+            const at::Tensor& t = THPVariable_Unpack(o);
+            const uint64_t at_ = (uint64_t)(uintptr_t)t.const_data_ptr();
+            if (at_ && t.numel() > 0) ranges.push_back({at_, at_ + (uint64_t)t.numel() * t.element_size(), i});
+        }
+        std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.at < b.at; });
+        for (size_t k = 1, far = 0; k < ranges.size(); ++k) {               // `far`: the one so far that reaches furthest
+            if (ranges[k].at < ranges[far].end) {
+                const Py_ssize_t a = ranges[far].index, b = ranges[k].index;
+                return Py_BuildValue("nn", std::min(a, b), std::max(a, b));
+            }
+            if (ranges[k].end > ranges[far].end) far = k;
+        }
+        Py_RETURN_NONE;
+    });
+}
+
 // changed(list, words): the tensors (words: those whose 64-bit word in these bytes is not 0) have been written to behind torch's back:
 // their version counters move, so that a backward that needs the old values says so instead of using the new ones
 PyObject* changed(PyObject*, PyObject* args) {
@@ -171,6 +201,7 @@ PyObject* changed(PyObject*, PyObject* args) {
 
 PyMethodDef methods[] = {{"words", words, METH_O, nullptr}, {"gradients", gradients, METH_VARARGS, nullptr},
                          {"memory", memory, METH_O, nullptr}, {"in_place", in_place, METH_VARARGS, nullptr},
+                         {"sharing", sharing, METH_O, nullptr},
                          {"changed", changed, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_list", nullptr, -1, methods};
 

@@ -310,7 +310,7 @@ class AdamW:
         return self.master_weights and p.dtype != torch.float32
 
     def _check_state(self, key, p, st):
-        """-> the tensors of the parameter's state that a step reads and writes."""
+        """-> names of the tensors of the parameter's state that a step reads and writes."""
         n, nb = p.numel(), -(-p.numel() // BLOCK)
         want = {"step": (torch.int32, 1)}
         kind = torch.float32 if self.state_bits == 32 else torch.uint8
@@ -323,7 +323,7 @@ class AdamW:
             t = st.get(k)
             if not isinstance(t, torch.Tensor) or t.dtype != dt or t.numel() != m or t.device != p.device or not t.is_contiguous():
                 raise ValueError(f"AdamW: state[{key!r}][{k!r}] must be {m} contiguous elements of {dt} on {p.device}")
-        return [st[k] for k in want]
+        return list(want)
 
     def _build(self, identity, need):
         """Plan of all parameters that have a state, and of those in `need`, which get one.  `identity`: the native lists' words."""
@@ -339,21 +339,31 @@ class AdamW:
         if len(set(map(id, plan.params))) != len(plan.params):
             raise ValueError("AdamW: a parameter appears twice")
         self._check_dense(plan.params)
-        by, plan.state, plan.keep = {}, [], []
+        by, plan.state, plan.keep, names, stepped, fresh = {}, [], [], [], [], []
         for i, (p, key) in enumerate(zip(plan.params, keys)):
             if key not in self.state:
                 if i not in need:
                     continue
                 dict.__setitem__(self.state, key, self._fresh(p))
+                fresh.append(key)
             st = self.state[key]
             if type(st) is not _Watched:
                 st = _Watched(self, st)
                 dict.__setitem__(self.state, key, st)
             if self._has_master(p) and "master" not in st:
                 dict.__setitem__(st, "master", p.detach().float().contiguous())
-            plan.state += self._check_state(key, p, st)
+            held = self._check_state(key, p, st)
+            plan.state += [st[k] for k in held]
+            names += [f"state[{key!r}][{k!r}]" for k in held]
+            stepped.append(i)
             by.setdefault(_TYPES[p.dtype], []).append(i)
         plan.buckets, plan.covered = [], sum(map(len, by.values()))
+        twice = _native().sharing(plan.state + [plan.params[i] for i in stepped])
+        if twice:
+            names += [f"parameter {keys[i]!r}" for i in stepped]
+            for key in fresh:
+                dict.__delitem__(self.state, key)
+            raise ValueError(f"AdamW: {' and '.join(names[i] for i in twice)} share memory: one launch would write it twice, in no order")
         plan.memory = _native().memory(plan.state)
         for kind, at in by.items():
             b = _Bucket()
