@@ -299,3 +299,22 @@ def test_memory_that_a_step_would_write_twice_is_refused(device):
         p.grad = torch.ones_like(p)
     opt.step()
     assert not torch.equal(x[598:600], before[598:600]) and int(opt.state["0.1"]["step"]) == 1
+
+
+def test_clipping_refuses_what_it_cannot_scale_once(device):
+    """Gradients with memory in common, or expanded ones: refused with nothing written; other layouts are scaled as before."""
+    from vcr_gaus_amd.optim import clip_grad_norm_
+    ps = [torch.nn.Parameter(torch.zeros(6, device=device)) for _ in range(3)]
+    flat = torch.full((12,), 3.0, device=device)
+    ps[0].grad, ps[1].grad, ps[2].grad = flat[:6], torch.full((6,), 3.0, device=device), flat[5:11]
+    with pytest.raises(ValueError, match="gradients 0 and 2 share memory"):
+        clip_grad_norm_(ps, 1.0)
+    ps[2].grad = torch.full((1,), 3.0, device=device).expand(6)
+    with pytest.raises(ValueError, match="expanded"):
+        clip_grad_norm_(ps, 1.0)
+    assert bool((flat == 3).all()) and bool((ps[1].grad == 3).all()) and float(ps[2].grad[0]) == 3.0
+    ps[2].grad = torch.full((12,), 3.0, device=device)[::2]
+    norm = clip_grad_norm_(ps, 1.0)
+    assert abs(float(norm) - 3 * 18 ** 0.5) <= 2.0 ** -23 * float(norm)
+    for p in ps:                                       # (the factor's rounding and the product's)
+        assert float((p.grad - 18 ** -0.5).abs().max()) <= 3 * 2.0 ** -24

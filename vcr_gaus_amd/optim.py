@@ -124,6 +124,11 @@ def clip_grad_norm_(parameters, max_norm):
     if len(set(map(id, grads))) != len(grads):
         raise ValueError("clip_grad_norm_: a gradient appears twice")
     words = _List(grads, "gradients", "clip_grad_norm_")
+    if words.work is not grads and any(n > 1 and s == 0 for g in grads for n, s in zip(g.shape, g.stride())):
+        raise ValueError("clip_grad_norm_: an expanded gradient, whose elements share memory, cannot be scaled in place")
+    twice = _native().sharing(words.work)
+    if twice:
+        raise ValueError(f"clip_grad_norm_: gradients {twice[0]} and {twice[1]} share memory")
     dev = words.device
     norm, stream = torch.empty((), device=dev), _stream(dev.index)
 
