@@ -174,6 +174,9 @@ def test_native_lists_find_shared_memory():
                           ([x[10:20], x[30:40], x[:35]], (0, 2)), ([x, x[5:6], x[90:91]], (0, 1)), ([x[:0], x, x[50:50]], None),
                           ([x[20:40], x[:20].view(torch.bfloat16), x[40:].view(torch.uint8)], None), ([x[:21].view(torch.uint8), x[20:40]], (0, 1))):
         assert native.sharing(tensors) == want, want
+        for k in range(len(tensors) + 1):
+            assert native.sharing(tensors[:k], tensors[k:]) == want, want
+    assert native.sharing() is None
     for bad in ((x,), [x, 1]):
         with pytest.raises(TypeError):
-            native.sharing(bad)
+            native.sharing([x], bad)

@@ -318,3 +318,21 @@ def test_clipping_refuses_what_it_cannot_scale_once(device):
     assert abs(float(norm) - 3 * 18 ** 0.5) <= 2.0 ** -23 * float(norm)
     for p in ps:                                       # (the factor's rounding and the product's)
         assert float((p.grad - 18 ** -0.5).abs().max()) <= 3 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_refuse_outputs_that_share_memory(device, bits):
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([300, 5], F, device, seed=118)
+    opt = AdamW(params, state_bits=bits)
+    opt.step()
+    flat = torch.full((610,), 7.0, device=device)
+    m, v = [flat[:300], flat[300:305]], [flat[305:605], flat[605:]]
+    for lists, which in (((m, m), "0 and 2"), ((m, [flat[304:604], flat[605:]]), "1 and 2"), (([flat[:300], flat[295:300]], None), "0 and 1"),
+                         ((None, [flat[:300], flat[:5]]), "2 and 3")):
+        with pytest.raises(ValueError, match=f"outputs {which}"):
+            opt.moments(*lists)
+    assert bool((flat == 7).all())
+    opt.moments(m, v)
+    want = opt.moments()
+    assert all(torch.equal(a, b) for a, b in zip(m + v, want[0] + want[1]))

@@ -149,26 +149,34 @@ PyObject* in_place(PyObject*, PyObject* args) {
     });
 }
 
-// sharing(list) -> None, or the indices of two contiguous tensors of the list that have memory in common: a launch over the list
-// would write it twice, in no order
-PyObject* sharing(PyObject*, PyObject* list) {
+// sharing(lists...) -> None, or the numbers of two contiguous tensors, counted through all lists, that have memory in common: a launch
+// over them would write it twice, in no order
+PyObject* sharing(PyObject*, PyObject* lists) {
     return guarded([&]() -> PyObject* {
-        if (!PyList_CheckExact(list)) { PyErr_SetString(PyExc_TypeError, "sharing: a list of tensors"); return nullptr; }
-        struct Range { uint64_t at, end; Py_ssize_t index; };
+        struct Range { uint64_t at, end; Py_ssize_t number; };
         std::vector<Range> ranges;
-        const Py_ssize_t n = PyList_GET_SIZE(list);
-        ranges.reserve(n);
-        for (Py_ssize_t i = 0; i < n; ++i) {
-            PyObject* o = PyList_GET_ITEM(list, i);
-            if (!THPVariable_Check(o)) { PyErr_SetString(PyExc_TypeError, "sharing: a list of tensors"); return nullptr; }
-            const at::Tensor& t = THPVariable_Unpack(o);
-            const uint64_t at_ = (uint64_t)(uintptr_t)t.const_data_ptr();
-            if (at_ && t.numel() > 0) ranges.push_back({at_, at_ + (uint64_t)t.numel() * t.element_size(), i});
+        Py_ssize_t number = 0;
+        bool ascending = true;
+        for (Py_ssize_t l = 0; l < PyTuple_GET_SIZE(lists); ++l) {
+            PyObject* list = PyTuple_GET_ITEM(lists, l);
+            const Py_ssize_t n = PyList_CheckExact(list) ? PyList_GET_SIZE(list) : 0;
+            if (l == 0) ranges.reserve(n * PyTuple_GET_SIZE(lists));
+            bool good = PyList_CheckExact(list);
+            for (Py_ssize_t i = 0; good && i < n; ++i, ++number) {
+                PyObject* o = PyList_GET_ITEM(list, i);
+                if (!(good = THPVariable_Check(o))) break;
+                const at::Tensor& t = THPVariable_Unpack(o);
+                const uint64_t at_ = (uint64_t)(uintptr_t)t.const_data_ptr();
+                if (!at_ || t.numel() == 0) continue;
+                ascending = ascending && (ranges.empty() || at_ >= ranges.back().at);
+                ranges.push_back({at_, at_ + (uint64_t)t.numel() * t.element_size(), number});
+            }
+            if (!good) { PyErr_SetString(PyExc_TypeError, "sharing: lists of tensors"); return nullptr; }
         }
-        std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.at < b.at; });
+        if (!ascending) std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.at < b.at; });
         for (size_t k = 1, far = 0; k < ranges.size(); ++k) {               // `far`: the one so far that reaches furthest
             if (ranges[k].at < ranges[far].end) {
-                const Py_ssize_t a = ranges[far].index, b = ranges[k].index;
+                const Py_ssize_t a = ranges[far].number, b = ranges[k].number;
                 return Py_BuildValue("nn", std::min(a, b), std::max(a, b));
             }
             if (ranges[k].end > ranges[far].end) far = k;
@@ -201,7 +209,7 @@ PyObject* changed(PyObject*, PyObject* args) {
 
 PyMethodDef methods[] = {{"words", words, METH_O, nullptr}, {"gradients", gradients, METH_VARARGS, nullptr},
                          {"memory", memory, METH_O, nullptr}, {"in_place", in_place, METH_VARARGS, nullptr},
-                         {"sharing", sharing, METH_O, nullptr},
+                         {"sharing", sharing, METH_VARARGS, nullptr},
                          {"changed", changed, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_list", nullptr, -1, methods};
 

@@ -363,7 +363,7 @@ class AdamW:
             stepped.append(i)
             by.setdefault(_TYPES[p.dtype], []).append(i)
         plan.buckets, plan.covered = [], sum(map(len, by.values()))
-        twice = _native().sharing(plan.state + [plan.params[i] for i in stepped])
+        twice = _native().sharing(plan.state, [plan.params[i] for i in stepped])
         if twice:
             names += [f"parameter {keys[i]!r}" for i in stepped]
             for key in fresh:
@@ -517,25 +517,29 @@ class AdamW:
         """The moments as values, whatever they are held in: two lists, one tensor for each parameter in the groups' order.  Given
         lists are written to (contiguous, all of one type) instead of new tensors of `dtype`; a parameter that has not been stepped
         yet has zeros.  8-bit moments are exact in bfloat16."""
-        params = self._tensors()
-        outs = []
-        dtype = next((o[0].dtype for o in (exp_avgs, exp_avg_sqs) if o), dtype)
-        for given in (exp_avgs, exp_avg_sqs):
-            if given is None:
-                given = [torch.empty(p.shape, dtype=dtype, device=p.device) for p in params]
-            elif len(given) != len(params):
-                raise ValueError(f"moments: {len(given)} tensors for {len(params)} parameters")
-            outs.append(given)
+        params, native = self._tensors(), _native()
         n, none = len(params), bytes(len(params))
-        found = [_native().words(list(o)) for o in outs]          # device, words, their address
-        kind = None if None in found else found[0][1][16 * n:16 * n + 4]
-        if kind is None or any(f[1][16 * n:] != kind * n for f in found):
+        for given in (exp_avgs, exp_avg_sqs):
+            if given is not None:
+                dtype = given[0].dtype if len(given) else dtype
+                if len(given) != n:
+                    raise ValueError(f"moments: {len(given)} tensors for {n} parameters")
+        outs = [[torch.empty(p.shape, dtype=dtype, device=p.device) for p in params] if given is None else given
+                for given in (exp_avgs, exp_avg_sqs)]
+        lists = [o if type(o) is list else list(o) for o in outs]
+        a, c = found = [native.words(o) for o in lists]          # device, words, their address
+        kind = None if None in found else a[1][16 * n:16 * n + 4]
+        if kind is None or not a[1][16 * n:] == c[1][16 * n:] == kind * n:
             kinds = {t.dtype for o in outs for t in o}
             if len(kinds) != 1 or not kinds <= _TYPES.keys():
                 raise ValueError(f"moments: the outputs must be of one type among float32, bfloat16, float16: {kinds}")
-        plan, stream = self._current(params, (_native().gradients(params, none) or self._looked_at(params, none))[2], none)
-        if any(f is None or f[0] != plan.device.index or f[1][8 * n:16 * n] != plan.identity[16 * n:24 * n] for f in found):
+        plan, stream = self._current(params, (native.gradients(params, none) or self._looked_at(params, none))[2], none)
+        sizes = plan.identity[16 * n:24 * n]
+        if None in found or not (a[0] == c[0] == plan.device.index and a[1][8 * n:16 * n] == c[1][8 * n:16 * n] == sizes):
             raise ValueError("moments: an output has another size or device than its parameter, or is not contiguous")
+        twice = None if exp_avgs is exp_avg_sqs is None else native.sharing(*lists)
+        if twice:
+            raise ValueError(f"moments: outputs {twice[0]} and {twice[1]} (counted through both lists) share memory")
         if plan.covered < len(params):
             held = {i for b in plan.buckets for i in b.at}
             for i in range(len(params)):
@@ -551,11 +555,11 @@ class AdamW:
             kind = int.from_bytes(kind, sys.byteorder)
             for b in plan.buckets:
                 some = None if b.every else [array("Q", [o[i].data_ptr() for i in b.at]) for o in outs]
-                m, v = (f[2] for f in found) if b.every else map(_address, some)
+                m, v = (a[2], c[2]) if b.every else map(_address, some)
                 _lib.check(_on(plan.device, _lib.load().vcr_moments8_decode, b.n, b.plan.data_ptr(), _address(b.numels), m, v, kind, stream))
-            for given, o in zip((exp_avgs, exp_avg_sqs), outs):
+            for given, o in zip((exp_avgs, exp_avg_sqs), lists):
                 if given is not None:
-                    _native().changed(list(o), None)
+                    native.changed(o, None)
         return outs
 
     @torch.no_grad()
