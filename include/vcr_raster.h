@@ -282,7 +282,8 @@ typedef struct VcrAdamWStep {
     int32_t masters;          /* != 0: 16-bit parameters with fp32 masters */
     uint32_t seed;            /* of the stochastic rounding of 8-bit moments */
     void* plan;               /* device; the step keeps its tickets there */
-    const void* const* grads; /* HOST array of device pointers; NULL = this tensor is not stepped */
+    const void* const* grads; /* HOST array of device pointers; NULL = this tensor is not stepped (one without elements, of which
+                               * only the counter moves: any other value) */
     const int64_t* numel;     /* HOST, as in the plan */
     const int32_t* group_of;  /* HOST, as in the plan; ascending */
     const VcrOptimGroup* groups; /* HOST */

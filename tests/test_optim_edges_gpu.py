@@ -11,6 +11,10 @@ pytestmark = pytest.mark.gpu
 BF, HF, F = torch.bfloat16, torch.float16, torch.float32
 
 
+class Other(torch.Tensor):
+    """A tensor of another Python type."""
+
+
 def quiet_lanes(n, seed, late):
     """Gradients of three steps: ordinary ones; every fifth element has none in the first two, and `late` in the third."""
     g = torch.Generator().manual_seed(seed)
@@ -336,3 +340,41 @@ def test_moments_refuse_outputs_that_share_memory(device, bits):
     opt.moments(m, v)
     want = opt.moments()
     assert all(torch.equal(a, b) for a, b in zip(m + v, want[0] + want[1]))
+
+
+@pytest.mark.parametrize("bits, dtype, master", [(32, F, False), (8, F, False), (32, BF, True), (8, BF, True)])
+def test_counters_of_empty_tensors_move(device, bits, dtype, master):
+    """As torch.optim.AdamW's do: with a gradient, and only then; not in a skipped step; in a replayed one."""
+    from vcr_gaus_amd.optim import AdamW
+    params, _ = make([0, 5, 0, 4097], dtype, device, seed=119)
+    opt = AdamW(params, state_bits=bits, master_weights=master)
+    steps = lambda: [int(opt.state[f"0.{k}"]["step"]) for k in range(4)]  # noqa: E731
+    opt.step()
+    opt.step(max_norm=1.0)
+    assert steps() == [2, 2, 2, 2]
+    params[0].grad = None
+    opt.step()
+    assert steps() == [2, 3, 3, 3]
+    params[0].grad = torch.zeros(0, dtype=dtype, device=device).as_subclass(Other)          # (not an ordinary list)
+    keep = params[1].grad.clone()
+    params[1].grad.fill_(float("nan"))
+    opt.step(max_norm=1.0)
+    assert steps() == [2, 3, 3, 3]
+    params[1].grad = keep
+    opt.step()
+    assert steps() == [3, 4, 4, 4]
+    params[0].grad = torch.zeros(0, dtype=dtype, device=device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert steps() == [4 + k, 5 + k, 5 + k, 5 + k]
+    m, v = opt.moments()
+    assert m[0].shape == (0,) and bool(torch.isfinite(m[3]).all())
+    only = AdamW([params[0]], state_bits=bits, master_weights=master)
+    only.step(max_norm=1.0)
+    only.step()
+    assert int(only.state["0"]["step"]) == 2

@@ -331,7 +331,7 @@ __device__ __forceinline__ bool last_of(GLOBAL uint32_t* word, uint32_t of) {
 }
 template <int ROUNDS> __device__ __forceinline__ void leave(const VcrOptimTensor& R, uint32_t* words, const Place& at, int step) {
     if (threadIdx.x != 0) return;
-    const uint32_t nchunks = (uint32_t)((R.numel + VCR_OPT_CHUNK - 1) / VCR_OPT_CHUNK), n = nchunks * parts<ROUNDS>();
+    const uint32_t nchunks = R.numel ? (uint32_t)((R.numel + VCR_OPT_CHUNK - 1) / VCR_OPT_CHUNK) : 1u, n = nchunks * parts<ROUNDS>();
     bool last = true;
     if (n > 1) {
         GLOBAL uint32_t* w = global(words) + (size_t)R.words * TICKET_STRIDE;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw_kernel(const VcrOptimTe
     if (!g || (clip && clip->skip)) return;
     const VcrOptimTensor& R = tensors[at.tensor];
     const uint32_t group = (uint32_t)(R.group - g0);
-    if (group >= VCR_OPT_GROUPS || R.m_scale || (MASTER && !R.master)) return;             // (a plan that was made for another call)
+    if (group >= VCR_OPT_GROUPS || R.m_scale || (MASTER && !R.master && R.numel)) return;             // (a plan that was made for another call)
     const float gs = clip ? clip->gscale : gscale;
     const long long off = at.first + threadIdx.x * 4, left = R.numel - off;
     GLOBAL T* p = global((T*)R.p) + off;
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimT
     if (!grad || (clip && clip->skip)) return;
     const VcrOptimTensor& R = tensors[at.tensor];
     const uint32_t group = (uint32_t)(R.group - g0);
-    if (group >= VCR_OPT_GROUPS || !R.m_scale || (MASTER && !R.master)) return;       // (a plan that was made for another call)
+    if (group >= VCR_OPT_GROUPS || ((!R.m_scale || (MASTER && !R.master)) && R.numel)) return;       // (a plan that was made for another call)
     const float gs = clip ? clip->gscale : gscale;
     const Entry e = enter(R, pk.group[group]);
     const Fast fast = fast_of(e.coef);
@@ -740,6 +740,8 @@ __global__ void __launch_bounds__(256) encode_kernel(const VcrOptimTensor* __res
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
 inline int64_t chunks_of(int64_t numel, int64_t chunk) { return (numel + chunk - 1) / chunk; }
+// entries of a plan: a tensor without elements has one too, for its counter
+inline int64_t entries_of(int64_t numel) { return numel > 0 ? chunks_of(numel, VCR_OPT_CHUNK) : 1; }
 inline size_t plan_head(int n) { return vcr_align(sizeof(VcrOptimTensor) * (size_t)n); }
 inline size_t plan_words(int n, int64_t chunks) { return vcr_align(plan_head(n) + sizeof(uint2) * (size_t)chunks); }
 inline uint32_t tickets_of(int64_t chunks) { return chunks > TICKET_FLAT ? 1 + TICKET_GROUPS : 1; }
@@ -751,8 +753,8 @@ int64_t plan_check(const char* who, const void* plan, int n, const int64_t* nume
     int64_t total = 0;
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0) { vcr_set_error("%s: tensor %d has numel %lld", who, k, (long long)numel[k]); return -1; }
-        if (chunks_of(numel[k], VCR_OPT_CHUNK) > VCR_OPT_LAUNCH_CHUNKS) { vcr_set_error("%s: tensor %d with %lld elements is too large", who, k, (long long)numel[k]); return -1; }
-        total += chunks_of(numel[k], VCR_OPT_CHUNK);
+        if (entries_of(numel[k]) > VCR_OPT_LAUNCH_CHUNKS) { vcr_set_error("%s: tensor %d with %lld elements is too large", who, k, (long long)numel[k]); return -1; }
+        total += entries_of(numel[k]);
     }
     if (total > 0x0FFFFFFF) { vcr_set_error("%s: %lld chunks", who, (long long)total); return -1; }
     return total;
@@ -802,7 +804,7 @@ extern "C" size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel) {
     int64_t total = 0;
     size_t tickets = 0;
     for (int k = 0; k < ntensors; ++k) {
-        const int64_t nc = numel[k] > 0 ? chunks_of(numel[k], VCR_OPT_CHUNK) : 0;
+        const int64_t nc = entries_of(numel[k]);
         total += nc;
         tickets += tickets_of(nc);
     }
@@ -819,8 +821,8 @@ extern "C" int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, void*
             vcr_set_error("vcr_optim_plan: tensor %d has numel %lld and a pointer missing", k, (long long)t.numel);
             return 1;
         }
-        total += chunks_of(t.numel, VCR_OPT_CHUNK);
-        tickets += tickets_of(chunks_of(t.numel, VCR_OPT_CHUNK));
+        total += entries_of(t.numel);
+        tickets += tickets_of(entries_of(t.numel));
     }
     const size_t words = plan_words(ntensors, total), need = words + tickets * TICKET_STRIDE * sizeof(uint32_t);
     if (total > 0x0FFFFFFF || tickets > 0x7FFFFFFF || bytes < need) { vcr_set_error("vcr_optim_plan: %zu bytes for %lld chunks", bytes, (long long)total); return 1; }
@@ -828,7 +830,7 @@ extern "C" int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, void*
     uint2* c = (uint2*)((char*)host_plan + plan_head(ntensors));
     int32_t word = 0;
     for (int k = 0; k < ntensors; ++k) {
-        const uint32_t nc = (uint32_t)chunks_of(tensors[k].numel, VCR_OPT_CHUNK);
+        const uint32_t nc = (uint32_t)entries_of(tensors[k].numel);
         out[k] = tensors[k];
         out[k].words = word;
         word += (int32_t)tickets_of(nc);
@@ -872,11 +874,11 @@ extern "C" int vcr_adamw_step(const VcrAdamWStep* args, void* stream) {
         bool any = false;
         const int g0 = a.group_of[t0];
         for (; t1 < a.ntensors && t1 - t0 < VCR_OPT_TENSORS && a.group_of[t1] - g0 < VCR_OPT_GROUPS; ++t1) {
-            const int64_t c = chunks_of(a.numel[t1], VCR_OPT_CHUNK);
+            const int64_t c = entries_of(a.numel[t1]);
             if (nchunks + c > VCR_OPT_LAUNCH_CHUNKS) break;
             pk.g[t1 - t0] = a.grads[t1];
             nchunks += c;
-            any |= a.grads[t1] != nullptr && a.numel[t1] > 0;
+            any |= a.grads[t1] != nullptr;
         }
         for (int k = g0; k <= a.group_of[t1 - 1]; ++k) {
             const VcrOptimGroup& g = a.groups[k];
@@ -913,7 +915,7 @@ static int pairs_call(const char* who, int n, const void* plan, const int64_t* n
         PairPack pk = {};
         int64_t nchunks = 0;
         for (; t1 < n && t1 - t0 < VCR_OPT_PAIRS; ++t1) {
-            const int64_t c = chunks_of(numel[t1], VCR_OPT_CHUNK);
+            const int64_t c = entries_of(numel[t1]);
             if (nchunks + c > VCR_OPT_LAUNCH_CHUNKS) break;
             pk.a[t1 - t0] = a[t1];
             pk.b[t1 - t0] = b[t1];

@@ -58,7 +58,7 @@ PyObject* words(PyObject*, PyObject* list) {
 }
 
 // gradients(params, flags) -> None or (device index, how many have a gradient, bytes, address of the bytes): n addresses of the
-// gradients (0: none, or its byte in `flags` is 0), and what identifies the parameters: n objects, addresses, sizes, kinds.
+// gradients (0: none, or its byte in `flags` is 0; 1: one without elements), and what identifies the parameters: n objects, addresses, sizes, kinds.
 // Every gradient is of its parameter's type, size and device.
 PyObject* gradients(PyObject*, PyObject* args) {
     return guarded([&]() -> PyObject* {
@@ -93,8 +93,8 @@ PyObject* gradients(PyObject*, PyObject* args) {
                 const at::Tensor& g = t->grad();
                 if (g.defined() && (!wanted || wanted[i])) {
                     good = kind_of(g) == k && g.numel() == numel[i] && g.device().index() == device;
-                    if (good) { grad[i] = (uint64_t)(uintptr_t)g.const_data_ptr(); ++live; }
-                    good = good && (grad[i] || numel[i] == 0);
+                    if (good) { grad[i] = numel[i] ? (uint64_t)(uintptr_t)g.const_data_ptr() : 1; ++live; }
+                    good = good && grad[i];
                 }
             }
             if (!good) Py_RETURN_NONE;

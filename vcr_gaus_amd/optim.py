@@ -471,8 +471,8 @@ class AdamW:
             if g.dtype is not dtypes[i] or g.numel() != params[i].numel() or g.device != dev:
                 raise ValueError(f"AdamW: the gradient of {self._keys()[i]!r} has type {g.dtype} and {g.numel()} elements on {g.device}, "
                                  f"the parameter {dtypes[i]} and {params[i].numel()} on {dev}")
-            grads[i] = g.data_ptr()
-            if not grads[i] and g.numel():
+            grads[i] = g.data_ptr() if g.numel() else 1
+            if not grads[i]:
                 raise ValueError(f"AdamW: the gradient of {self._keys()[i]!r} has no memory")
         words = b"".join(a.tobytes() for a in (grads, array("Q", map(id, params)), array("Q", [p.data_ptr() for p in params]),
                                                array("q", [p.numel() for p in params]), array("i", [_TYPES[d] for d in dtypes])))
