@@ -1,8 +1,10 @@
 """What of `vcr_gaus_amd.optim`'s rarer calls needs no device."""
 import copy
+import ctypes as C
 import gc
 import pickle
 import weakref
+from array import array
 
 import pytest
 import torch
@@ -180,3 +182,28 @@ def test_native_lists_find_shared_memory():
     for bad in ((x,), [x, 1]):
         with pytest.raises(TypeError):
             native.sharing([x], bad)
+
+
+@pytest.mark.parametrize("huge", [2 ** 63 - 1, 2 ** 62, 4096 * 4194303 + 1])
+def test_c_entries_refuse_tensors_that_no_launch_can_hold(huge):
+    """With a reason, and before anything reaches a device; the largest sizes overflow no sum on the way."""
+    lib = _lib.load()
+    word = lambda kind, *v: (lambda a: (a, a.buffer_info()[0]))(array(kind, v))  # noqa: E731
+    (_n, numel), (_p, ptrs), (_k, kinds), (_g, group_of) = word("q", 8, huge, huge), word("Q", *[4096] * 3), word("i", 0, 0, 0), word("i", 0, 0, 0)
+    groups = (_lib.VcrOptimGroup * 1)(_lib.VcrOptimGroup(1e-3, 0.9, 0.999, 1e-8, 0.0, None))
+    step = _lib.VcrAdamWStep(ntensors=3, ngroups=1, state_bits=32, plan=4096, grads=ptrs, numel=numel, group_of=group_of, groups=groups)
+    rec = (_lib.VcrOptimTensor * 3)()
+    for r, n in zip(rec, (8, huge, huge)):
+        r.p = r.m = r.v = r.step = 4096
+        r.numel = n
+    host = C.create_string_buffer(4096)
+    assert lib.vcr_optim_plan_bytes(3, numel) == 0
+    calls = [lambda: lib.vcr_adamw_step(C.byref(step), None), lambda: lib.vcr_optim_plan(3, rec, C.addressof(host), 4096),
+             lambda: lib.vcr_moments8_decode(3, 4096, numel, ptrs, ptrs, 0, None), lambda: lib.vcr_moments8_encode(3, 4096, numel, ptrs, ptrs, None)]
+    if huge > 2 ** 45:                                  # (the norm takes more: 16 384 elements a piece, 2^31 - 1 pieces)
+        calls += [lambda: lib.vcr_grad_norm(3, ptrs, numel, kinds, 4096, 1 << 20, 1.0, 1.0, 0, 4096, None, None),
+                  lambda: lib.vcr_clip_gradients(3, ptrs, numel, kinds, 4096, 1.0, None)]
+        assert 0 < lib.vcr_grad_norm_partials(3, numel) < 10000
+    for call in calls:
+        _lib.load().vcr_adamw_step(None, None)          # (another error in between)
+        assert call() == 1 and "tensor 1 with" in _lib.last_error() and "too large" in _lib.last_error()

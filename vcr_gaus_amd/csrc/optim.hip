@@ -37,6 +37,7 @@ namespace {
 // The norm's workgroups stride over chunks (800 M fp32 elements: 459 us with 1024 workgroups, 469 with 2048, 468 with 4096).
 #define VCR_OPT_NORM_BLOCKS 1024
 #define NORM_CHUNK 16384
+#define NORM_LAUNCH_CHUNKS 0x7FFFFFFF      // of one tensor, and of one launch
 // Up to this many chunks in all, of one type: one workgroup and one launch (64 K fp32 elements, 4 chunks: 8.9 instead of 11.8 us from
 // Python, 4.8 us either way in a captured graph; 8 chunks 8.9 instead of 12.0, but 8.5 instead of 4.9 captured).
 #define VCR_OPT_NORM_ONE 4
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(256) encode_kernel(const VcrOptimTensor* __res
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
-inline int64_t chunks_of(int64_t numel, int64_t chunk) { return (numel + chunk - 1) / chunk; }
+inline int64_t chunks_of(int64_t numel, int64_t chunk) { return numel / chunk + (numel % chunk != 0); }          // (no overflow)
 // entries of a plan: a tensor without elements has one too, for its counter
 inline int64_t entries_of(int64_t numel) { return numel > 0 ? chunks_of(numel, VCR_OPT_CHUNK) : 1; }
 inline size_t plan_head(int n) { return vcr_align(sizeof(VcrOptimTensor) * (size_t)n); }
@@ -772,16 +773,13 @@ int each_norm_pack(int n, const void* const* tensors, const int64_t* numel, cons
         for (; k < n && used < VCR_OPT_NORM_TENSORS; ++k) {
             if (numel[k] == 0 || types[k] != type) continue;
             const int64_t c = chunks_of(numel[k], NORM_CHUNK);
-            if (start + c > 0x7FFFFFFF) break;
+            if (start + c > NORM_LAUNCH_CHUNKS) break;
             pk.g[used] = tensors[k];
             pk.n[used] = numel[k];
             start += c;
             pk.start[++used] = (uint32_t)start;
         }
-        if (used == 0) {
-            if (k < n) { vcr_set_error("tensor %d with %lld elements is too large", k, (long long)numel[k]); return 1; }
-            break;
-        }
+        if (used == 0) break;
         if (launch(pk, used, (uint32_t)start)) return 1;
     }
     return 0;
@@ -789,11 +787,13 @@ int each_norm_pack(int n, const void* const* tensors, const int64_t* numel, cons
 
 int list_check(const char* who, int n, const void* const* tensors, const int64_t* numel, const int32_t* types) {
     if (n < 0 || (n > 0 && (!tensors || !numel || !types))) { vcr_set_error("%s: the list of tensors is missing", who); return 1; }
-    for (int k = 0; k < n; ++k)
+    for (int k = 0; k < n; ++k) {
         if (numel[k] < 0 || (numel[k] > 0 && !tensors[k]) || types[k] < 0 || types[k] > VCR_F16) {
             vcr_set_error("%s: tensor %d has numel %lld, pointer %p, type %d", who, k, (long long)numel[k], tensors[k], types[k]);
             return 1;
         }
+        if (chunks_of(numel[k], NORM_CHUNK) > NORM_LAUNCH_CHUNKS) { vcr_set_error("%s: tensor %d with %lld elements is too large", who, k, (long long)numel[k]); return 1; }
+    }
     return 0;
 }
 
@@ -805,6 +805,7 @@ extern "C" size_t vcr_optim_plan_bytes(int ntensors, const int64_t* numel) {
     size_t tickets = 0;
     for (int k = 0; k < ntensors; ++k) {
         const int64_t nc = entries_of(numel[k]);
+        if (nc > VCR_OPT_LAUNCH_CHUNKS) return 0;          // (vcr_optim_plan says why)
         total += nc;
         tickets += tickets_of(nc);
     }
@@ -821,6 +822,7 @@ extern "C" int vcr_optim_plan(int ntensors, const VcrOptimTensor* tensors, void*
             vcr_set_error("vcr_optim_plan: tensor %d has numel %lld and a pointer missing", k, (long long)t.numel);
             return 1;
         }
+        if (entries_of(t.numel) > VCR_OPT_LAUNCH_CHUNKS) { vcr_set_error("vcr_optim_plan: tensor %d with %lld elements is too large", k, (long long)t.numel); return 1; }
         total += entries_of(t.numel);
         tickets += tickets_of(entries_of(t.numel));
     }
@@ -949,7 +951,10 @@ extern "C" int vcr_moments8_encode(int ntensors, const void* plan, const int64_t
 extern "C" int vcr_grad_norm_partials(int ntensors, const int64_t* numel) {
     if (ntensors < 1 || !numel) return 1;
     int64_t chunks = 0;
-    for (int k = 0; k < ntensors; ++k) chunks += numel[k] > 0 ? chunks_of(numel[k], NORM_CHUNK) : 0;
+    for (int k = 0; k < ntensors; ++k) {
+        const int64_t c = numel[k] > 0 ? chunks_of(numel[k], NORM_CHUNK) : 0;
+        if (c <= NORM_LAUNCH_CHUNKS) chunks += c;          // (a larger one is refused by vcr_grad_norm)
+    }
     const int64_t packs = ntensors / VCR_OPT_NORM_TENSORS + 3 + chunks / 0x40000000;     // (a pack ends with its type)
     const int64_t most = packs * VCR_OPT_NORM_BLOCKS;
     return (int)(chunks < most ? chunks + 1 : most);
