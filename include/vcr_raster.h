@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define VCR_ABI_VERSION 20
+#define VCR_ABI_VERSION 21
 
 /* Buffers whose size depends on the number of tile instances R are obtained through this callback
  * (the Python shim backs it with torch's caching allocator, so no hipMalloc on the hot path).
@@ -302,6 +302,15 @@ int vcr_moments8_decode(int ntensors, const void* plan, const int64_t* numel, vo
                         void* const* exp_avg_sq, int type, void* stream);
 int vcr_moments8_encode(int ntensors, const void* plan, const int64_t* numel, const float* const* exp_avg,
                         const float* const* exp_avg_sq, void* stream);
+/* Rows of 8-bit moments in another order (prune, append): row r of the outputs is row index[r] (device, rows_out numbers) of the
+ * inputs, zeros where that is not in 0 ... rows_in - 1.  Blocks are formed anew, values rounded to the nearest code.  Inputs and
+ * outputs must not overlap. */
+typedef struct VcrRows8 {
+    const uint8_t *m, *v, *m_scale, *v_scale;            /* codes [rows_in, width], exponents of their blocks */
+    uint8_t *m_out, *v_out, *m_scale_out, *v_scale_out;  /* codes [rows_out, width], exponents */
+    int32_t width, pad;
+} VcrRows8;
+int vcr_moments8_rows(int narrays, const VcrRows8* arrays, int64_t rows_in, int64_t rows_out, const int32_t* index, void* stream);
 /* 2-norm over all tensors, mixed types (HOST arrays): *norm = sqrt(sum of squares) * |grad_scale|, and with `clip` (8 bytes on the
  * device) the factor grad_scale * min(1, max_norm / (norm + 1e-6)) of a clipped step, which is skipped if the norm is not finite.
  * `partials`: scratch for `capacity` >= vcr_grad_norm_partials(ntensors, numel) doubles.  `read_again` != 0: the tensors are read

@@ -11,7 +11,7 @@ import torch
 
 from vcr_gaus_amd import _lib
 from vcr_gaus_amd.gaussian_model import FusedAdam, GaussianAdamW
-from vcr_gaus_amd.optim import AdamW, decode8, encode8
+from vcr_gaus_amd.optim import AdamW, decode8, encode8, rows8
 
 
 def P(*shape):
@@ -207,3 +207,28 @@ def test_c_entries_refuse_tensors_that_no_launch_can_hold(huge):
     for call in calls:
         _lib.load().vcr_adamw_step(None, None)          # (another error in between)
         assert call() == 1 and "tensor 1 with" in _lib.last_error() and "too large" in _lib.last_error()
+
+
+def test_rows_of_codes_are_checked():
+    lib = _lib.load()
+    st = {k: torch.zeros((100, 3) if "scale" not in k else 2, dtype=torch.uint8) for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
+    index = torch.zeros(5, dtype=torch.int32)
+    for bad in (index.long(), index.view(5, 1), torch.zeros(10, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="index"):
+            rows8([st], bad)
+    for bad in (dict(st, exp_avg_sq=st["exp_avg_sq"].view(300)), dict(st, exp_avg=st["exp_avg"].view(3, 100))):
+        with pytest.raises(ValueError, match="rows"):
+            rows8([st, bad] if bad["exp_avg"].shape != (100, 3) else [bad], index)
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        rows8([dict(st, exp_avg_scale=torch.zeros(1, dtype=torch.uint8))], index)
+    with pytest.raises(ValueError, match="HIP device"):
+        rows8([st], index)
+    arr = lambda width, **kw: (_lib.VcrRows8 * 1)(_lib.VcrRows8(width=width, **dict(  # noqa: E731
+        dict.fromkeys(("m", "v", "m_scale", "v_scale", "m_out", "v_out", "m_scale_out", "v_scale_out"), 4096), **kw)))
+    for args, msg in (((-1, None, 1, 1, 4096, None), "inconsistent"), ((1, None, 1, 1, 4096, None), "inconsistent"),
+                      ((1, arr(3), -1, 1, 4096, None), "inconsistent"), ((1, arr(3), 1, 1, None, None), "inconsistent"),
+                      ((1, arr(0), 1, 1, 4096, None), "width 0"), ((1, arr(3), 2 ** 62, 1, 4096, None), "width 3"),
+                      ((1, arr(3), 1, 2 ** 34, 4096, None), "width 3"), ((1, arr(3, v=None), 1, 1, 4096, None), "pointer"),
+                      ((1, arr(3, m_scale_out=None), 0, 1, 4096, None), "pointer")):
+        assert lib.vcr_moments8_rows(*args) == 1 and msg in _lib.last_error(), (args, _lib.last_error())
+    assert lib.vcr_moments8_rows(1, arr(3, m_out=None), 7, 0, None, None) == 0 and lib.vcr_moments8_rows(0, None, 0, 0, None, None) == 0

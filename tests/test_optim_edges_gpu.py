@@ -378,3 +378,74 @@ def test_counters_of_empty_tensors_move(device, bits, dtype, master):
     only.step(max_norm=1.0)
     only.step()
     assert int(only.state["0"]["step"]) == 2
+
+
+@pytest.mark.parametrize("width", [1, 3, 45, 257])
+def test_rows_of_8_bit_moments(device, width):
+    """Rows kept, repeated, appended as zeros and out of range, from and to any number of rows: the codes of the moved values, to the
+    nearest, by the definition; nothing beside the outputs is written, and the inputs stay."""
+    from vcr_gaus_amd.optim import rows8
+    rng = np.random.default_rng(width)
+    for rows_in, rows_out in ((1, 1), (300, 200), (513, 1000), (7, 0), (0, 5), (1000, 1)):
+        shapes = [(rows_in, width), (rows_in, 1, 3)]
+        states, host_states = [], []
+        for shape in shapes:
+            n = int(np.prod(shape))
+            nb = -(-n // R.BLOCK)
+            h = dict(exp_avg=rng.integers(0, 256, n, dtype=np.uint8), exp_avg_sq=rng.integers(0, 255, n, dtype=np.uint8),
+                     exp_avg_scale=rng.integers(90, 130, nb, dtype=np.uint8), exp_avg_sq_scale=rng.integers(60, 120, nb, dtype=np.uint8))
+            host_states.append(h)
+            states.append({k: torch.from_numpy(x.copy()).to(device).view(shape if "scale" not in k else -1) for k, x in h.items()})
+        index = rng.integers(-2, rows_in + 2, rows_out).astype(np.int32)
+        index[::5] = -1
+        out = rows8(states, torch.from_numpy(index).to(device))
+        good = (index >= 0) & (index < rows_in)
+        for shape, h, st, o in zip(shapes, host_states, states, out):
+            per = int(np.prod(shape[1:]))
+            assert o["exp_avg"].shape == (rows_out, *shape[1:])
+            for signed, c, s in ((True, "exp_avg", "exp_avg_scale"), (False, "exp_avg_sq", "exp_avg_sq_scale")):
+                x = np.zeros((rows_out, per), np.float32)
+                x[good] = R.decode(h[c], h[s], signed).reshape(rows_in, per)[index[good]]
+                want = R.encode(x.reshape(-1), R.nearest, signed)
+                assert np.array_equal(o[c].cpu().numpy().reshape(-1), want[0]) and np.array_equal(o[s].cpu().numpy(), want[1]), (rows_in, rows_out)
+                assert np.array_equal(st[c].cpu().numpy().reshape(-1), h[c]) and np.array_equal(st[s].cpu().numpy(), h[s])
+
+
+def test_row_surgery_does_not_expand_8_bit_moments(device):
+    """Prune and append of 100 000 Gaussians: on top of what is held, the new parameters (4 bytes a value), the new codes and scales
+    (2.01) and 64 bytes a row of masks, plans and indices at most; values and counters as the 32-bit form's surgery would leave them."""
+    from tests.test_optim_gpu import GROUPS, adamw_trainer
+    tr = adamw_trainer(device, state_bits=8)
+    tr.train_step()
+    m, opt = tr.model, tr.model.optimizer
+    with torch.no_grad():
+        m._append_selected(torch.ones(m._xyz.shape[0], dtype=torch.bool, device=device), copies=39)
+    n = m._xyz.shape[0]
+    assert n == 100_000
+    for g in opt.param_groups:                       # (moments that differ from row to row)
+        p = g["params"][0]
+        x = torch.randn(p.shape, device=device, generator=torch.Generator(device=device).manual_seed(p.numel()))
+        opt.set_moments(g["name"], x, x.square())
+    floats = sum(opt.state[k]["exp_avg"][0].numel() for k in GROUPS)
+    keep = torch.arange(n, device=device) % 7 != 0
+    rows = int(keep.sum())
+    before = {k: opt.moments_of(k) for k in GROUPS}
+    steps = {k: int(opt.state[k]["step"]) for k in GROUPS}
+    for what, new in ((lambda: m.prune_points(~keep), rows), (lambda: m._append_selected(torch.arange(rows, device=device) < 5000, copies=2), rows + 10_000)):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats(device)
+        held = torch.cuda.memory_allocated(device)
+        with torch.no_grad():
+            what()
+        extra = torch.cuda.max_memory_allocated(device) - held
+        assert extra <= new * (floats * (4 + 2 + 2 / 256) + 64) + (1 << 20), (extra, new * floats)
+    for k in GROUPS:
+        for old, got, low in zip(before[k], opt.moments_of(k), (2.0 ** -17, 2.0 ** -33)):
+            want = old[keep].reshape(-1)
+            flat = got.reshape(-1)
+            top = torch.nn.functional.pad(flat.abs(), (0, -flat.numel() % 256)).view(-1, 256).amax(1).repeat_interleave(256)[:want.numel()]
+            assert bool(((flat[:want.numel()] - want).abs() <= 2 * top * low).all()), k
+            assert got.shape[0] == rows + 10_000 and float(got[rows:].abs().sum()) == 0
+        assert int(opt.state[k]["step"]) == steps[k]
+    tr.train_step()
+    assert int(opt.state["xyz"]["step"]) == steps["xyz"] + 1

@@ -16,7 +16,7 @@ c_int_p = C.POINTER(C.c_int32)
 ALLOC_FN = C.CFUNCTYPE(C.c_void_p, C.c_void_p, C.c_int32, C.c_size_t)
 HOOK_FN = C.CFUNCTYPE(None, C.c_void_p)
 BUF_GEOM, BUF_BINNING, BUF_IMAGE, BUF_SCRATCH = 0, 1, 2, 3
-ABI_VERSION = 20         # VCR_ABI_VERSION of include/vcr_raster.h this binding was written against
+ABI_VERSION = 21         # VCR_ABI_VERSION of include/vcr_raster.h this binding was written against
 
 
 class VcrShUpdate(C.Structure):
@@ -42,6 +42,11 @@ class VcrAdamWStep(C.Structure):
                [("seed", C.c_uint32), ("plan", C.c_void_p), ("grads", C.c_void_p),
                 ("numel", C.c_void_p), ("group_of", C.c_void_p), ("groups", C.POINTER(VcrOptimGroup)),
                 ("grad_scale", C.c_double), ("clip", C.c_void_p)]
+
+
+class VcrRows8(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("m", "v", "m_scale", "v_scale", "m_out", "v_out", "m_scale_out", "v_scale_out")] + \
+               [("width", C.c_int32), ("pad", C.c_int32)]
 
 
 class VcrGeometryStep(C.Structure):
@@ -140,6 +145,7 @@ SYMBOLS = {
     "vcr_adamw_step": (C.c_int, [C.POINTER(VcrAdamWStep), C.c_void_p]),
     "vcr_moments8_decode": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_void_p]),
     "vcr_moments8_encode": (C.c_int, [C.c_int] + [C.c_void_p] * 5),
+    "vcr_moments8_rows": (C.c_int, [C.c_int, C.POINTER(VcrRows8), C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
     "vcr_grad_norm_partials": (C.c_int, [C.c_int, C.c_void_p]),
     "vcr_grad_norm": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_int, C.c_double, C.c_double, C.c_int] + [C.c_void_p] * 3),
     "vcr_clip_gradients": (C.c_int, [C.c_int] + [C.c_void_p] * 4 + [C.c_double, C.c_void_p]),

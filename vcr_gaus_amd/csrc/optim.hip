@@ -708,35 +708,63 @@ __device__ __forceinline__ uint32_t nearest_v(float v, int s) {
     const uint32_t y = __float_as_uint(ldexpf(fabsf(v), V_TOP - s));
     return encode_v(v, s, 0x7FFFFu + (y >> 20 & 1u));
 }
+// One block of 256 values, four of them 64 apart in each lane, as codes and exponents.
+__device__ __forceinline__ void encode_block(const float (&m)[4], const float (&v)[4], long long blk, uint32_t lane, long long numel,
+                                             GLOBAL uint8_t* mc, GLOBAL uint8_t* vc, GLOBAL uint8_t* ms, GLOBAL uint8_t* vs) {
+    uint32_t mb = 0, vb = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { mb = max(mb, finite_bits(m[k])); vb = max(vb, finite_bits(v[k])); }
+    const int nm = scale_of(rows_max(row_max(mb))), nv = scale_of(rows_max(row_max(vb)));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const long long i = blk * VCR_OPT_BLOCK + lane + 64 * k;
+        if (i < numel) { mc[i] = (uint8_t)nearest_m(m[k], nm); vc[i] = (uint8_t)nearest_v(v[k], nv); }
+    }
+    if (lane == 0) { ms[blk] = (uint8_t)nm; vs[blk] = (uint8_t)nv; }
+}
 __global__ void __launch_bounds__(256) encode_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,
                                                      PairPack in, int t0) {
     const uint2 cw = chunks[blockIdx.x];
     const VcrOptimTensor& R = tensors[cw.x];
     if (!R.m_scale) return;
     const GLOBAL float *mi = global((const float*)in.a[cw.x - t0]), *vi = global((const float*)in.b[cw.x - t0]);
-    GLOBAL uint8_t *mc = global((uint8_t*)R.m), *vc = global((uint8_t*)R.v);
     const uint32_t lane = threadIdx.x & 63;
     for (uint32_t b = threadIdx.x >> 6; b < VCR_OPT_CHUNK / VCR_OPT_BLOCK; b += 4) {
         const long long blk = (long long)cw.y * (VCR_OPT_CHUNK / VCR_OPT_BLOCK) + b, first = blk * VCR_OPT_BLOCK + lane;
         if (blk * VCR_OPT_BLOCK >= R.numel) break;
         float m[4], v[4];
-        uint32_t mb = 0, vb = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const long long i = first + 64 * k;
             m[k] = i < R.numel ? mi[i] : 0.f;
             v[k] = i < R.numel ? vi[i] : 0.f;
-            mb = max(mb, finite_bits(m[k]));
-            vb = max(vb, finite_bits(v[k]));
         }
-        const int nm = scale_of(rows_max(row_max(mb))), nv = scale_of(rows_max(row_max(vb)));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const long long i = first + 64 * k;
-            if (i < R.numel) { mc[i] = (uint8_t)nearest_m(m[k], nm); vc[i] = (uint8_t)nearest_v(v[k], nv); }
-        }
-        if (lane == 0) { global(R.m_scale)[blk] = (uint8_t)nm; global(R.v_scale)[blk] = (uint8_t)nv; }
+        encode_block(m, v, blk, lane, R.numel, global((uint8_t*)R.m), global((uint8_t*)R.v), global(R.m_scale), global(R.v_scale));
     }
+}
+
+// Rows of 8-bit moments in another order: row r of the output is row index[r] of the input, zeros where that is no row.  One wave per
+// block of the output, whose exponents are formed anew from the values that land in it; four elements per lane, gathered one by one
+// (a row is shorter than a block, and begins anywhere).  Read and written are codes: expanded to fp32 and back the moments would
+// take 16 bytes a parameter on the way instead of 4, more than a caller who chose 8 bits has.
+__global__ void __launch_bounds__(256) rows8_kernel(VcrRows8 A, long long rows_in, long long numel, const int32_t* __restrict__ index) {
+    const long long blk = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (blk * VCR_OPT_BLOCK >= numel) return;
+    const uint32_t lane = threadIdx.x & 63;
+    const GLOBAL uint8_t *mc = global(A.m), *vc = global(A.v), *ms = global(A.m_scale), *vs = global(A.v_scale);
+    float m[4], v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const long long i = blk * VCR_OPT_BLOCK + lane + 64 * k;
+        m[k] = v[k] = 0.f;
+        if (i >= numel) continue;
+        const long long row = i / A.width, from = global(index)[row];
+        if (from < 0 || from >= rows_in) continue;
+        const long long e = from * A.width + (i - row * A.width);
+        m[k] = decode_m(mc[e], ms[e / VCR_OPT_BLOCK]);
+        v[k] = decode_v(vc[e], vs[e / VCR_OPT_BLOCK]);
+    }
+    encode_block(m, v, blk, lane, numel, global(A.m_out), global(A.v_out), global(A.m_scale_out), global(A.v_scale_out));
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
@@ -946,6 +974,33 @@ extern "C" int vcr_moments8_encode(int ntensors, const void* plan, const int64_t
                                    const float* const* exp_avg_sq, void* stream) {
     return pairs_call("vcr_moments8_encode", ntensors, plan, numel, (const void* const*)exp_avg, (const void* const*)exp_avg_sq, VCR_F32,
                       true, (hipStream_t)stream);
+}
+
+extern "C" int vcr_moments8_rows(int narrays, const VcrRows8* arrays, int64_t rows_in, int64_t rows_out, const int32_t* index, void* stream) {
+    if (narrays < 0 || (narrays > 0 && !arrays) || rows_in < 0 || rows_out < 0 || (rows_out > 0 && !index)) {
+        vcr_set_error("vcr_moments8_rows: inconsistent arguments");
+        return 1;
+    }
+    const int64_t most = (int64_t)VCR_OPT_LAUNCH_CHUNKS * VCR_OPT_CHUNK;
+    for (int k = 0; k < narrays; ++k) {
+        const VcrRows8& a = arrays[k];
+        if (a.width < 1 || rows_in > most / a.width || rows_out > most / a.width) {
+            vcr_set_error("vcr_moments8_rows: array %d has width %d, %lld rows -> %lld", k, a.width, (long long)rows_in, (long long)rows_out);
+            return 1;
+        }
+        if ((rows_in > 0 && (!a.m || !a.v || !a.m_scale || !a.v_scale)) || (rows_out > 0 && (!a.m_out || !a.v_out || !a.m_scale_out || !a.v_scale_out))) {
+            vcr_set_error("vcr_moments8_rows: array %d has a pointer missing", k);
+            return 1;
+        }
+    }
+    if (rows_out == 0) return 0;
+    for (int k = 0; k < narrays; ++k) {
+        const int64_t numel = rows_out * arrays[k].width;
+        hipLaunchKernelGGL(rows8_kernel, dim3((uint32_t)chunks_of(numel, 4 * VCR_OPT_BLOCK)), dim3(256), 0, (hipStream_t)stream, arrays[k], (long long)rows_in,
+                           (long long)numel, index);
+    }
+    VCR_HIP_CHECK(hipGetLastError());
+    return 0;
 }
 
 extern "C" int vcr_grad_norm_partials(int ntensors, const int64_t* numel) {

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .general_utils import build_rotation, get_expon_lr_func, inverse_sigmoid
-from .optim import AdamW
+from .optim import AdamW, rows8
 
 GROUPS = ["xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation", "obj_dc"]
 
@@ -717,7 +717,7 @@ class GaussianModel:
     def _move_rows(self, mask, mode, copies=1, reset_stats=True):
         """mode 0: keep the rows where `mask` (prune); mode 1: append `copies` copies of the rows where `mask` (clone /
         split), Adam moments of the appended rows zero.  Parameters, both moments and the densification statistics are
-        re-packed by `vcr_rows_plan` + `vcr_rows_move`; returns the number of selected rows."""
+        re-packed by `vcr_rows_plan` + `vcr_rows_move`, 8-bit moments by `vcr_moments8_rows`; returns the number of selected rows."""
         lib = _lib.load()
         dev, N = self.device, self._xyz.shape[0]
         m8 = mask.to(torch.uint8).contiguous()
@@ -727,10 +727,13 @@ class GaussianModel:
         M = int(plan[-1])                                   # the one host sync (the reference's boolean indexing has the same)
         newN = M if mode == 0 else N + copies * M
         items = []                                          # (setter, old tensor, zero_new)
+        packed = isinstance(self.optimizer, AdamW) and self.optimizer.state_bits == 8
         for g in self.optimizer.param_groups:
             if g.get("aux"):
                 continue
             items.append((("p", g), g["params"][0].detach(), False))
+            if packed:                                      # (8-bit moments move as codes, below)
+                continue
             mv = self._moments_of(g["name"])
             if mv is not None:
                 items.append((("m", g["name"]), mv[0], True))
@@ -763,6 +766,12 @@ class GaussianModel:
             else:
                 setattr(self, ref, out)
         self._set_params(new_params)
+        held = [self.optimizer.state[n] for n in new_params if n in self.optimizer.state] if packed else []
+        if held:
+            index = m8.nonzero().view(-1).int() if mode == 0 else torch.cat(
+                (torch.arange(N, dtype=torch.int32, device=dev), torch.full((copies * M,), -1, dtype=torch.int32, device=dev)))
+            for st8, new in zip(held, rows8(held, index)):
+                st8.update(new)
         if not keep_stats:
             self.xyz_gradient_accum = torch.zeros((newN, 1), device=dev)
             self.denom = torch.zeros((newN, 1), device=dev)

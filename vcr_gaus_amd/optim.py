@@ -733,3 +733,33 @@ def decode8(st):
         _lib.check(_on(dev, _lib.load().vcr_moments8_decode, 1, plan.data_ptr(), _address(ns), _address(m), _address(v), 0,
                        _lib.stream_of(st["exp_avg"])))
     return outs
+
+
+def rows8(states, index):
+    """8-bit moments with their rows (along the first dimension) in another order: for each of `states` (dicts as `decode8`'s, all of the
+    same number of rows) new tensors whose row r is row index[r] of the old ones; zeros where index[r] is no row (-1).  By code: blocks
+    are formed anew, to the nearest, and nothing is expanded on the way."""
+    if index.dtype != torch.int32 or index.dim() != 1 or not index.is_contiguous():
+        raise ValueError("rows8: `index` must be a contiguous vector of int32")
+    shapes = [st["exp_avg"].shape for st in states]
+    if any(len(s) == 0 or s[0] != shapes[0][0] or st["exp_avg_sq"].shape != s for st, s in zip(states, shapes)):
+        raise ValueError("rows8: moments of one number of rows, both of a parameter's shape, are needed")
+    arr, new = (_lib.VcrRows8 * len(states))(), []
+    for a, st, shape in zip(arr, states, shapes):
+        _check_codes(st)
+        if st["exp_avg"].device != index.device:
+            raise ValueError(f"rows8: moments on {st['exp_avg'].device}, `index` on {index.device}")
+        out = {k: torch.empty((index.numel(), *shape[1:]), dtype=torch.uint8, device=index.device) for k in ("exp_avg", "exp_avg_sq")}
+        blocks = -(-out["exp_avg"].numel() // BLOCK)
+        out.update({k: torch.empty(blocks, dtype=torch.uint8, device=index.device) for k in ("exp_avg_scale", "exp_avg_sq_scale")})
+        a.width = shape[1:].numel()
+        for k, i, o in (("exp_avg", "m", "m_out"), ("exp_avg_sq", "v", "v_out"), ("exp_avg_scale", "m_scale", "m_scale_out"),
+                        ("exp_avg_sq_scale", "v_scale", "v_scale_out")):
+            setattr(a, i, st[k].data_ptr())
+            setattr(a, o, out[k].data_ptr())
+        new.append(out)
+    live = [a for a in arr if a.width]                       # (rows without elements: nothing to move)
+    if live:
+        _lib.check(_on(index.device, _lib.load().vcr_moments8_rows, len(live), (_lib.VcrRows8 * len(live))(*live), shapes[0][0],
+                       index.numel(), index.data_ptr(), _stream(index.device.index)))
+    return new
