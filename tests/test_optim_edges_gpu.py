@@ -449,3 +449,24 @@ def test_row_surgery_does_not_expand_8_bit_moments(device):
         assert int(opt.state[k]["step"]) == steps[k]
     tr.train_step()
     assert int(opt.state["xyz"]["step"]) == steps["xyz"] + 1
+
+
+@pytest.mark.parametrize("optimizer", ["adam", "adamw"])
+def test_row_surgery_takes_32_bit_moments_over(device, optimizer):
+    """Beside the new parameters and moments (12 bytes a value) nothing of their size is made: the moved moments are the new ones."""
+    from tests.test_optim_gpu import GROUPS, adamw_trainer
+    tr = adamw_trainer(device, optimizer=optimizer)
+    tr.train_step()
+    tr.join_side()
+    m = tr.model
+    with torch.no_grad():
+        m._append_selected(torch.ones(m._xyz.shape[0], dtype=torch.bool, device=device), copies=39)
+        n = m._xyz.shape[0]
+        floats = sum(m.optimizer.state[k]["exp_avg"][0].numel() for k in GROUPS)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats(device)
+        held = torch.cuda.memory_allocated(device)
+        m.prune_points(torch.arange(n, device=device) % 7 == 0)
+    assert torch.cuda.max_memory_allocated(device) - held <= m._xyz.shape[0] * (floats * 12 + 64) + (1 << 20)
+    tr.train_step()
+    assert int(m.optimizer.state["xyz"]["step"]) == 2

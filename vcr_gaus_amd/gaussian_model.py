@@ -689,11 +689,11 @@ class GaussianModel:
         return st["exp_avg"], st["exp_avg_sq"]
 
     def _store_moments(self, name, m, v):
-        """The group's parameter has been replaced: these are its moments now (8 bits: to the nearest code)."""
-        if isinstance(self.optimizer, AdamW):
+        """The group's parameter has been replaced: these new tensors are its moments now (8 bits: to the nearest code)."""
+        if isinstance(self.optimizer, AdamW) and self.optimizer.state_bits == 8:
             self.optimizer.set_moments(name, m, v)
         else:
-            self.optimizer.state[name]["exp_avg"], self.optimizer.state[name]["exp_avg_sq"] = m, v
+            self.optimizer.state[name].update(exp_avg=m, exp_avg_sq=v)
 
     def _set_params(self, new):
         for name, attr in self._param_table().items():
