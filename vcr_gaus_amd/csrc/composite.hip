@@ -15,7 +15,7 @@
 namespace {
 
 // Reduce 16 per-lane values (8 pairs) over the wave with a halving butterfly: v_permlane32_swap / v_permlane16_swap
-// exchange half of the live values per step (8+4 swaps, the sums as packed adds), then 4 row rotations finish the
+// exchange half of the live values per step (8+4 swaps, the sums in pairs), then 4 row rotations finish the
 // remaining 4.  On return lane l holds, in out[0..3], the wave totals of slots 8*(l>>5) + 4*((l>>4)&1) + 0..3
 // (slot 2j = v[j].x, slot 2j+1 = v[j].y).
 __device__ __forceinline__ void wave_reduce16(const f2 v[8], float out[4]) {

@@ -83,8 +83,8 @@ __device__ __forceinline__ bool tile_touch(float4 q0, float4 q1, int tx, int ty)
 
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// Packed fp32 (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32 issue two fp32 lanes-worth per instruction on CDNA3/4):
-// the shading loops are VALU-issue-bound, so everything that comes in natural pairs is written on this type.
+// What comes in natural pairs in the shading loops is written on this type.  It compiles to single fp32 instructions (the build switches
+// packed fp32 off); packed ones would issue two results at a time, 4 % of the compositing forward's time.
 __device__ __forceinline__ f2 pk_fma(f2 a, f2 b, f2 c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f2 splat(float x) { return f2{x, x}; }
 

@@ -388,7 +388,7 @@ struct GaussWin { float w[11]; };
 // window is evaluated separably with REGISTER sliding windows: every lane produces 4 adjacent outputs in the horizontal pass (14
 // loaded values feed 4 x 11 taps) and TY / 8 in the vertical pass, ~3x fewer LDS reads per output pixel than the one-output-per-
 // lane form (LDS-bound: 84 us at 1080p).  The five window sums travel in natural pairs -- (a, b), (a^2, b^2) and a b alone --
-// on packed fp32 (v_pk_fma_f32: 3 instructions per tap instead of 5; the kernel is VALU-bound).  Zero padding as
+// though as single fp32 instructions (the build switches packed fp32 off; the kernel is VALU-bound).  Zero padding as
 // F.conv2d(padding=5).
 // sums[0] += sum |a-b| ; sums[1] += sum ssim_map.  If `part` != null stores d ssim / d{mu1, sigma1^2, sigma12}.
 typedef float lf2 __attribute__((ext_vector_type(2)));
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(256) l1_ssim_fwd_kernel(int H, int W, GaussWin
 }
 
 // dimg1(p) = gl1 * sign(a-b) + gss * sum_q w(q-p) [ dm1(q) + 2 a(p) dq11(q) + b(p) dq12(q) ]      (same tiling; the three
-// planes as one packed pair + one scalar)
+// planes as one pair + one scalar)
 template <int TY>
 __global__ void __launch_bounds__(256) l1_ssim_bwd_kernel(int H, int W, GaussWin gw, const float* __restrict__ img1,
                                                           const float* __restrict__ img2, const float* __restrict__ part,
