@@ -470,3 +470,44 @@ def test_row_surgery_takes_32_bit_moments_over(device, optimizer):
     assert torch.cuda.max_memory_allocated(device) - held <= m._xyz.shape[0] * (floats * 12 + 64) + (1 << 20)
     tr.train_step()
     assert int(m.optimizer.state["xyz"]["step"]) == 2
+
+
+@pytest.mark.parametrize("bits, dtype, master", [(32, F, False), (8, F, False), (8, BF, True), (32, HF, False)])
+def test_a_captured_training_tail(device, bits, dtype, master):
+    """Clipping in place, a clipped step, its moments into given tensors: one graph, replayed between eager work; every replay gives the bits
+    of the same eager calls."""
+    from vcr_gaus_amd.optim import AdamW, clip_grad_norm_
+    twins = []
+    for _ in range(2):
+        params, _ = make([5, 4097, 0, 70001], dtype, device, seed=120, grad=1.0)
+        opt = AdamW(params, state_bits=bits, master_weights=master, seed=3)
+        opt.step()
+        outs = [[torch.zeros(p.shape, device=device) for p in params] for _ in range(2)]
+        twins.append((params, opt, outs))
+
+    def tail(params, opt, outs):
+        a = clip_grad_norm_(params, 2.0)
+        b = opt.step(max_norm=0.5)
+        opt.moments(*outs)
+        return a, b
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norms = tail(*twins[0])
+    g = torch.Generator(device=device).manual_seed(4)
+    for r in range(4):
+        for p, q in zip(twins[0][0], twins[1][0]):
+            p.grad.copy_(torch.randn(p.shape, device=device, generator=g))
+            q.grad.copy_(p.grad)
+        graph.replay()
+        want = tail(*twins[1])
+        torch.cuda.synchronize()
+        junk = torch.randn(1 << 20, device=device).sum()
+        assert all(torch.equal(x, y) for x, y in zip(norms, want)), r
+        for (p, q) in zip(twins[0][0], twins[1][0]):
+            assert torch.equal(p, q) and torch.equal(p.grad, q.grad), r
+        for x, y in zip(twins[0][2][0] + twins[0][2][1], twins[1][2][0] + twins[1][2][1]):
+            assert torch.equal(x, y), r
+        del junk
+    assert [int(st["step"]) for st in twins[0][1].state.values()] == [5] * 4
