@@ -471,9 +471,10 @@ __device__ __forceinline__ Fast fast_of(const Coef& c) {
 // A whole block of finite numbers of ordinary size: the definition above with its scalings as multiplications by powers of two
 // (exact, so that b2 and the scale of v are one factor), the first moment's codes decoded by the hardware (they are OCP e4m3:
 // bias 7, code exponent 14 = 2^7), and everything shifted up by 4 so that a code is the top byte of its word.  Returns false, with
-// nothing changed, where it does not apply: a code or a moment that is not finite, block exponents out of the ranges above, or, where
-// eps is small enough for it to be seen (`guard`), a second moment below 2^-126, which the square root instruction would flush.  Its 150 vector instructions, of 190 a block in all, are what
-// bounds the update of 16-bit parameters: in 90 % of the cycles one is at work.
+// nothing changed, where it does not apply: a code or a moment that is not finite, block exponents out of the ranges above, or,
+// where eps is small enough for it to be seen (`guard`), a second moment below 2^-126, which the square root instruction would
+// flush.  Its 154 vector instructions, of 196 a block in all, are what bounds the update of 16-bit parameters without masters: in
+// 95 % of the cycles one is at work (with masters in 54 %).
 __device__ __forceinline__ bool block_fast(Lane8& r, int& sm, int& sv, uint32_t bkey, const uint32_t (&j_step)[4], float gs, const Coef& c,
                                            const Fast& f) {
 #pragma clang fp contract(off)
@@ -563,8 +564,9 @@ template <typename T> struct Block8 {
 };
 template <typename T, bool MASTER>
 __device__ __forceinline__ Lane8 load_block(const Block8<T>& b, uint32_t j0) {
-    // (measured both ways: with the non-temporal kind 302 M bf16 elements take 523 instead of 564 us, but fp32 ones, 295 M, 776 instead
-    //  of 752, and bf16 ones with masters 821 instead of 803)
+    // (measured both ways in turn on one card, which the kept forms are not alike on: with the non-temporal kind 302 M bf16 elements take
+    //  523 instead of 564 us, but fp32 ones, 295 M, 776 instead of 752, and bf16 ones with masters 821 instead of 803; on others the
+    //  kept forms take up to 597 and 821 us)
     constexpr bool NT = sizeof(T) == 2 && !MASTER;
     Lane8 r = {};
     if (b.whole) {
@@ -607,7 +609,7 @@ __device__ __forceinline__ void store_block(const Block8<T>& b, uint32_t j0, con
 // Blocks of a wave, one after another.  What every wave does once (addresses, factors) is a third of its instructions with one block:
 // 16-bit parameters without masters (10 bytes an element) are bound by instructions and take four (302 M elements 731, 601, 524 us
 // with 1, 2, 4 blocks), with masters two (19 M elements in odd sizes 57.5, 49.4, 51.0 us); fp32 (16 bytes) is bound by memory, which
-// favours short runs of a workgroup, and takes one (295 M elements 772, 777, 840 us).
+// favours short runs of a workgroup, and takes one (295 M elements 772, 777, 840 us).  Each of these sets on one card, in turn.
 template <typename T, bool MASTER> constexpr int blocks8() { return sizeof(T) == 4 ? 1 : MASTER ? 2 : 4; }
 template <typename T, bool MASTER>
 __global__ void __launch_bounds__(VCR_OPT_THREADS) adamw8_kernel(const VcrOptimTensor* __restrict__ tensors, const uint2* __restrict__ chunks,

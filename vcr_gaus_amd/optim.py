@@ -114,7 +114,8 @@ def grad_norm(tensors, out=None):
 def clip_grad_norm_(parameters, max_norm):
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)), norm their 2-norm over all; -> norm (a 0-dim
     float32 tensor; nothing waits for it).  For optimizers that take gradients as they are; `AdamW.step(max_norm=...)` applies the
-    factor inside the update instead, without writing the gradients again."""
+    factor inside the update instead, without writing the gradients again.  Gradients must not share memory, with each other or (expanded
+    ones) with themselves."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = _positive(max_norm, "max_norm")
     grads = [p.grad for p in parameters]
@@ -191,7 +192,7 @@ class _Plan:
 
 class AdamW:
     """AdamW over any number of tensors (a list, or groups: dicts with `params` and optionally `name`, `lr`, `betas`, `eps`,
-    `weight_decay`), updated in one launch per 400 tensors of a type:
+    `weight_decay`), updated in one launch per 352 tensors and 14 groups of a type:
 
         m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2;  p <- p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
@@ -205,9 +206,14 @@ class AdamW:
     parameter that is changed from outside between steps does not change its master: delete `state[key]["master"]`, and the
     next step takes it from the parameter again.
     Parameters must be contiguous; gradients of another layout are copied.  Tensors without a gradient are skipped, and so are
-    their counters, as in torch.  Memory: plan and state belong to the optimizer; a captured step keeps its plan alive (and holds
-    the rates of its groups as they were, but for those given as device scalars).  One optimizer's steps are one sequence: two that
-    run at the same time on two streams, or two of its captured graphs replayed so, race on the parameters."""
+    their counters, as in torch.  A tensor of the state, or of the parameters, may be replaced, also its storage under it (`.data = `,
+    `set_`): the next step sees it and looks at its tensors anew, which costs host work and one wait for the stream and cannot be
+    captured.  Tensors that a step would write must not share memory.  `seed` and the groups' rates may be changed at any time;
+    `state_bits` and `master_weights` are fixed.
+    Memory: plan and state belong to the optimizer, which must live as long as graphs of its steps are replayed; a captured step writes
+    the storages it was captured with (and holds the rates of its groups as they were, but for those given as device scalars).  One
+    optimizer's steps are one sequence: two that run at the same time on two streams, or two of its captured graphs replayed so,
+    race on the parameters."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False, seed=0):
         params = list(params)
@@ -515,8 +521,8 @@ class AdamW:
     # ---- moments as values ---------------------------------------------------------------------------------------------
     def moments(self, exp_avgs=None, exp_avg_sqs=None, dtype=torch.float32):
         """The moments as values, whatever they are held in: two lists, one tensor for each parameter in the groups' order.  Given
-        lists are written to (contiguous, all of one type) instead of new tensors of `dtype`; a parameter that has not been stepped
-        yet has zeros.  8-bit moments are exact in bfloat16."""
+        lists are written to (contiguous, all of one type, sharing no memory) instead of new tensors of `dtype`; a parameter that has not
+        been stepped yet has zeros.  8-bit moments are exact in bfloat16."""
         params, native = self._tensors(), _native()
         n, none = len(params), bytes(len(params))
         for given in (exp_avgs, exp_avg_sqs):
@@ -618,7 +624,8 @@ class AdamW:
     def load_state_dict(self, sd):
         """Takes what `state_dict()` gave -- or torch.optim.AdamW's: float moments are rounded into the 8-bit form where this optimizer
         has that, and 8-bit ones expanded where it has not.  Tensors that already have this optimizer's type, layout and device are
-        kept, not copied, as torch does.  Groups are matched in order."""
+        kept, not copied, as torch does; a rate that is a tensor is copied.  Groups are matched in order, shapes must be the parameters'.
+        Files of torch's `amsgrad` and `maximize` variants are refused."""
         if len(sd["param_groups"]) != len(self.param_groups):
             raise ValueError(f"AdamW: {len(sd['param_groups'])} groups saved, {len(self.param_groups)} here")
         order = []
