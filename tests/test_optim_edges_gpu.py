@@ -120,6 +120,7 @@ def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits, loaded):
     sizes = [t.numel() * t.element_size() for t in opt.state["0"].values()]
     old = {t.data_ptr() for t in opt.state["0"].values() if t.numel() > 1 << 20}
     before = [t.clone() for t in (params[0], *opt.state["0"].values())]
+    torch.full((16,), 7, dtype=torch.uint8, device=device)            # (its kernel is loaded)
     held = torch.cuda.memory_allocated(device)
     side = torch.cuda.Stream(device)
     side.wait_stream(torch.cuda.current_stream(device))
@@ -130,7 +131,7 @@ def test_memory_goes_with_the_optimizer_and_no_sooner(device, bits, loaded):
         with torch.cuda.stream(side):
             if loaded:
                 opt.moments()                          # (builds the plan, and waits for this stream once)
-            torch.cuda._sleep(50_000_000)             # (tens of milliseconds)
+            torch.cuda._sleep(200_000_000)            # (of the order of 100 ms)
             opt.step()
         waiting = not side.query()
         del opt
